@@ -1,0 +1,433 @@
+// Dense layer batched over models (gfx950): y[g] = act(x[g] w[g] + b[g]) + r[g] and its gradients, any size, fp32 / bf16 /
+// fp16, ragged row counts, one input shared by all models.  include/mplc_hip_ops.h states the operator.
+//
+// All three products run on the tiled core of mma.h without a copy or a transposition of an operand:
+//   forward  y  [row][out] = sum over in  of x[row][in]  w[in][out]    A along r, B across r
+//   dx          [row][in]  = sum over out of dz[row][out] w[in][out]   A along r, B along r
+//   dw          [in][out]  = sum over row of x[row][in]  dz[row][out]  A across r, B across r
+// A shared input's dx sums over the models inside the same product: r runs over (model, out).
+//
+// Few tiles and a long sum (a training batch's rows against 9216 inputs): r is split over workgroups, the fp32 partial
+// sums go through the workspace and a second kernel adds them in order and applies the epilogue.
+//
+// act'(z) needs dz as an operand of two products: one pass computes it, rounds it to the operands' type and sums its
+// columns (db) on the way, in fp32, per 128 rows, the blocks of rows added in order.
+#include <math.h>
+
+#include "mma.h"
+#include "mplc_hip.h"
+#include "xcd.h"
+
+namespace {
+
+using namespace mma;
+
+struct Epilogue {
+  const void* bias;
+  int64_t bias_stride;
+  const void* res;
+  int64_t res_stride, res_ld;
+  void* out;
+  int64_t out_stride, out_ld;
+  float* z;
+  int64_t z_stride, z_ld;
+  int act;
+};
+
+struct Product {
+  const void* a;
+  int64_t a_stride, a_ld;
+  const void* b;
+  int64_t b_stride, b_ld;
+  int m, n, r;           // sizes of one model's product
+  int models, segments;  // segments > 1: one product, r runs over (model, r)
+  const int32_t* counts;
+  int count_is_r;        // counts limit r (dw), not m
+  int tiles_m, tiles_n, nk, splits, per_split;
+  float* partial;        // [split][model][m][n] where splits > 1
+};
+
+__device__ __forceinline__ int count_of(const int32_t* counts, int g, int most) {
+  if (counts == nullptr) return most;
+  const int c = counts[g];
+  return c < 0 ? 0 : (c > most ? most : c);
+}
+
+// a finite z far in the negative tail gives 0, so -infinity does too
+__device__ __forceinline__ float activate(int act, float z) {
+  switch (act) {
+    case MPLC_ACT_RELU: return z < 0.f ? 0.f : z;
+    case MPLC_ACT_GELU: return z < -64.f ? 0.f : 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case MPLC_ACT_SILU: return z < -1e4f ? 0.f : z / (1.f + __expf(-z));
+    default: return z;
+  }
+}
+__device__ __forceinline__ float slope(int act, float z) {
+  switch (act) {
+    case MPLC_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+    case MPLC_ACT_GELU:
+      if (fabsf(z) > 64.f) return z > 0.f ? 1.f : 0.f;
+      return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+    case MPLC_ACT_SILU: {
+      if (fabsf(z) > 1e4f) return z > 0.f ? 1.f : 0.f;
+      const float s = 1.f / (1.f + __expf(-z));
+      return s * (1.f + z * (1.f - s));
+    }
+    default: return 1.f;
+  }
+}
+
+// z of 4 columns n .. of row m of model g -> z, y
+template <Kind K> __device__ __forceinline__ void finish(const Epilogue& e, int g, int m, int n, int N, f32x4 v) {
+  typedef typename Elem<K>::T T;
+  const int valid = N - n;
+  if (e.bias) v += load4<K>(reinterpret_cast<const T*>(e.bias) + g * e.bias_stride + n, valid);
+  if (e.z) store4<F32>(e.z + g * e.z_stride + m * e.z_ld + n, v, valid);
+  if (e.act != MPLC_ACT_NONE)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = activate(e.act, v[i]);
+  if (e.res) v += load4<K>(reinterpret_cast<const T*>(e.res) + g * e.res_stride + m * e.res_ld + n, valid);
+  store4<K>(reinterpret_cast<T*>(e.out) + g * e.out_stride + m * e.out_ld + n, v, valid);
+}
+
+// Tile order of one product: 8 tile rows at a time, column by column, so that the workgroups in flight on an XCD share
+// their rows of A and columns of B in its L2.
+__device__ __forceinline__ void tile_of(int idx, int tm, int tn, int& m, int& n) {
+  const int band = idx / (8 * tn), first = band * 8;
+  const int size = tm - first < 8 ? tm - first : 8;
+  const int in = idx - band * 8 * tn;
+  m = first + in % size;
+  n = in / size;
+}
+
+template <Kind K, bool AA, bool BA, int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, const Epilogue e) {
+  typedef typename Elem<K>::T T;
+  typedef Block<K, AA, BA, WM, WN, FM, FN, 128, 1> B;
+  __shared__ __attribute__((aligned(16))) char lds[B::LDS_BYTES];
+  int64_t b = xcd_block();
+  const int tiles = p.tiles_m * p.tiles_n;
+  int tm, tn;
+  tile_of((int)(b % tiles), p.tiles_m, p.tiles_n, tm, tn);
+  b /= tiles;
+  const int split = (int)(b % p.splits), g = (int)(b / p.splits);
+  const int m0 = tm * B::BM, n0 = tn * B::BN;
+  const bool seg = p.segments > 1;
+  const int cnt = seg ? p.m : count_of(p.counts, g, p.count_is_r ? p.r : p.m);
+  const int M = p.count_is_r ? p.m : cnt, R = p.count_is_r ? cnt : p.r;
+  if (m0 >= M) return;
+  const int nk = seg ? p.nk : (R + B::BK - 1) / B::BK;
+  const int all = seg ? p.segments * nk : nk;
+  const int first = split * p.per_split, last = min(all, first + p.per_split);
+  const T* pa = reinterpret_cast<const T*>(p.a) + g * p.a_stride;
+  const T* pb = reinterpret_cast<const T*>(p.b) + g * p.b_stride;
+  B blk;
+  blk.clear();
+  blk.run(lds, m0, n0, last - first, [&](int it, Operand<T>& a, Operand<T>& o, int& r0, int& rend) {
+    it += first;
+    const int s = seg ? it / nk : 0;
+    a.p[0] = pa + s * p.a_stride;
+    o.p[0] = pb + s * p.b_stride;
+    a.ld = p.a_ld;
+    o.ld = p.b_ld;
+    a.rows = seg ? count_of(p.counts, s, p.m) : M;
+    o.rows = p.n;
+    r0 = (it - s * nk) * B::BK;
+    rend = R;
+  });
+  if (p.splits > 1) {
+    float* out = p.partial + ((int64_t)split * p.models + g) * p.m * p.n;
+    blk.each(m0, n0, [&](int m, int n, f32x4 v) {
+      if (m < M && n < p.n) store4<F32>(out + (int64_t)m * p.n + n, v, p.n - n);
+    });
+  } else {
+    blk.each(m0, n0, [&](int m, int n, f32x4 v) {
+      if (m < M && n < p.n) finish<K>(e, g, m, n, p.n, v);
+    });
+  }
+}
+
+// adds the partial sums of one product in order and finishes it
+template <Kind K> __global__ __launch_bounds__(256) void join_kernel(const Product p, const Epilogue e) {
+  const int n4 = (p.n + 3) >> 2;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= (int64_t)p.m * n4) return;
+  const int g = blockIdx.y, m = (int)(t / n4), n = (int)(t % n4) * 4;
+  if (!p.count_is_r && p.segments == 1 && m >= count_of(p.counts, g, p.m)) return;
+  const float* src = p.partial + (int64_t)g * p.m * p.n + (int64_t)m * p.n + n;
+  const int64_t step = (int64_t)p.models * p.m * p.n;
+  f32x4 v = load4<F32>(src, p.n - n);
+  for (int s = 1; s < p.splits; ++s) v += load4<F32>(src + s * step, p.n - n);
+  finish<K>(e, g, m, n, p.n, v);
+}
+
+constexpr int DZ_ROWS = 128;  // rows summed by one workgroup
+
+// dz = dy act'(z) and the sums of its columns over DZ_ROWS rows
+template <Kind K>
+__global__ __launch_bounds__(256) void dz_kernel(const void* dy_, int64_t dy_stride, int64_t dy_ld, const float* z,
+                                                 int64_t z_stride, int64_t z_ld, int act, int rows, int n,
+                                                 const int32_t* counts, void* dz_, int dz_ld, float* sums, void* db_,
+                                                 int64_t db_stride) {
+  typedef typename Elem<K>::T T;
+  __shared__ f32x4 part[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = blockIdx.z, c = (blockIdx.x * 64 + lane) * 4;
+  const int cnt = count_of(counts, g, rows);
+  const int r0 = blockIdx.y * DZ_ROWS, r1 = min(cnt, r0 + DZ_ROWS);
+  const T* dy = reinterpret_cast<const T*>(dy_) + g * dy_stride;
+  T* dz = dz_ ? reinterpret_cast<T*>(dz_) + (int64_t)g * rows * dz_ld : nullptr;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  if (c < n)
+    for (int r = r0 + wave; r < r1; r += 4) {
+      f32x4 d = load4<K>(dy + r * dy_ld + c, n - c);
+      if (act != MPLC_ACT_NONE) {
+        const f32x4 zz = load4<F32>(z + g * z_stride + r * z_ld + c, n - c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] *= slope(act, zz[i]);
+        if (dz) store4<K>(dz + (int64_t)r * dz_ld + c, d, n - c);
+      }
+      sum += d;
+    }
+  if (sums == nullptr && db_ == nullptr) return;
+  part[wave][lane] = sum;
+  __syncthreads();
+  if (wave == 0 && c < n) {
+    f32x4 v = part[0][lane] + part[1][lane];
+    v += part[2][lane] + part[3][lane];
+    if (sums) store4<F32>(sums + ((int64_t)g * gridDim.y + blockIdx.y) * n + c, v, n - c);
+    else store4<K>(reinterpret_cast<T*>(db_) + g * db_stride + c, v, n - c);
+  }
+}
+
+template <Kind K>
+__global__ __launch_bounds__(256) void db_kernel(const float* sums, int blocks, int n, int used_rows,
+                                                 const int32_t* counts, void* db_, int64_t db_stride) {
+  typedef typename Elem<K>::T T;
+  const int g = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= n) return;
+  const int cnt = count_of(counts, g, used_rows);
+  const int nb = min(blocks, (cnt + DZ_ROWS - 1) / DZ_ROWS);
+  float v = 0.f;
+  for (int i = 0; i < nb; ++i) v += sums[((int64_t)g * blocks + i) * n + c];
+  reinterpret_cast<T*>(db_)[g * db_stride + c] = from_f32<K>(v);
+}
+
+// ---------------------------------------------------------------------------------------------- host
+enum Form { FORWARD, DX, DW };
+
+struct Plan {
+  int cfg;  // 0: 128 x 128, 1: 64 x 64, 2: 32 x 128
+  Product p;
+  int64_t blocks;
+  size_t partial_bytes;
+};
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tile and split of one product.
+bool plan(const mplc_dense_t& t, Form form, Plan& out) {
+  Product p = {};
+  const bool shared_dx = form == DX && t.x_shared;
+  p.models = shared_dx ? 1 : t.n_models;
+  p.segments = shared_dx ? t.n_models : 1;
+  p.m = form == DW ? t.in : t.rows;
+  p.n = form == DX ? t.in : t.out;
+  p.r = form == FORWARD ? t.in : form == DX ? t.out : t.rows;
+  p.counts = t.counts;
+  p.count_is_r = form == DW;
+  const int bk = t.dtype == MPLC_DTYPE_F32 ? 32 : 64;
+  p.nk = (int)ceil_div(p.r, bk);
+  const int64_t big = ceil_div(p.m, 128) * ceil_div(p.n, 128) * p.models;
+  out.cfg = p.m <= 32 ? 2 : big >= 256 ? 0 : (p.m <= 64 || p.n <= 64 || big < 128) ? 1 : 0;
+  const int bm = out.cfg == 0 ? 128 : out.cfg == 1 ? 64 : 32, bn = out.cfg == 1 ? 64 : 128;
+  p.tiles_m = (int)ceil_div(p.m, bm);
+  p.tiles_n = (int)ceil_div(p.n, bn);
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.models;
+  const int64_t all = (int64_t)p.nk * p.segments;
+  int64_t splits = 1;
+  if (tiles < 512) {  // two workgroups per CU, at least 4 tiles of r each
+    splits = ceil_div(512, tiles > 0 ? tiles : 1);
+    if (splits > all / 4) splits = all / 4;
+    if (splits > 64) splits = 64;
+    if (splits < 1) splits = 1;
+  }
+  p.per_split = (int)ceil_div(all, splits);
+  p.splits = p.per_split > 0 ? (int)ceil_div(all, p.per_split) : 1;
+  if (p.splits < 1) p.splits = 1;
+  if (all > INT32_MAX || tiles * p.splits > (1 << 23)) return false;
+  out.blocks = tiles * p.splits;
+  out.partial_bytes = p.splits > 1 ? (size_t)p.splits * p.models * p.m * p.n * sizeof(float) : 0;
+  out.p = p;
+  return true;
+}
+
+template <Kind K, bool AA, bool BA> hipError_t launch(const Plan& pl, const Epilogue& e, hipStream_t s) {
+  const dim3 grid((unsigned)pl.blocks);
+  if (pl.cfg == 0) product_kernel<K, AA, BA, 2, 2, 2, 2><<<grid, 256, 0, s>>>(pl.p, e);
+  else if (pl.cfg == 1) product_kernel<K, AA, BA, 2, 2, 1, 1><<<grid, 256, 0, s>>>(pl.p, e);
+  else product_kernel<K, AA, BA, 1, 4, 1, 1><<<grid, 256, 0, s>>>(pl.p, e);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess || pl.p.splits == 1) return err;
+  const dim3 jg((unsigned)ceil_div((int64_t)pl.p.m * ((pl.p.n + 3) / 4), 256), (unsigned)pl.p.models);
+  join_kernel<K><<<jg, 256, 0, s>>>(pl.p, e);
+  return hipGetLastError();
+}
+
+size_t align16(size_t v) { return (v + 15) & ~(size_t)15; }
+
+bool sizes_ok(const mplc_dense_t& t) {
+  if (t.n_models < 0 || t.rows < 0 || t.in < 1 || t.out < 1) return false;
+  if (t.dtype < 0 || t.dtype > 2 || t.activation < 0 || t.activation > 3) return false;
+  return t.n_models <= 65535;
+}
+// a tensor of [models][rows][cols]: rows may not overlap one another
+bool view_ok(const void* p, int64_t ld, int cols) { return p != nullptr && ld >= cols; }
+
+struct BackwardSpace {
+  Plan dx, dw;
+  size_t dz, sums, partial, total;
+  int dz_ld, blocks;
+};
+
+bool backward_space(const mplc_dense_t& t, BackwardSpace& s) {
+  s = BackwardSpace{};
+  const size_t size = t.dtype == MPLC_DTYPE_F32 ? 4 : 2;
+  s.dz_ld = (t.out + 7) & ~7;
+  s.blocks = (int)ceil_div(t.rows, DZ_ROWS);
+  if ((t.dx || t.dw) && t.activation != MPLC_ACT_NONE)
+    s.dz = align16((size_t)t.n_models * t.rows * s.dz_ld * size);
+  if (t.db && s.blocks > 1) s.sums = align16((size_t)t.n_models * s.blocks * t.out * sizeof(float));
+  size_t partial = 0;
+  if (t.dx) {
+    if (!plan(t, DX, s.dx)) return false;
+    partial = s.dx.partial_bytes;
+  }
+  if (t.dw) {
+    if (!plan(t, DW, s.dw)) return false;
+    partial = partial > s.dw.partial_bytes ? partial : s.dw.partial_bytes;
+  }
+  s.partial = align16(partial);  // dx's partial sums are joined before dw's are written: one place for both
+  s.total = s.dz + s.sums + s.partial;
+  return s.blocks <= 65535;
+}
+
+template <Kind K> int forward(const mplc_dense_t& t, const Plan& pl0, hipStream_t s) {
+  Plan pl = pl0;
+  pl.p.a = t.x;
+  pl.p.a_stride = t.x_shared ? 0 : t.x_stride;
+  pl.p.a_ld = t.x_ld;
+  pl.p.b = t.w;
+  pl.p.b_stride = t.w_stride;
+  pl.p.b_ld = t.w_ld;
+  pl.p.partial = reinterpret_cast<float*>(t.workspace);
+  Epilogue e = {t.bias, t.bias_stride, t.residual, t.residual_stride, t.residual_ld, t.y, t.y_stride, t.y_ld,
+                t.z, t.z_stride, t.z_ld, t.activation};
+  return (int)launch<K, false, true>(pl, e, s);
+}
+
+template <Kind K> int backward(const mplc_dense_t& t, BackwardSpace& sp, hipStream_t s) {
+  char* ws = reinterpret_cast<char*>(t.workspace);
+  void* dz = sp.dz ? ws : nullptr;
+  float* sums = sp.sums ? reinterpret_cast<float*>(ws + sp.dz) : nullptr;
+  float* partial = reinterpret_cast<float*>(ws + sp.dz + sp.sums);
+  hipError_t err;
+  if (dz || t.db) {
+    const dim3 grid((unsigned)ceil_div(t.out, 256), (unsigned)(sp.blocks ? sp.blocks : 1), (unsigned)t.n_models);
+    dz_kernel<K><<<grid, 256, 0, s>>>(t.dy, t.dy_stride, t.dy_ld, t.z, t.z_stride, t.z_ld, t.activation, t.rows, t.out,
+                                      t.counts, dz, sp.dz_ld, sums, sums ? nullptr : t.db, t.db_stride);
+    if ((err = hipGetLastError()) != hipSuccess) return (int)err;
+    if (sums) {
+      db_kernel<K><<<dim3((unsigned)ceil_div(t.out, 256), (unsigned)t.n_models), 256, 0, s>>>(
+          sums, sp.blocks, t.out, t.rows, t.counts, t.db, t.db_stride);
+      if ((err = hipGetLastError()) != hipSuccess) return (int)err;
+    }
+  }
+  const void* d = dz ? dz : t.dy;
+  const int64_t d_stride = dz ? (int64_t)t.rows * sp.dz_ld : t.dy_stride, d_ld = dz ? sp.dz_ld : t.dy_ld;
+  if (t.dx && t.rows > 0) {
+    Plan& pl = sp.dx;
+    pl.p.a = d;
+    pl.p.a_stride = d_stride;
+    pl.p.a_ld = d_ld;
+    pl.p.b = t.w;
+    pl.p.b_stride = t.w_stride;
+    pl.p.b_ld = t.w_ld;
+    pl.p.partial = partial;
+    Epilogue e = {};
+    e.out = t.dx;
+    e.out_stride = t.x_shared ? 0 : t.dx_stride;
+    e.out_ld = t.dx_ld;
+    if ((err = launch<K, false, false>(pl, e, s)) != hipSuccess) return (int)err;
+  }
+  if (t.dw) {
+    Plan& pl = sp.dw;
+    pl.p.a = t.x;
+    pl.p.a_stride = t.x_shared ? 0 : t.x_stride;
+    pl.p.a_ld = t.x_ld;
+    pl.p.b = d;
+    pl.p.b_stride = d_stride;
+    pl.p.b_ld = d_ld;
+    pl.p.partial = partial;
+    Epilogue e = {};
+    e.out = t.dw;
+    e.out_stride = t.dw_stride;
+    e.out_ld = t.dw_ld;
+    if ((err = launch<K, true, true>(pl, e, s)) != hipSuccess) return (int)err;
+  }
+  return MPLC_OK;
+}
+
+}  // namespace
+
+extern "C" size_t mplc_dense_forward_workspace_bytes(const mplc_dense_t* t) {
+  Plan pl;
+  if (t == nullptr || !sizes_ok(*t) || !plan(*t, FORWARD, pl)) return 0;
+  return pl.partial_bytes;
+}
+
+extern "C" size_t mplc_dense_backward_workspace_bytes(const mplc_dense_t* t) {
+  BackwardSpace s;
+  if (t == nullptr || !sizes_ok(*t) || !backward_space(*t, s)) return 0;
+  return s.total;
+}
+
+extern "C" int mplc_dense_forward(const mplc_dense_t* t, void* stream) {
+  if (t == nullptr || !sizes_ok(*t)) return MPLC_E_ARG;
+  if (t->n_models == 0 || t->rows == 0) return MPLC_OK;
+  if (!view_ok(t->x, t->x_ld, t->in) || !view_ok(t->w, t->w_ld, t->out) || !view_ok(t->y, t->y_ld, t->out))
+    return MPLC_E_ARG;
+  if ((t->residual && t->residual_ld < t->out) || (t->z && t->z_ld < t->out)) return MPLC_E_ARG;
+  Plan pl;
+  if (!plan(*t, FORWARD, pl)) return MPLC_E_SHAPE;
+  if (pl.partial_bytes && (t->workspace == nullptr || t->workspace_bytes < pl.partial_bytes)) return MPLC_E_WORKSPACE;
+  if (((uintptr_t)t->workspace & 15) != 0) return MPLC_E_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  if (t->dtype == MPLC_DTYPE_F32) return forward<F32>(*t, pl, s);
+  if (t->dtype == MPLC_DTYPE_BF16) return forward<BF16>(*t, pl, s);
+  return forward<F16>(*t, pl, s);
+}
+
+extern "C" int mplc_dense_backward(const mplc_dense_t* t, void* stream) {
+  if (t == nullptr || !sizes_ok(*t)) return MPLC_E_ARG;
+  if (t->n_models == 0) return t->x_shared && t->dx && t->rows > 0 ? MPLC_E_SHAPE : MPLC_OK;
+  if (t->rows > 0) {
+    if (!view_ok(t->dy, t->dy_ld, t->out)) return MPLC_E_ARG;
+    if (t->activation != MPLC_ACT_NONE && !view_ok(t->z, t->z_ld, t->out)) return MPLC_E_ARG;
+    if (t->dx && (!view_ok(t->w, t->w_ld, t->out) || t->dx_ld < t->in)) return MPLC_E_ARG;
+    if (t->dw && !view_ok(t->x, t->x_ld, t->in)) return MPLC_E_ARG;
+  }
+  if (t->dw && t->dw_ld < t->out) return MPLC_E_ARG;
+  BackwardSpace sp;
+  if (!backward_space(*t, sp)) return MPLC_E_SHAPE;
+  if (sp.total && (t->workspace == nullptr || t->workspace_bytes < sp.total)) return MPLC_E_WORKSPACE;
+  if (((uintptr_t)t->workspace & 15) != 0) return MPLC_E_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  if (t->dtype == MPLC_DTYPE_F32) return backward<F32>(*t, sp, s);
+  if (t->dtype == MPLC_DTYPE_BF16) return backward<BF16>(*t, sp, s);
+  return backward<F16>(*t, sp, s);
+}
+
+extern "C" int64_t mplc_ops_layout(int what) {
+  return what == 0 ? (int64_t)sizeof(mplc_dense_t) : what == 1 ? (int64_t)sizeof(mplc_muon_t) : -1;
+}

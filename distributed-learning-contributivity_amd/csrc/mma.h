@@ -1,0 +1,336 @@
+// Tiled matrix products on the CDNA4 matrix cores, shared by the dense layer (dense.hip) and the orthogonalised update
+// (muon.hip).
+//
+// D[m][n] = sum over r of A[m][r] B[n][r], with either operand stored "along r" (element (i, r) at i * ld + r) or
+// "across r" (at r * ld + i); three element kinds: fp32 (v_mfma_f32_32x32x2), bf16 and fp16 (v_mfma_f32_32x32x16); all
+// sums fp32.
+//
+// Split fp16 (PL = 2 planes): a value v is held as hi = fp16(v), lo = fp16(v - hi), 22 bits together, and a product
+// takes three matrix instructions (hi hi, hi lo, lo hi; lo lo is below 2^-24 of the product).  Values must be scaled
+// into fp16's range by the caller.  It reaches fp32's accuracy at a third of the fp16 rate, about twice the fp32 rate.
+//
+// One workgroup computes a BM x BN tile.  Tiles of both operands go through registers into LDS, two buffers deep: the
+// loads of the next tile are in flight while the matrix cores work on this one, one barrier per tile.  A tile row "along
+// r" is BKB bytes and its 16-byte chunks are exchanged (XOR with the row) so that the 16 rows that one pass of
+// ds_read_b128 touches fall on different banks.  A tile "across r" keeps its rows as they are, with a pad that puts
+// the rows that one pass touches on different banks; 16-bit fragments are gathered with ds_read_b64_tr_b16, which
+// transposes 4 x 16 elements inside 16 lanes, fp32 fragments with four ds_read_b32.
+//
+// The matrix instruction is issued as B A^T, so that a lane ends up with 4 consecutive columns n of one row m (wide
+// stores and wide reads of the residual) instead of 4 rows of one column.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace mma {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+enum Kind { F32 = 0, BF16 = 1, F16 = 2 };
+
+template <Kind K> struct Elem { typedef uint16_t T; };
+template <> struct Elem<F32> { typedef float T; };
+
+__device__ __forceinline__ float bf16_to_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+__device__ __forceinline__ uint16_t f32_to_bf16(float v) {
+  union { __bf16 b; uint16_t u; } c;
+  c.b = (__bf16)v;  // round to nearest even
+  return c.u;
+}
+__device__ __forceinline__ float f16_to_f32(uint16_t v) {
+  union { uint16_t u; _Float16 h; } c;
+  c.u = v;
+  return (float)c.h;
+}
+__device__ __forceinline__ uint16_t f32_to_f16(float v) {
+  union { uint16_t u; _Float16 h; } c;
+  c.h = (_Float16)v;
+  return c.u;
+}
+template <Kind K> __device__ __forceinline__ float to_f32(typename Elem<K>::T v) {
+  if constexpr (K == F32) return v;
+  else if constexpr (K == BF16) return bf16_to_f32(v);
+  else return f16_to_f32(v);
+}
+template <Kind K> __device__ __forceinline__ typename Elem<K>::T from_f32(float v) {
+  if constexpr (K == F32) return v;
+  else if constexpr (K == BF16) return f32_to_bf16(v);
+  else return f32_to_f16(v);
+}
+
+// vectors of any element alignment (gfx950 global memory takes unaligned dwordx4)
+struct __attribute__((packed, aligned(2))) U4a2 { uint32_t v[4]; };
+struct __attribute__((packed, aligned(2))) U2a2 { uint32_t v[2]; };
+struct __attribute__((packed, aligned(4))) U4a4 { uint32_t v[4]; };
+
+__device__ __forceinline__ u32x4 load16(const void* p) {
+  const U4a2 t = *reinterpret_cast<const U4a2*>(p);
+  u32x4 r;
+  r[0] = t.v[0]; r[1] = t.v[1]; r[2] = t.v[2]; r[3] = t.v[3];
+  return r;
+}
+
+// `n` valid elements from p (n <= 0: none), the rest zero
+template <Kind K> __device__ __forceinline__ u32x4 load16_edge(const typename Elem<K>::T* p, int n) {
+  constexpr int CH = 16 / sizeof(typename Elem<K>::T);
+  if (n >= CH) return load16(p);
+  u32x4 r = {0, 0, 0, 0};
+  if constexpr (K == F32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) r[e] = __float_as_uint(p[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) r[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+  }
+  return r;
+}
+
+// 4 consecutive elements starting at p, n of them valid
+template <Kind K> __device__ __forceinline__ f32x4 load4(const typename Elem<K>::T* p, int n) {
+  f32x4 r = {0.f, 0.f, 0.f, 0.f};
+  if (n >= 4) {
+    if constexpr (K == F32) {
+      const U4a4 t = *reinterpret_cast<const U4a4*>(p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = __uint_as_float(t.v[e]);
+    } else {
+      const U2a2 t = *reinterpret_cast<const U2a2*>(p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = to_f32<K>((uint16_t)(t.v[e >> 1] >> (16 * (e & 1))));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < n) r[e] = to_f32<K>(p[e]);
+  }
+  return r;
+}
+template <Kind K> __device__ __forceinline__ void store4(typename Elem<K>::T* p, f32x4 v, int n) {
+  if (n >= 4) {
+    if constexpr (K == F32) {
+      U4a4 t;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t.v[e] = __float_as_uint(v[e]);
+      *reinterpret_cast<U4a4*>(p) = t;
+    } else {
+      U2a2 t;
+      t.v[0] = (uint32_t)from_f32<K>(v[0]) | ((uint32_t)from_f32<K>(v[1]) << 16);
+      t.v[1] = (uint32_t)from_f32<K>(v[2]) | ((uint32_t)from_f32<K>(v[3]) << 16);
+      *reinterpret_cast<U2a2*>(p) = t;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < n) p[e] = from_f32<K>(v[e]);
+  }
+}
+
+template <Kind K> __device__ __forceinline__ void mfma(f32x16& d, const u32x4& a, const u32x4& b) {
+  if constexpr (K == F32) {
+    // 4 instructions of 2 r each: instruction e takes r = e (lanes 0-31) and r = 4 + e (lanes 32-63) of the 8
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      d = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), d, 0, 0, 0);
+  } else if constexpr (K == BF16) {
+    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), d, 0, 0, 0);
+  } else {
+    d = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), d, 0, 0, 0);
+  }
+}
+
+// One operand of the product as the kernel sees it.
+template <typename T> struct Operand {
+  const T* p[2];   // planes (p[1] only where PL = 2)
+  int64_t ld;
+  int rows;        // valid i
+};
+
+// The tile of one operand: BT rows i by BK r.
+template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
+  typedef typename Elem<K>::T T;
+  static constexpr int CH = 16 / sizeof(T);              // elements of a chunk
+  static constexpr int BK = BKB / sizeof(T);             // r per tile
+  static constexpr int RPC = ACROSS ? BT / CH : BK / CH; // chunks of a stored row
+  static constexpr int CHUNKS = BT * BK / CH;
+  static constexpr int PER = (CHUNKS + NT - 1) / NT;
+  static constexpr int PAD = K == F32 ? 32 : 64;
+  static constexpr int ROWB = ACROSS ? BT * (int)sizeof(T) + PAD : BKB;
+  static constexpr int PLANE_BYTES = ACROSS ? BK * ROWB : BT * BKB;
+  static constexpr int BYTES = PL * PLANE_BYTES;
+  static_assert(CHUNKS % NT == 0, "whole chunks per thread");
+
+  u32x4 reg[PL][PER];
+
+  __device__ __forceinline__ static int swz(int row, int ch) {
+    if constexpr (BKB == 128) return ch ^ ((row >> 1) & 7);
+    else return ch ^ ((row >> 2) & 3);
+  }
+
+  // tile rows [i0, i0 + BT), r in [r0, r0 + BK); rend: the end of r
+  __device__ __forceinline__ void load(const Operand<T>& o, int i0, int r0, int rend, int tid) {
+    const bool full = i0 + BT <= o.rows && r0 + BK <= rend;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int c = tid + j * NT;
+      const int row = c / RPC, ch = c % RPC;
+      const int i = ACROSS ? i0 + ch * CH : i0 + row;
+      const int r = ACROSS ? r0 + row : r0 + ch * CH;
+      const int64_t off = ACROSS ? (int64_t)r * o.ld + i : (int64_t)i * o.ld + r;
+      if (full) {
+#pragma unroll
+        for (int p = 0; p < PL; ++p) reg[p][j] = load16(o.p[p] + off);
+      } else {
+        int n = ACROSS ? (r < rend ? o.rows - i : 0) : (i < o.rows ? rend - r : 0);
+#pragma unroll
+        for (int p = 0; p < PL; ++p) reg[p][j] = load16_edge<K>(o.p[p] + off, n);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* lds, int tid) const {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int c = tid + j * NT;
+      const int row = c / RPC, ch = c % RPC;
+      const int at = ACROSS ? row * ROWB + ch * 16 : row * ROWB + swz(row, ch) * 16;
+#pragma unroll
+      for (int p = 0; p < PL; ++p) *reinterpret_cast<u32x4*>(lds + p * PLANE_BYTES + at) = reg[p][j];
+    }
+  }
+  // the fragment of rows [i, i + 32) for k-step ks (2 chunks of r)
+  __device__ __forceinline__ static u32x4 frag(const char* lds, int plane, int i, int ks, int lane) {
+    const char* base = lds + plane * PLANE_BYTES;
+    if constexpr (!ACROSS) {
+      const int row = i + (lane & 31);
+      return *reinterpret_cast<const u32x4*>(base + row * ROWB + swz(row, 2 * ks + (lane >> 5)) * 16);
+    } else if constexpr (K == F32) {
+      const int r = (2 * ks + (lane >> 5)) * 4;
+      const float* f = reinterpret_cast<const float*>(base + r * ROWB + (i + (lane & 31)) * 4);
+      u32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(f[e * (ROWB / 4)]);
+      return v;
+    } else {
+      // 16 lanes fetch 4 rows of 16 elements (lane q of them: row q / 4, elements 4 (q % 4) ..) and lane q receives
+      // element q of the 4 rows; twice, for 8 r
+      const int q = lane & 15;
+      const int r = (2 * ks + (lane >> 5)) * 8 + (q >> 2);
+      const char* a = base + r * ROWB + (i + (lane & 16) + 4 * (q & 3)) * 2;
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a));
+      const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 4 * ROWB));
+      const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
+      u32x4 v;
+      v[0] = w0[0]; v[1] = w0[1]; v[2] = w1[0]; v[3] = w1[1];
+      return v;
+    }
+  }
+};
+
+// A workgroup of WM x WN waves, each FM x FN fragments of 32 x 32.
+template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int FN_, int BKB, int PL> struct Block {
+  typedef typename Elem<K>::T T;
+  static constexpr int WM = WM_, WN = WN_, FM = FM_, FN = FN_;
+  static constexpr int NT = 64 * WM * WN;
+  static constexpr int BM = 32 * WM * FM, BN = 32 * WN * FN;
+  typedef Tile<K, A_ACROSS, BM, BKB, NT, PL> TA;
+  typedef Tile<K, B_ACROSS, BN, BKB, NT, PL> TB;
+  static constexpr int BK = TA::BK;
+  static constexpr int STAGE = TA::BYTES + TB::BYTES;
+  static constexpr int LDS_BYTES = 2 * STAGE;
+
+  f32x16 acc[FM][FN];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  }
+
+  __device__ __forceinline__ void compute(const char* la, const char* lb, int lane, int wm, int wn) {
+#pragma unroll
+    for (int ks = 0; ks < BKB / 32; ++ks) {
+      u32x4 a[PL][FM], b[PL][FN];
+#pragma unroll
+      for (int p = 0; p < PL; ++p) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) a[p][i] = TA::frag(la, p, (wm * FM + i) * 32, ks, lane);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) b[p][j] = TB::frag(lb, p, (wn * FN + j) * 32, ks, lane);
+      }
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          if constexpr (PL == 2) {  // small terms first
+            mfma<K>(acc[i][j], b[1][j], a[0][i]);
+            mfma<K>(acc[i][j], b[0][j], a[1][i]);
+          }
+          mfma<K>(acc[i][j], b[0][j], a[0][i]);
+        }
+    }
+  }
+
+  // acc += the product over the tiles it = [0, n): at(it, A, B, r0, rend) says where tile `it` is
+  template <typename At> __device__ __forceinline__ void run(char* lds, int m0, int n0, int n, At at) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave / WN, wn = wave % WN;
+    if (n <= 0) return;
+    TA ta;
+    TB tb;
+    Operand<T> A, B;
+    int r0, rend;
+    at(0, A, B, r0, rend);
+    ta.load(A, m0, r0, rend, tid);
+    tb.load(B, n0, r0, rend, tid);
+    ta.store(lds, tid);
+    tb.store(lds + TA::BYTES, tid);
+    __syncthreads();
+    for (int it = 0; it < n; ++it) {
+      char* cur = lds + (it & 1) * STAGE;
+      char* nxt = lds + ((it + 1) & 1) * STAGE;
+      const bool more = it + 1 < n;
+      if (more) {
+        at(it + 1, A, B, r0, rend);
+        ta.load(A, m0, r0, rend, tid);
+        tb.load(B, n0, r0, rend, tid);
+      }
+      compute(cur, cur + TA::BYTES, lane, wm, wn);
+      if (more) {
+        ta.store(nxt, tid);
+        tb.store(nxt + TA::BYTES, tid);
+      }
+      __syncthreads();
+    }
+  }
+
+  // f(m, n, v): 4 consecutive columns n .. n + 3 of row m
+  template <typename F> __device__ __forceinline__ void each(int m0, int n0, F f) const {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave / WN, wn = wave % WN;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
+          f(m0 + (wm * FM + i) * 32 + (lane & 31), n0 + (wn * FN + j) * 32 + 8 * q + 4 * (lane >> 5), v);
+        }
+  }
+};
+
+}  // namespace mma

@@ -60,6 +60,15 @@ SIGNATURES = {
                                c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int,
                                c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                c_void_p]),
+    # operators on lockstep batches (include/mplc_hip_ops.h); mplc.dense and mplc.muon re-bind them with their structs
+    "mplc_dense_forward_workspace_bytes": (c_size_t, [c_void_p]),
+    "mplc_dense_backward_workspace_bytes": (c_size_t, [c_void_p]),
+    "mplc_dense_forward": (c_int, [c_void_p, c_void_p]),
+    "mplc_dense_backward": (c_int, [c_void_p, c_void_p]),
+    "mplc_muon_workspace_bytes": (c_size_t, [c_void_p]),
+    "mplc_orthogonalize": (c_int, [c_void_p, c_void_p]),
+    "mplc_muon_step": (c_int, [c_void_p, c_void_p]),
+    "mplc_ops_layout": (c_int64, [c_int]),
 }
 
 ABI_VERSION = 4  # include/mplc_hip.h MPLC_ABI_VERSION

@@ -168,5 +168,6 @@ int mplc_tmc_moments(const double* V, int n, const uint8_t* perms, uint64_t seed
 
 #include "mplc_hip_cnn.h"
 #include "mplc_hip_cifar.h"
+#include "mplc_hip_ops.h"
 
 #endif /* MPLC_HIP_H */
