@@ -116,32 +116,37 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
   const int cnt = seg ? p.m : count_of(p.counts, g, p.count_is_r ? p.r : p.m);
   const int M = p.count_is_r ? p.m : cnt, R = p.count_is_r ? cnt : p.r;
   if (m0 >= M) return;
-  const int nk = seg ? p.nk : (R + B::BK - 1) / B::BK;
-  const int all = seg ? p.segments * nk : nk;
-  const int first = split * p.per_split, last = min(all, first + p.per_split);
+  // a split's share: models of a sum over models, tiles of r otherwise
+  const int nk = (R + B::BK - 1) / B::BK;
+  const int first = split * p.per_split, last = min(seg ? p.segments : nk, first + p.per_split);
   const T* pa = reinterpret_cast<const T*>(p.a) + g * p.a_stride;
   const T* pb = reinterpret_cast<const T*>(p.b) + g * p.b_stride;
   B blk;
   blk.clear();
-  blk.run(lds, m0, n0, last - first, [&](int it, Operand<T>& a, Operand<T>& o, int& r0, int& rend) {
-    it += first;
-    const int s = seg ? it / nk : 0;
-    a.p[0] = pa + s * p.a_stride;
-    o.p[0] = pb + s * p.b_stride;
-    a.ld = p.a_ld;
-    o.ld = p.b_ld;
-    a.rows = seg ? count_of(p.counts, s, p.m) : M;
-    o.rows = p.n;
-    r0 = (it - s * nk) * B::BK;
-    rend = R;
-  });
+  if (seg) {
+    blk.run(lds, m0, n0, nk, last - first, [&](int s, Operand<T>& a, Operand<T>& o, int& r0, int& rend) {
+      s += first;
+      a.p[0] = pa + s * p.a_stride;
+      o.p[0] = pb + s * p.b_stride;
+      a.ld = p.a_ld;
+      o.ld = p.b_ld;
+      a.rows = p.m;
+      o.rows = p.n;
+      r0 = 0;
+      rend = R;
+      return count_of(p.counts, s, p.m);
+    });
+  } else {
+    const Operand<T> a = {{pa, nullptr}, p.a_ld, M}, o = {{pb, nullptr}, p.b_ld, p.n};
+    blk.run(lds, a, o, m0, n0, first * B::BK, min(R, last * B::BK));
+  }
   if (p.splits > 1) {
     float* out = p.partial + ((int64_t)split * p.models + g) * p.m * p.n;
-    blk.each(m0, n0, [&](int m, int n, f32x4 v) {
+    blk.each_row(lds, m0, n0, [&](int m, int n, f32x4 v) {
       if (m < M && n < p.n) store4<F32>(out + (int64_t)m * p.n + n, v, p.n - n);
     });
   } else {
-    blk.each(m0, n0, [&](int m, int n, f32x4 v) {
+    blk.each_row(lds, m0, n0, [&](int m, int n, f32x4 v) {
       if (m < M && n < p.n) finish<K>(e, g, m, n, p.n, v);
     });
   }
@@ -217,7 +222,7 @@ __global__ __launch_bounds__(256) void db_kernel(const float* sums, int blocks, 
 enum Form { FORWARD, DX, DW };
 
 struct Plan {
-  int cfg;  // 0: 128 x 128, 1: 64 x 64, 2: 32 x 128
+  int cfg;  // 0: 128 x 128, 1: 64 x 64, 2: 32 x 128, 3: 256 x 256, 4: 64 x 128
   Product p;
   int64_t blocks;
   size_t partial_bytes;
@@ -239,16 +244,18 @@ bool plan(const mplc_dense_t& t, Form form, Plan& out) {
   const int bk = t.dtype == MPLC_DTYPE_F32 ? 32 : 64;
   p.nk = (int)ceil_div(p.r, bk);
   const int64_t big = ceil_div(p.m, 128) * ceil_div(p.n, 128) * p.models;
-  out.cfg = p.m <= 32 ? 2 : big >= 256 ? 0 : (p.m <= 64 || p.n <= 64 || big < 128) ? 1 : 0;
-  const int bm = out.cfg == 0 ? 128 : out.cfg == 1 ? 64 : 32, bn = out.cfg == 1 ? 64 : 128;
+  const int64_t huge = ceil_div(p.m, 256) * ceil_div(p.n, 256) * p.models;
+  out.cfg = p.m <= 32 ? 2 : p.m <= 64 && p.n > 64 ? 4 : (t.dtype != MPLC_DTYPE_F32 && huge >= 256) ? 3 : big >= 256 ? 0 : (p.m <= 64 || p.n <= 64 || big < 128) ? 1 : 0;
+  const int bm = out.cfg == 3 ? 256 : out.cfg == 0 ? 128 : out.cfg == 2 ? 32 : 64, bn = out.cfg == 3 ? 256 : out.cfg == 1 ? 64 : 128;
   p.tiles_m = (int)ceil_div(p.m, bm);
   p.tiles_n = (int)ceil_div(p.n, bn);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.models;
-  const int64_t all = (int64_t)p.nk * p.segments;
+  const int64_t all = p.segments > 1 ? p.segments : p.nk;  // what a split takes a share of
   int64_t splits = 1;
   if (tiles < 512) {  // two workgroups per CU, at least 4 tiles of r each
     splits = ceil_div(512, tiles > 0 ? tiles : 1);
-    if (splits > all / 4) splits = all / 4;
+    const int64_t least = p.segments > 1 ? ceil_div(4, p.nk) : 4;
+    if (splits > all / least) splits = all / least;
     if (splits > 64) splits = 64;
     if (splits < 1) splits = 1;
   }
@@ -266,6 +273,10 @@ template <Kind K, bool AA, bool BA> hipError_t launch(const Plan& pl, const Epil
   const dim3 grid((unsigned)pl.blocks);
   if (pl.cfg == 0) product_kernel<K, AA, BA, 2, 2, 2, 2><<<grid, 256, 0, s>>>(pl.p, e);
   else if (pl.cfg == 1) product_kernel<K, AA, BA, 2, 2, 1, 1><<<grid, 256, 0, s>>>(pl.p, e);
+  else if (pl.cfg == 4) product_kernel<K, AA, BA, 1, 4, 2, 1><<<grid, 256, 0, s>>>(pl.p, e);
+  else if (pl.cfg == 3) {
+    if constexpr (K != F32) product_kernel<K, AA, BA, 2, 4, 4, 2><<<grid, 512, 0, s>>>(pl.p, e);
+  }
   else product_kernel<K, AA, BA, 1, 4, 1, 1><<<grid, 256, 0, s>>>(pl.p, e);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || pl.p.splits == 1) return err;

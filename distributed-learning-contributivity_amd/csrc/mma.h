@@ -134,12 +134,10 @@ template <Kind K> __device__ __forceinline__ void store4(typename Elem<K>::T* p,
   }
 }
 
-template <Kind K> __device__ __forceinline__ void mfma(f32x16& d, const u32x4& a, const u32x4& b) {
+// fp32: instruction e of 4 takes r = e (lanes 0-31) and r = 4 + e (lanes 32-63) of the fragments' 8
+template <Kind K> __device__ __forceinline__ void mfma(f32x16& d, const u32x4& a, const u32x4& b, int e) {
   if constexpr (K == F32) {
-    // 4 instructions of 2 r each: instruction e takes r = e (lanes 0-31) and r = 4 + e (lanes 32-63) of the 8
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      d = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), d, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), d, 0, 0, 0);
   } else if constexpr (K == BF16) {
     d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), d, 0, 0, 0);
   } else {
@@ -169,31 +167,65 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
   static_assert(CHUNKS % NT == 0, "whole chunks per thread");
 
   u32x4 reg[PL][PER];
+  const T* ptr[PL][PER];
+  int live[PER];  // ACROSS: valid elements of the chunk's columns
 
   __device__ __forceinline__ static int swz(int row, int ch) {
     if constexpr (BKB == 128) return ch ^ ((row >> 1) & 7);
     else return ch ^ ((row >> 2) & 3);
   }
 
-  // tile rows [i0, i0 + BT), r in [r0, r0 + BK); rend: the end of r
-  __device__ __forceinline__ void load(const Operand<T>& o, int i0, int r0, int rend, int tid) {
-    const bool full = i0 + BT <= o.rows && r0 + BK <= rend;
+  // Points at the tile of rows [i0, i0 + BT) and r = r0 ...  Rows behind o.rows (never stored) repeat the last one, so
+  // that only the end of r needs checks; chunks of columns across r behind o.rows read the row's first ones.
+  __device__ __forceinline__ void seek(const Operand<T>& o, int i0, int r0, int tid) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const int c = tid + j * NT;
       const int row = c / RPC, ch = c % RPC;
-      const int i = ACROSS ? i0 + ch * CH : i0 + row;
-      const int r = ACROSS ? r0 + row : r0 + ch * CH;
-      const int64_t off = ACROSS ? (int64_t)r * o.ld + i : (int64_t)i * o.ld + r;
-      if (full) {
-#pragma unroll
-        for (int p = 0; p < PL; ++p) reg[p][j] = load16(o.p[p] + off);
+      int64_t off;
+      if constexpr (ACROSS) {
+        const int i = i0 + ch * CH;
+        live[j] = o.rows - i;
+        off = (int64_t)(r0 + row) * o.ld + (live[j] > 0 ? i : 0);
       } else {
-        int n = ACROSS ? (r < rend ? o.rows - i : 0) : (i < o.rows ? rend - r : 0);
-#pragma unroll
-        for (int p = 0; p < PL; ++p) reg[p][j] = load16_edge<K>(o.p[p] + off, n);
+        off = (int64_t)min(i0 + row, o.rows - 1) * o.ld + r0 + ch * CH;
       }
+#pragma unroll
+      for (int p = 0; p < PL; ++p) ptr[p][j] = o.p[p] + off;
     }
+  }
+  __device__ __forceinline__ void advance(int64_t ld) {
+#pragma unroll
+    for (int p = 0; p < PL; ++p)
+#pragma unroll
+      for (int j = 0; j < PER; ++j) ptr[p][j] += ACROSS ? BK * ld : BK;
+  }
+  // the tile at ptr, of which `left` r are valid (left >= BK: all); `whole`: no chunk of columns is cut (uniform)
+  __device__ __forceinline__ void load(int left, bool whole, int tid) {
+    if (left >= BK && (!ACROSS || whole)) {
+#pragma unroll
+      for (int p = 0; p < PL; ++p)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) reg[p][j] = load16(ptr[p][j]);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int c = tid + j * NT;
+      const int row = c / RPC, ch = c % RPC;
+      const int n = ACROSS ? (row < left ? (live[j] > 0 ? live[j] : (whole ? CH : 0)) : 0) : left - ch * CH;
+#pragma unroll
+      for (int p = 0; p < PL; ++p) reg[p][j] = load16_edge<K>(ptr[p][j], n);
+    }
+  }
+  // rows at or behind `rows` are not part of this sum
+  __device__ __forceinline__ void drop_rows(int i0, int rows, int tid) {
+    if constexpr (!ACROSS)
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (i0 + (tid + j * NT) / RPC >= rows)
+#pragma unroll
+          for (int p = 0; p < PL; ++p) reg[p][j] = u32x4{0, 0, 0, 0};
   }
   __device__ __forceinline__ void store(char* lds, int tid) const {
 #pragma unroll
@@ -258,53 +290,106 @@ template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int F
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
   }
 
+  struct Frags {
+    u32x4 a[PL][FM], b[PL][FN];
+  };
+  __device__ __forceinline__ static void read(Frags& f, const char* la, const char* lb, int ks, int lane, int wm, int wn) {
+#pragma unroll
+    for (int p = 0; p < PL; ++p) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) f.a[p][i] = TA::frag(la, p, (wm * FM + i) * 32, ks, lane);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) f.b[p][j] = TB::frag(lb, p, (wn * FN + j) * 32, ks, lane);
+    }
+  }
+  __device__ __forceinline__ void multiply(const Frags& f) {
+    // consecutive instructions write different accumulators: none waits for the one before it
+    if constexpr (PL == 2) {  // small terms first
+      each_pair([&](int i, int j) { mfma<K>(acc[i][j], f.b[1][j], f.a[0][i], 0); });
+      each_pair([&](int i, int j) { mfma<K>(acc[i][j], f.b[0][j], f.a[1][i], 0); });
+    }
+#pragma unroll
+    for (int e = 0; e < (K == F32 ? 4 : 1); ++e)
+      each_pair([&](int i, int j) { mfma<K>(acc[i][j], f.b[0][j], f.a[0][i], e); });
+  }
+  // One tile: the fragments of step ks + 1 are on their way while the matrix cores work on step ks.  Left to itself the
+  // compiler reads each fragment right before its use and waits (fp32 128 x 128: 72 % of the cycles busy).
   __device__ __forceinline__ void compute(const char* la, const char* lb, int lane, int wm, int wn) {
+    constexpr int KS = BKB / 32;
+    Frags f[2];
+    read(f[0], la, lb, 0, lane, wm, wn);
 #pragma unroll
-    for (int ks = 0; ks < BKB / 32; ++ks) {
-      u32x4 a[PL][FM], b[PL][FN];
-#pragma unroll
-      for (int p = 0; p < PL; ++p) {
-#pragma unroll
-        for (int i = 0; i < FM; ++i) a[p][i] = TA::frag(la, p, (wm * FM + i) * 32, ks, lane);
-#pragma unroll
-        for (int j = 0; j < FN; ++j) b[p][j] = TB::frag(lb, p, (wn * FN + j) * 32, ks, lane);
-      }
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          if constexpr (PL == 2) {  // small terms first
-            mfma<K>(acc[i][j], b[1][j], a[0][i]);
-            mfma<K>(acc[i][j], b[0][j], a[1][i]);
-          }
-          mfma<K>(acc[i][j], b[0][j], a[0][i]);
-        }
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks + 1 < KS) read(f[(ks + 1) & 1], la, lb, ks + 1, lane, wm, wn);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(f[ks & 1]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
-  // acc += the product over the tiles it = [0, n): at(it, A, B, r0, rend) says where tile `it` is
-  template <typename At> __device__ __forceinline__ void run(char* lds, int m0, int n0, int n, At at) {
+  template <typename F> __device__ __forceinline__ static void each_pair(F f) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) f(i, j);
+  }
+
+  // acc += the sum over r of the whole product; A.rows, B.rows > 0
+  __device__ __forceinline__ void run(char* lds, const Operand<T>& A, const Operand<T>& B, int m0, int n0, int r0,
+                                      int rend) {
+    run(lds, m0, n0, (rend - r0 + BK - 1) / BK, 1, [&](int, Operand<T>& a, Operand<T>& b, int& first, int& end) {
+      a = A;
+      b = B;
+      first = r0;
+      end = rend;
+      return A.rows;
+    });
+  }
+
+  // acc += the sum over `segments` pieces of n tiles each: at(s, A, B, r0, rend) says where piece s is and returns how
+  // many rows of A take part in it (the others contribute nothing)
+  template <typename At> __device__ __forceinline__ void run(char* lds, int m0, int n0, int n, int segments, At at) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave / WN, wn = wave % WN;
-    if (n <= 0) return;
+    const int all = n * segments;
+    if (all <= 0) return;
     TA ta;
     TB tb;
     Operand<T> A, B;
-    int r0, rend;
-    at(0, A, B, r0, rend);
-    ta.load(A, m0, r0, rend, tid);
-    tb.load(B, n0, r0, rend, tid);
+    int r0, rend, rows, t = 0, s = 0;
+    bool whole_a, whole_b;
+    auto seek = [&]() {
+      rows = at(s, A, B, r0, rend);
+      ta.seek(A, m0, r0, tid);
+      tb.seek(B, n0, r0, tid);
+      whole_a = m0 + BM <= A.rows || A.rows % TA::CH == 0;
+      whole_b = n0 + BN <= B.rows || B.rows % TB::CH == 0;
+    };
+    auto load = [&]() {
+      const int left = rend - r0 - t * BK;
+      ta.load(left, whole_a, tid);
+      tb.load(left, whole_b, tid);
+      if (rows < min(A.rows, m0 + BM)) ta.drop_rows(m0, rows, tid);
+    };
+    seek();
+    load();
     ta.store(lds, tid);
     tb.store(lds + TA::BYTES, tid);
     __syncthreads();
-    for (int it = 0; it < n; ++it) {
+    for (int it = 0; it < all; ++it) {
       char* cur = lds + (it & 1) * STAGE;
       char* nxt = lds + ((it + 1) & 1) * STAGE;
-      const bool more = it + 1 < n;
+      const bool more = it + 1 < all;
       if (more) {
-        at(it + 1, A, B, r0, rend);
-        ta.load(A, m0, r0, rend, tid);
-        tb.load(B, n0, r0, rend, tid);
+        if (++t == n) {
+          t = 0;
+          ++s;
+          seek();
+        } else {
+          ta.advance(A.ld);
+          tb.advance(B.ld);
+        }
+        load();
       }
       compute(cur, cur + TA::BYTES, lane, wm, wn);
       if (more) {
@@ -315,7 +400,8 @@ template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int F
     }
   }
 
-  // f(m, n, v): 4 consecutive columns n .. n + 3 of row m
+  // f(m, n, v): 4 consecutive columns n .. n + 3 of row m, as the accumulators hold them: the 32 lanes of a half wave
+  // have consecutive m
   template <typename F> __device__ __forceinline__ void each(int m0, int n0, F f) const {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave / WN, wn = wave % WN;
@@ -330,6 +416,39 @@ template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int F
           for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
           f(m0 + (wm * FM + i) * 32 + (lane & 31), n0 + (wn * FN + j) * 32 + 8 * q + 4 * (lane >> 5), v);
         }
+  }
+
+  // The same with neighbouring lanes at neighbouring columns, 32 FN of a row, through the wave's own part of LDS (which
+  // run() has left): stores and the residual's loads cover whole lines.
+  template <typename F> __device__ __forceinline__ void each_row(char* lds, int m0, int n0, F f) const {
+    constexpr int LD = 32 * FN + 4;  // floats; the rows one pass writes fall on different banks
+    constexpr int PERROW = 8 * FN, ROWS = 64 / PERROW;
+    static_assert(WM * WN * 32 * LD * 4 <= LDS_BYTES, "the epilogue's rows fit");
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave / WN, wn = wave % WN;
+    float* buf = reinterpret_cast<float*>(lds) + wave * 32 * LD;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
+          *reinterpret_cast<f32x4*>(buf + (lane & 31) * LD + j * 32 + 8 * q + 4 * (lane >> 5)) = v;
+        }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int r = 0; r < 32; r += ROWS) {
+        const int row = r + lane / PERROW, col = (lane % PERROW) * 4;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(buf + row * LD + col);
+        f(m0 + (wm * FM + i) * 32 + row, n0 + wn * FN * 32 + col, v);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
   }
 };
 

@@ -204,13 +204,8 @@ __global__ __launch_bounds__(64 * W * W) void product_kernel(const Prod p) {
   ob.rows = p.n;
   B blk;
   blk.clear();
-  blk.run(lds, m0, n0, last - first, [&](int it, Operand<uint16_t>& A, Operand<uint16_t>& O, int& r0, int& rend) {
-    A = oa;
-    O = ob;
-    r0 = (first + it) * B::BK;
-    rend = p.r;
-  });
-  blk.each(m0, n0, [&](int m, int n, f32x4 v) {
+  blk.run(lds, oa, ob, m0, n0, first * B::BK, min(p.r, last * B::BK));
+  auto result = [&](int m, int n, f32x4 v) {
     if (m >= p.m || n >= p.n) return;
     if constexpr (E == PARTIAL) {
       store4<F32>(p.partial + ((int64_t)sp * p.models + g) * p.m * p.n + (int64_t)m * p.n + n, v, p.n - n);
@@ -233,7 +228,9 @@ __global__ __launch_bounds__(64 * W * W) void product_kernel(const Prod p) {
       v *= p.alpha;
       write_result<K, E>(p, g, m, n, v);
     }
-  });
+  };
+  if ((E == OUT || E == STEP) && p.transposed) blk.each(m0, n0, result);
+  else blk.each_row(lds, m0, n0, result);
 }
 
 // the Gram matrix from its partial sums, added in order
