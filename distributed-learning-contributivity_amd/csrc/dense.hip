@@ -222,13 +222,20 @@ __global__ __launch_bounds__(256) void db_kernel(const float* sums, int blocks, 
 enum Form { FORWARD, DX, DW };
 
 struct Plan {
-  int cfg;  // 0: 128 x 128, 1: 64 x 64, 2: 32 x 128, 3: 256 x 256, 4: 64 x 128
+  int cfg;  // place in SHAPES_16 / SHAPES_F32
   Product p;
   int64_t blocks;
   size_t partial_bytes;
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Multiply-adds per cycle and CU (measured on large products; 0: shape not built).  256 x 256 in fp32 would leave one
+// wave per SIMD without gaining anything: the fp32 matrix rate is reached by 128 x 128.
+constexpr TileShape SHAPES_16[5] = {{128, 128, 2, 640.f}, {64, 64, 3, 330.f}, {32, 128, 2, 280.f}, {256, 256, 1, 840.f},
+                                    {64, 128, 2, 450.f}};
+constexpr TileShape SHAPES_F32[5] = {{128, 128, 2, 115.f}, {64, 64, 4, 105.f}, {32, 128, 3, 95.f}, {256, 256, 1, 0.f},
+                                     {64, 128, 3, 108.f}};
 
 // Tile and split of one product.
 bool plan(const mplc_dense_t& t, Form form, Plan& out) {
@@ -241,28 +248,17 @@ bool plan(const mplc_dense_t& t, Form form, Plan& out) {
   p.r = form == FORWARD ? t.in : form == DX ? t.out : t.rows;
   p.counts = t.counts;
   p.count_is_r = form == DW;
-  const int bk = t.dtype == MPLC_DTYPE_F32 ? 32 : 64;
-  p.nk = (int)ceil_div(p.r, bk);
-  const int64_t big = ceil_div(p.m, 128) * ceil_div(p.n, 128) * p.models;
-  const int64_t huge = ceil_div(p.m, 256) * ceil_div(p.n, 256) * p.models;
-  out.cfg = p.m <= 32 ? 2 : p.m <= 64 && p.n > 64 ? 4 : (t.dtype != MPLC_DTYPE_F32 && huge >= 256) ? 3 : big >= 256 ? 0 : (p.m <= 64 || p.n <= 64 || big < 128) ? 1 : 0;
-  const int bm = out.cfg == 3 ? 256 : out.cfg == 0 ? 128 : out.cfg == 2 ? 32 : 64, bn = out.cfg == 3 ? 256 : out.cfg == 1 ? 64 : 128;
-  p.tiles_m = (int)ceil_div(p.m, bm);
-  p.tiles_n = (int)ceil_div(p.n, bn);
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.models;
-  const int64_t all = p.segments > 1 ? p.segments : p.nk;  // what a split takes a share of
-  int64_t splits = 1;
-  if (tiles < 512) {  // two workgroups per CU, at least 4 tiles of r each
-    splits = ceil_div(512, tiles > 0 ? tiles : 1);
-    const int64_t least = p.segments > 1 ? ceil_div(4, p.nk) : 4;
-    if (splits > all / least) splits = all / least;
-    if (splits > 64) splits = 64;
-    if (splits < 1) splits = 1;
-  }
-  p.per_split = (int)ceil_div(all, splits);
-  p.splits = p.per_split > 0 ? (int)ceil_div(all, p.per_split) : 1;
-  if (p.splits < 1) p.splits = 1;
-  if (all > INT32_MAX || tiles * p.splits > (1 << 23)) return false;
+  const bool f32 = t.dtype == MPLC_DTYPE_F32;
+  p.nk = (int)ceil_div(p.r, f32 ? 32 : 64);
+  const int64_t units = p.segments > 1 ? p.segments : p.nk;
+  const Choice c = choose(f32 ? SHAPES_F32 : SHAPES_16, 5, p.models, p.m, p.n, (int64_t)p.r * p.segments, units, true);
+  out.cfg = c.tile;
+  p.splits = c.splits;
+  p.per_split = c.per_split;
+  const int64_t tiles = c.tiles_m * c.tiles_n * p.models;
+  if (tiles * c.splits > (1 << 23)) return false;
+  p.tiles_m = (int)c.tiles_m;
+  p.tiles_n = (int)c.tiles_n;
   out.blocks = tiles * p.splits;
   out.partial_bytes = p.splits > 1 ? (size_t)p.splits * p.models * p.m * p.n * sizeof(float) : 0;
   out.p = p;

@@ -316,14 +316,23 @@ template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int F
   // compiler reads each fragment right before its use and waits (fp32 128 x 128: 72 % of the cycles busy).
   __device__ __forceinline__ void compute(const char* la, const char* lb, int lane, int wm, int wn) {
     constexpr int KS = BKB / 32;
-    Frags f[2];
-    read(f[0], la, lb, 0, lane, wm, wn);
+    if constexpr (PL * (FM + FN) > 8) {  // no registers for two sets: many instructions per fragment hide the reads
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      if (ks + 1 < KS) read(f[(ks + 1) & 1], la, lb, ks + 1, lane, wm, wn);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(f[ks & 1]);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int ks = 0; ks < KS; ++ks) {
+        Frags f;
+        read(f, la, lb, ks, lane, wm, wn);
+        multiply(f);
+      }
+    } else {
+      Frags f[2];
+      read(f[0], la, lb, 0, lane, wm, wn);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (ks + 1 < KS) read(f[(ks + 1) & 1], la, lb, ks + 1, lane, wm, wn);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(f[ks & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
 
@@ -451,5 +460,53 @@ template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int F
     }
   }
 };
+
+// ------------------------------------------------------------------------------------------ host: tile and split
+struct TileShape {
+  int bm, bn, per_cu;  // workgroups of it that a CU holds
+  float rate;          // multiply-adds per cycle and CU of one CU full of them
+};
+struct Choice {
+  int tile, splits, per_split;  // per_split: units of the sum per split
+  int64_t tiles_m, tiles_n;
+};
+
+// The tile shape and the split of a product of `models` matrices m x n over r, whose sum comes in `units` pieces: the one
+// with the least estimated cycles.  Counted are the rounds in which the workgroups run on 256 CUs, the products of padded
+// tiles at the shape's measured rate, a fixed cost per workgroup, and for a split the partial sums' traffic (about 2 KB
+// per cycle) and the second launch.
+inline Choice choose(const TileShape* shapes, int n_shapes, int64_t models, int64_t m, int64_t n, int64_t r, int64_t units,
+                     bool can_split, double* cost = nullptr) {
+  Choice best = {};
+  double least = 0;
+  for (int s = 0; s < n_shapes; ++s) {
+    const TileShape& t = shapes[s];
+    if (t.rate <= 0) continue;
+    const int64_t tm = (m + t.bm - 1) / t.bm, tn = (n + t.bn - 1) / t.bn, tiles = tm * tn * models;
+    for (int64_t want = 1; want <= 64 && (want == 1 || (can_split && want <= units)); want *= 2) {
+      int64_t per = (units + want - 1) / want;
+      if (per < 1) per = 1;
+      const int64_t splits = units > 0 ? (units + per - 1) / per : 1;
+      if (want > 1 && splits * 2 <= want) continue;
+      const double share = (double)r * per / (units > 0 ? units : 1);
+      const int64_t blocks = tiles * splits;
+      // a CU that holds fewer workgroups than it could runs them faster, down to one at 60 % of the full rate
+      const int64_t full = blocks / (256 * t.per_cu), rest = blocks - full * 256 * t.per_cu;
+      const double one = (double)t.bm * t.bn * share / t.rate + 2500;
+      double cycles = full * t.per_cu * one;
+      if (rest > 0) {
+        const int64_t k = (rest + 255) / 256;
+        cycles += one * (k > 1 ? k : (t.per_cu > 1 ? 1.6 : 1.0));
+      }
+      if (splits > 1) cycles += 8000 + (double)models * m * n * 4 * (splits + 1) / 2000;
+      if (best.splits == 0 || cycles < least) {
+        least = cycles;
+        best = Choice{s, (int)splits, (int)per, tm, tn};
+      }
+    }
+  }
+  if (cost) *cost = least;
+  return best;
+}
 
 }  // namespace mma

@@ -27,7 +27,7 @@ using namespace mma;
 
 constexpr float X_SCALE = 16384.f;  // |X| <= 2
 constexpr float A_SCALE = 8192.f;   // |A|, |P A| <= 4
-constexpr int NORM_CHUNKS = 64;
+constexpr int NORM_CHUNKS = 256;
 
 struct Planes {  // split fp16 of a matrix times its scale
   uint16_t* hi;
@@ -73,71 +73,106 @@ struct Source {
   int nesterov, rows, cols;
 };
 
-// U at (r, c); FIRST: the pass that updates the momentum
-template <Kind K, bool FIRST> __device__ __forceinline__ float update_at(const Source& s, int g, int r, int c) {
+// U at (r, c .. c + 3), `valid` of them inside; FIRST: the pass that updates the momentum
+template <Kind K, bool FIRST> __device__ __forceinline__ f32x4 update4(const Source& s, int g, int64_t r, int c, int valid) {
   typedef typename Elem<K>::T T;
-  const float v = to_f32<K>(reinterpret_cast<const T*>(s.g)[g * s.g_stride + r * s.g_ld + c]);
-  if (s.m == nullptr) return v;
+  f32x4 u = load4<K>(reinterpret_cast<const T*>(s.g) + g * s.g_stride + r * s.g_ld + c, valid);
+  if (s.m == nullptr) return u;
   float* pm = s.m + g * s.m_stride + r * s.m_ld + c;
-  float m = *pm;
+  f32x4 m = load4<F32>(pm, valid);
   if (FIRST) {
-    m = s.beta * m + v;
-    *pm = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = s.beta * m[i] + u[i];
+    store4<F32>(pm, m, valid);
   }
-  return s.nesterov ? s.beta * m + v : m;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = s.nesterov ? s.beta * m[i] + u[i] : m[i];
+  return u;
 }
 
-// |U|^2 in 64 bits (neither 1e-30 nor 1e30 leaves the range), NORM_CHUNKS partial sums per model
+// Walks a matrix's groups of 4 columns, NT threads side by side, without a division per group.
+struct Walk {
+  int r, c4, dr, dc, n4;
+  __device__ __forceinline__ Walk(int first, int step, int n4_) : n4(n4_) {
+    r = first / n4;
+    c4 = first - r * n4;
+    dr = step / n4;
+    dc = step - dr * n4;
+  }
+  __device__ __forceinline__ void next() {
+    r += dr;
+    c4 += dc;
+    if (c4 >= n4) {
+      c4 -= n4;
+      ++r;
+    }
+  }
+};
+
+__device__ __forceinline__ double block_sum(double v, double* part) {  // part: 4 doubles; every thread gets the sum
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// X_SCALE / |U| from |U|^2; 0 for U = 0, NaN where U is not finite
+__device__ __forceinline__ double inverse_norm(double square) {
+  if (square == 0.) return 0.;
+  if (!(square < (double)INFINITY)) return (double)NAN;
+  return (double)X_SCALE / sqrt(square);
+}
+
+// |U|^2 in 64 bits (neither 1e-30 nor 1e30 leaves the range), one partial sum per workgroup, NORM_CHUNKS at most per model
 template <Kind K> __global__ __launch_bounds__(256) void norm_kernel(const Source s, double* sums) {
   __shared__ double part[4];
   const int g = blockIdx.y;
-  const int64_t n = (int64_t)s.rows * s.cols;
   double sum = 0.;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
-    const int r = (int)(t / s.cols), c = (int)(t - (int64_t)r * s.cols);
-    const double v = update_at<K, true>(s, g, r, c);
-    sum += v * v;
-  }
+  for (Walk w(blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, (s.cols + 3) >> 2); w.r < s.rows; w.next()) {
+    const f32x4 v = update4<K, true>(s, g, w.r, w.c4 * 4, s.cols - w.c4 * 4);
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) sum += __shfl_down(sum, d, 64);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) sums[(int64_t)g * gridDim.x + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+    for (int i = 0; i < 4; ++i) sum += (double)v[i] * (double)v[i];
+  }
+  sum = block_sum(sum, part);
+  if (threadIdx.x == 0) sums[(int64_t)g * gridDim.x + blockIdx.x] = sum;
 }
 
-// X_SCALE / |U|; 0 for U = 0, NaN where U is not finite
-__device__ __forceinline__ double inverse_norm(const double* sums, int g, int chunks) {
-  double sum = 0.;
-  for (int i = 0; i < chunks; ++i) sum += sums[(int64_t)g * chunks + i];
-  if (sum == 0.) return 0.;
-  if (!(sum < (double)INFINITY)) return (double)NAN;
-  return (double)X_SCALE / sqrt(sum);
+// X_0 as planes [L][ld]; L = rows
+template <Kind K> __global__ __launch_bounds__(256) void start_kernel(const Source s, const double* sums, int chunks, const Planes x) {
+  __shared__ double part[4];
+  const int g = blockIdx.y;
+  const double inv = inverse_norm(block_sum(threadIdx.x < chunks ? sums[(int64_t)g * chunks + threadIdx.x] : 0., part));
+  for (Walk w(blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, (s.cols + 3) >> 2); w.r < s.rows; w.next()) {
+    f32x4 v = update4<K, false>(s, g, w.r, w.c4 * 4, s.cols - w.c4 * 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (float)((double)v[i] * inv);
+    store_planes(x, g, w.r, w.c4 * 4, v);
+  }
 }
 
-// X_0 as planes [L][ld], its columns behind k zero.  TALL: rows = L.  32 x 32 tiles, transposed through LDS where not.
-template <Kind K, bool TALL>
-__global__ __launch_bounds__(256) void start_kernel(const Source s, const double* sums, int chunks, const Planes x) {
-  __shared__ float tile[32][33];
+// The same with L = cols: 64 x 64 tiles, transposed through LDS
+template <Kind K> __global__ __launch_bounds__(256) void start_wide_kernel(const Source s, const double* sums, int chunks, const Planes x) {
+  __shared__ double part[4];
+  __shared__ float tile[64][65];
   const int g = blockIdx.z;
-  const double inv = inverse_norm(sums, g, chunks);
-  const int L = TALL ? s.rows : s.cols, k = TALL ? s.cols : s.rows;
-  const int l0 = blockIdx.x * 32, k0 = blockIdx.y * 32;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  for (int i = ty; i < 32; i += 8) {
-    const int r = TALL ? l0 + i : k0 + i, c = TALL ? k0 + tx : l0 + tx;
-    float v = 0.f;
-    if (r < s.rows && c < s.cols) v = (float)((double)update_at<K, false>(s, g, r, c) * inv);
-    if (TALL) tile[i][tx] = v;
-    else tile[tx][i] = v;
+  const double inv = inverse_norm(block_sum(threadIdx.x < chunks ? sums[(int64_t)g * chunks + threadIdx.x] : 0., part));
+  const int l0 = blockIdx.x * 64, k0 = blockIdx.y * 64;
+  const int q = (threadIdx.x & 15) * 4, ty = threadIdx.x >> 4;
+  for (int i = ty; i < 64; i += 16) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (k0 + i < s.rows && l0 + q < s.cols) v = update4<K, false>(s, g, k0 + i, l0 + q, s.cols - l0 - q);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tile[q + e][i] = (float)((double)v[e] * inv);
   }
   __syncthreads();
-  const int row = threadIdx.x >> 3, col = (threadIdx.x & 7) * 4;
-  if (l0 + row < L && k0 + col < x.ld) {
-    f32x4 v;
+  for (int i = ty; i < 64; i += 16)
+    if (l0 + i < s.cols && k0 + q < x.ld) {
+      f32x4 v;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = k0 + col + e < k ? tile[row][col + e] : 0.f;
-    store_planes(x, g, l0 + row, k0 + col, v);
-  }
+      for (int e = 0; e < 4; ++e) v[e] = k0 + q + e < s.rows ? tile[i][q + e] : 0.f;
+      store_planes(x, g, l0 + i, k0 + q, v);
+    }
 }
 
 // ------------------------------------------------------------------------------------------ products
@@ -146,6 +181,7 @@ enum Epi { PLANES, POLY, PARTIAL, OUT, STEP };
 struct Prod {
   Planes a, b;
   int m, n, r, models, tiles_m, tiles_n, splits, per_split;
+  int symmetric;     // the result is: tiles above the diagonal are not computed but written twice
   float alpha;       // value = alpha * sum
   Planes out;        // PLANES, POLY: value times the output's scale (in alpha)
   Planes add;        // POLY: A, whose square the product is
@@ -179,16 +215,41 @@ template <Kind K, Epi E> __device__ __forceinline__ void write_result(const Prod
   }
 }
 
+// tile i of those at and below the diagonal: (0,0) (1,0) (1,1) (2,0) ...
+__device__ __forceinline__ void lower_tile(int i, int& tm, int& tn) {
+  tm = (int)((sqrtf(8.f * i + 1.f) - 1.f) * 0.5f);
+  while (tm * (tm + 1) / 2 > i) --tm;
+  while ((tm + 1) * (tm + 2) / 2 <= i) ++tm;
+  tn = i - tm * (tm + 1) / 2;
+}
+
+// planes at (n .. n + 3, m): the mirror image of a tile below the diagonal
+__device__ __forceinline__ void store_planes_mirrored(const Planes& p, int g, int m, int n, int N, f32x4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < N) {
+      const int64_t at = g * p.stride + (int64_t)(n + i) * p.ld + m;
+      split(v[i], p.hi[at], p.lo[at]);
+    }
+}
+
 // GRAM: both operands are X and the sum runs over its rows
-template <Kind K, bool GRAM, Epi E, int W, int F>
-__global__ __launch_bounds__(64 * W * W) void product_kernel(const Prod p) {
-  typedef Block<F16, GRAM, GRAM, W, W, F, F, 64, 2> B;
+template <Kind K, bool GRAM, Epi E, int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Prod p) {
+  typedef Block<F16, GRAM, GRAM, WM, WN, FM, FN, 64, 2> B;
   __shared__ __attribute__((aligned(16))) char lds[B::LDS_BYTES];
   int64_t b = xcd_block();
-  const int tn = (int)(b % p.tiles_n);
-  b /= p.tiles_n;
-  const int tm = (int)(b % p.tiles_m);
-  b /= p.tiles_m;
+  int tm, tn;
+  if (p.symmetric) {
+    const int tiles = p.tiles_m * (p.tiles_m + 1) / 2;
+    lower_tile((int)(b % tiles), tm, tn);
+    b /= tiles;
+  } else {
+    tn = (int)(b % p.tiles_n);
+    b /= p.tiles_n;
+    tm = (int)(b % p.tiles_m);
+    b /= p.tiles_m;
+  }
   const int sp = (int)(b % p.splits), g = (int)(b / p.splits);
   const int m0 = tm * B::BM, n0 = tn * B::BN;
   const int nk = (p.r + B::BK - 1) / B::BK;
@@ -205,62 +266,302 @@ __global__ __launch_bounds__(64 * W * W) void product_kernel(const Prod p) {
   B blk;
   blk.clear();
   blk.run(lds, oa, ob, m0, n0, first * B::BK, min(p.r, last * B::BK));
-  auto result = [&](int m, int n, f32x4 v) {
-    if (m >= p.m || n >= p.n) return;
-    if constexpr (E == PARTIAL) {
-      store4<F32>(p.partial + ((int64_t)sp * p.models + g) * p.m * p.n + (int64_t)m * p.n + n, v, p.n - n);
-    } else if constexpr (E == PLANES) {
-      v *= p.alpha;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i >= p.n) v[i] = 0.f;
-      store_planes(p.out, g, m, n, v);
-    } else if constexpr (E == POLY) {
+  auto value = [&](int m, int n, f32x4 v) {
+    if constexpr (E == POLY) {
       const f32x4 a = load_planes(p.add, g, m, n);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         v[i] = p.cc * v[i] + p.cb * a[i];
         if (n + i == m) v[i] += p.ca;
-        if (n + i >= p.n) v[i] = 0.f;
       }
-      store_planes(p.out, g, m, n, v);
-    } else {
+    } else if constexpr (E != PARTIAL) {
       v *= p.alpha;
-      write_result<K, E>(p, g, m, n, v);
     }
+    if constexpr (E == PLANES || E == POLY)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i >= p.n) v[i] = 0.f;
+    return v;
+  };
+  auto result = [&](int m, int n, f32x4 v) {
+    if (m >= p.m || n >= p.n) return;
+    v = value(m, n, v);
+    if constexpr (E == PARTIAL)
+      store4<F32>(p.partial + ((int64_t)sp * p.models + g) * p.m * p.n + (int64_t)m * p.n + n, v, p.n - n);
+    else if constexpr (E == PLANES || E == POLY) store_planes(p.out, g, m, n, v);
+    else write_result<K, E>(p, g, m, n, v);
   };
   if ((E == OUT || E == STEP) && p.transposed) blk.each(m0, n0, result);
   else blk.each_row(lds, m0, n0, result);
+  if constexpr (E == PLANES || E == POLY)
+    if (p.symmetric && tm != tn)
+      blk.each(m0, n0, [&](int m, int n, f32x4 v) {
+        if (m < p.m && n < p.n) store_planes_mirrored(p.out, g, m, n, p.n, value(m, n, v));
+      });
 }
 
-// the Gram matrix from its partial sums, added in order
+// the Gram matrix from its partial sums, added in order: 64 x 64 tiles at and below the diagonal, the others mirrored
 __global__ __launch_bounds__(256) void join_kernel(const Prod p) {
-  const int n4 = p.out.ld >> 2;
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= (int64_t)p.m * n4) return;
-  const int g = blockIdx.y, m = (int)(t / n4), n = (int)(t % n4) * 4;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  if (n < p.n) {
-    const float* src = p.partial + (int64_t)g * p.m * p.n + (int64_t)m * p.n + n;
-    const int64_t step = (int64_t)p.models * p.m * p.n;
-    v = load4<F32>(src, p.n - n);
-    for (int s = 1; s < p.splits; ++s) v += load4<F32>(src + s * step, p.n - n);
-    v *= p.alpha;
+  __shared__ float tile[64][65];
+  const int g = blockIdx.y;
+  int tm, tn;
+  lower_tile(blockIdx.x, tm, tn);
+  const int m0 = tm * 64, n0 = tn * 64;
+  const float* src = p.partial + (int64_t)g * p.m * p.n;
+  const int64_t step = (int64_t)p.models * p.m * p.n;
+  const int q = (threadIdx.x & 15) * 4;
+  for (int i = threadIdx.x >> 4; i < 64; i += 16) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    const int m = m0 + i, n = n0 + q;
+    if (m < p.m && n < p.n) {
+      const float* at = src + (int64_t)m * p.n + n;
+      v = load4<F32>(at, p.n - n);
+      for (int s = 1; s < p.splits; ++s) v += load4<F32>(at + s * step, p.n - n);
+      v *= p.alpha;
+      store_planes(p.out, g, m, n, v);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tile[q + e][i] = v[e];
   }
-  store_planes(p.out, g, m, n, v);
+  if (tm == tn) return;
+  __syncthreads();
+  for (int i = threadIdx.x >> 4; i < 64; i += 16) {
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = tile[i][q + e];
+    if (n0 + i < p.n && m0 + q < p.m) store_planes(p.out, g, n0 + i, m0 + q, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ matrices that fit in LDS
+// One workgroup does everything for one model: U (and the momentum) is read once, X stays in LDS in fp32, and so do the
+// k x k matrices; all products on v_mfma_f32_16x16x4.  Such a matrix needs 10 MFLOP or less, so what counts is that one
+// launch replaces 20.  KT: k in tiles of 16.  Rows of S = 16 KT + 4 floats put the 16 rows of a fragment on different banks.
+// A fragment of 16 r is one 16-byte read per lane: lane (i, h) holds r = 4 h .. 4 h + 3 and instruction e takes its
+// element e - the order of r is free as long as both operands agree.
+struct Small {
+  Source src;
+  int L, k, tall, steps, phases;
+  float a, b, c;
+  void* dst;
+  int64_t dst_stride, dst_ld;
+  float keep, step;
+};
+
+constexpr int small_scratch(int KT) {  // floats: T, P and Q, or four waves' partial Gram tiles
+  const int mats = 3 * 16 * KT * (16 * KT + 4), parts = 4 * 256 * (KT * (KT + 1) / 2);
+  return mats > parts ? mats : parts;
+}
+
+template <int KT> struct SmallBlock {
+  static constexpr int KP = 16 * KT, S = KP + 4;
+  static __device__ __forceinline__ f32x4 frag(const float* m, int row, int s, int lane) {
+    return *reinterpret_cast<const f32x4*>(m + (row + (lane & 15)) * S + 16 * s + 4 * (lane >> 4));
+  }
+  // tile (ti, tj) of lhs rhs^T
+  static __device__ __forceinline__ f32x4 tile(const float* lhs, const float* rhs, int ti, int tj, int lane) {
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < KT; ++s) {
+      const f32x4 a = frag(lhs, ti * 16, s, lane), b = frag(rhs, tj * 16, s, lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], acc, 0, 0, 0);
+    }
+    return acc;
+  }
+  // out = f(row, col, lhs rhs) for symmetric matrices that commute; out is neither
+  template <typename F> static __device__ __forceinline__ void product(float* out, const float* lhs, const float* rhs, F f) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int t = wave; t < KT * KT; t += 4) {
+      const int ti = t / KT, tj = t % KT;
+      const f32x4 v = tile(lhs, rhs, ti, tj, lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = ti * 16 + (lane >> 4) * 4 + e, col = tj * 16 + (lane & 15);
+        out[row * S + col] = f(row, col, v[e]);
+      }
+    }
+    __syncthreads();
+  }
+  // A = X^T X; rows of X dealt to the waves, four at a time; the waves' sums added in order
+  static __device__ __forceinline__ void gram(float* A, const float* X, float* scratch, int Lp) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int TILES = KT * (KT + 1) / 2;
+    f32x4 acc[TILES];
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int l = wave * 4; l < Lp; l += 16) {
+      float f[KT];
+#pragma unroll
+      for (int t = 0; t < KT; ++t) f[t] = X[(l + (lane >> 4)) * S + t * 16 + (lane & 15)];
+      int i = 0;
+#pragma unroll
+      for (int ti = 0; ti < KT; ++ti)
+#pragma unroll
+        for (int tj = 0; tj <= ti; ++tj, ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[ti], f[tj], acc[i], 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) *reinterpret_cast<f32x4*>(scratch + ((wave * TILES + i) * 64 + lane) * 4) = acc[i];
+    __syncthreads();
+    for (int i = wave; i < TILES; i += 4) {
+      const float* at = scratch + (i * 64 + lane) * 4;
+      f32x4 v = *reinterpret_cast<const f32x4*>(at);
+#pragma unroll
+      for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(at + w * TILES * 256);
+      int ti = 0;
+      while ((ti + 1) * (ti + 2) / 2 <= i) ++ti;
+      const int tj = i - ti * (ti + 1) / 2;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = ti * 16 + (lane >> 4) * 4 + e, col = tj * 16 + (lane & 15);
+        A[row * S + col] = v[e];
+        if (ti != tj) A[col * S + row] = v[e];
+      }
+    }
+    __syncthreads();
+  }
+  // X = X Q, each wave its own rows
+  static __device__ __forceinline__ void apply(float* X, const float* Q, int Lp) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int r = wave * 16; r < Lp; r += 64) {
+      f32x4 v[KT];
+#pragma unroll
+      for (int t = 0; t < KT; ++t) v[t] = tile(X + r * S, Q, 0, t, lane);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) X[(r + (lane >> 4) * 4 + e) * S + t * 16 + (lane & 15)] = v[t][e];
+    }
+    __syncthreads();
+  }
+};
+
+template <Kind K, int KT, Epi E> __global__ __launch_bounds__(256) void small_kernel(const Small p) {
+  typedef SmallBlock<KT> B;
+  typedef typename Elem<K>::T T;  // of U
+  constexpr int S = B::S, MAT = B::KP * S;
+  extern __shared__ __attribute__((aligned(16))) float sm[];
+  __shared__ double part[4];
+  const int g = blockIdx.x, tid = threadIdx.x;
+  const int Lp = (p.L + 15) & ~15;
+  float* X = sm;
+  float* A = X + Lp * S;
+  float* scratch = A + MAT;
+  const Source& s = p.src;
+  const int n4 = (s.cols + 3) >> 2;
+  for (int i = tid * 4; i < Lp * S; i += 1024) *reinterpret_cast<f32x4*>(X + i) = f32x4{0.f, 0.f, 0.f, 0.f};
+  __syncthreads();
+  double sum = 0.;
+  for (Walk w(tid, 256, n4); w.r < s.rows; w.next()) {
+    const int c = w.c4 * 4;
+    const f32x4 v = update4<K, true>(s, g, w.r, c, s.cols - c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < s.cols) {
+        X[p.tall ? w.r * S + c + e : (c + e) * S + w.r] = v[e];
+        sum += (double)v[e] * (double)v[e];
+      }
+  }
+  const double inv = inverse_norm(block_sum(sum, part)) * (1. / X_SCALE);
+  for (int i = tid * 4; i < Lp * S; i += 1024) {
+    f32x4 v = *reinterpret_cast<f32x4*>(X + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)((double)v[e] * inv);
+    *reinterpret_cast<f32x4*>(X + i) = v;
+  }
+  __syncthreads();
+  int done = 0;
+  for (int ph = 0; ph < p.phases; ++ph) {
+    const int n = (p.steps - done + (p.phases - ph) - 1) / (p.phases - ph);
+    done += n;
+    B::gram(A, X, scratch, Lp);
+    float *P = scratch, *T1 = scratch + MAT, *Q = scratch + 2 * MAT;
+    for (int i = 0; i < n; ++i) {
+      float* cur = i == 0 ? Q : P;
+      B::product(cur, A, A, [&](int row, int col, float v) {
+        return p.c * v + (p.b * A[row * S + col] + (row == col ? p.a : 0.f));
+      });
+      auto same = [](int, int, float v) { return v; };
+      if (i + 1 < n) {
+        B::product(T1, cur, A, same);
+        B::product(A, T1, cur, same);
+      }
+      if (i > 0) {
+        B::product(T1, P, Q, same);
+        float* h = Q;
+        Q = T1;
+        T1 = h;
+      }
+    }
+    B::apply(X, Q, Lp);
+  }
+  typedef typename Elem<E == STEP ? F32 : K>::T O;
+  O* dst = reinterpret_cast<O*>(p.dst) + g * p.dst_stride;
+  for (Walk w(tid, 256, n4); w.r < s.rows; w.next()) {
+    const int c = w.c4 * 4;
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = c + e < s.cols ? X[p.tall ? w.r * S + c + e : (c + e) * S + w.r] : 0.f;
+    O* at = dst + w.r * p.dst_ld + c;
+    if constexpr (E == STEP) {
+      const f32x4 old = load4<F32>(at, s.cols - c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = p.keep * old[e] - p.step * v[e];
+      store4<F32>(at, v, s.cols - c);
+    } else {
+      store4<K>(at, v, s.cols - c);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------ host
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align16(size_t v) { return (v + 15) & ~(size_t)15; }
 
+// Multiply-adds per cycle and CU of split products (measured on large ones)
+constexpr TileShape SHAPES[3] = {{256, 256, 1, 280.f}, {128, 128, 2, 205.f}, {64, 64, 3, 120.f}};
+
+// LDS of small_kernel, 0 where the matrix does not fit
+size_t small_bytes(int L, int k) {
+  if (k > 64) return 0;
+  const int kt = (k + 15) / 16, s = 16 * kt + 4;
+  const int64_t bytes = ((int64_t)((L + 15) & ~15) * s + 16 * kt * s + small_scratch(kt)) * 4;
+  return bytes <= 160 * 1024 - 256 ? (size_t)bytes : 0;
+}
+
 struct Space {
-  int k, L, ld, phases, gram_splits, gram_per_split, chunks;
+  int k, L, ld, phases, chunks;
+  size_t small;
+  Choice gram;
   size_t sums, x, square, partial, total;  // bytes of one of each
   int n_x;
 };
 
-bool wide_tile(int64_t tiles128) { return tiles128 >= 64; }
+Choice shape_for(int64_t models, int64_t m, int64_t n, int64_t r, bool symmetric, bool can_split) {
+  Choice best = {};
+  double least = 0;
+  for (int s = 0; s < 3; ++s) {  // choose() per shape, its tiles halved where the result is symmetric
+    TileShape one = SHAPES[s];
+    const int64_t t = ceil_div(m, one.bm);
+    const int64_t tiles = symmetric ? t * (t + 1) / 2 : t * ceil_div(n, one.bn);
+    double cost;
+    Choice c = choose(&one, 1, models * tiles, one.bm, one.bn, r, ceil_div(r, 32), can_split, &cost);
+    c.tile = s;
+    c.tiles_m = t;
+    c.tiles_n = symmetric ? t : ceil_div(n, one.bn);
+    if (s == 0 || cost < least) {
+      least = cost;
+      best = c;
+    }
+  }
+  return best;
+}
+
+int64_t blocks_of(const Choice& c, int64_t models, bool symmetric) {
+  return (symmetric ? c.tiles_m * (c.tiles_m + 1) / 2 : c.tiles_m * c.tiles_n) * models * c.splits;
+}
 
 bool space(const mplc_muon_t& t, Space& s) {
   if (t.n_models < 0 || t.n_models > 65535 || t.rows < 1 || t.cols < 1 || t.dtype < 0 || t.dtype > 2) return false;
@@ -270,29 +571,25 @@ bool space(const mplc_muon_t& t, Space& s) {
   s.L = t.rows < t.cols ? t.cols : t.rows;
   s.ld = (s.k + 7) & ~7;
   s.phases = 2 * (int64_t)s.L >= 3 * (int64_t)s.k ? (t.steps + 2) / 3 : t.steps;
-  s.n_x = s.phases > 1 ? 2 : 1;
-  const int64_t elems = (int64_t)t.rows * t.cols;
-  s.chunks = (int)(ceil_div(elems, 4096) < NORM_CHUNKS ? ceil_div(elems, 4096) : NORM_CHUNKS);
-  const int64_t t64 = ceil_div(s.k, 64), t128 = ceil_div(s.k, 128);
-  const int64_t tiles = (s.k <= 64 ? t64 * t64 : t128 * t128) * t.n_models;
-  const int64_t nk = ceil_div(s.L, 32);
-  int64_t splits = 1;
-  if (tiles < 512 && tiles > 0) {  // two workgroups per CU, at least 8 tiles of r each
-    splits = ceil_div(512, tiles);
-    if (splits > nk / 8) splits = nk / 8;
-    if (splits > 64) splits = 64;
-    if (splits < 1) splits = 1;
+  s.small = small_bytes(s.L, s.k);
+  if (s.small) {  // reading X again costs nothing here: phases of two steps lose less to the Gram matrix's error
+    s.phases = (t.steps + 1) / 2;
+    return true;
   }
-  s.gram_per_split = (int)ceil_div(nk, splits);
-  s.gram_splits = (int)ceil_div(nk, s.gram_per_split);
+  s.n_x = s.phases > 1 ? 2 : 1;
+  const int64_t groups = (int64_t)t.rows * ceil_div(t.cols, 4);
+  if (groups > (int64_t)1 << 30) return false;
+  const int64_t most = t.n_models >= 16 ? 64 : NORM_CHUNKS;
+  s.chunks = (int)(ceil_div(groups, 1024) < most ? ceil_div(groups, 1024) : most);
+  s.gram = shape_for(t.n_models, s.k, s.k, s.L, true, true);
   const size_t G = (size_t)t.n_models;
   s.sums = align16(G * s.chunks * sizeof(double));
   s.x = align16(G * s.L * s.ld * 2) * 2;       // both planes
   s.square = align16(G * s.k * s.ld * 2) * 2;
-  s.partial = s.gram_splits > 1 ? align16(G * s.gram_splits * (size_t)s.k * s.k * sizeof(float)) : 0;
+  s.partial = s.gram.splits > 1 ? align16(G * s.gram.splits * (size_t)s.k * s.k * sizeof(float)) : 0;
   s.total = s.sums + s.n_x * s.x + 6 * s.square + s.partial;
-  const int64_t most = ceil_div(s.L, 64) * ceil_div(s.k, 64) * (int64_t)t.n_models;
-  return most <= (1 << 23) && tiles * s.gram_splits <= (1 << 23) && ceil_div(s.k, 32) <= 65535;
+  return ceil_div(s.L, 64) * ceil_div(s.k, 64) * (int64_t)t.n_models <= (1 << 23) &&
+         blocks_of(s.gram, t.n_models, true) <= (1 << 23) && ceil_div(s.k, 64) <= 65535;
 }
 
 // largest |a s + b s^3 + c s^5| for s in [0, r]
@@ -327,23 +624,47 @@ float scale_for(double bound) {
   return (float)ldexp(1., e);
 }
 
-template <Kind K, bool GRAM, Epi E> hipError_t product(Prod p, hipStream_t s) {
-  const int64_t big = ceil_div(p.m, 128) * ceil_div(p.n, 128) * p.models;
-  const bool wide = GRAM ? p.m > 64 : (p.n > 64 && wide_tile(big));
-  const int b = wide ? 128 : 64;
-  p.tiles_m = (int)ceil_div(p.m, b);
-  p.tiles_n = (int)ceil_div(p.n, b);
-  if (!GRAM) {
-    p.splits = 1;
-    p.per_split = (int)ceil_div(p.r, 32);
-  }
-  const dim3 grid((unsigned)((int64_t)p.tiles_m * p.tiles_n * p.splits * p.models));
-  if (wide) product_kernel<K, GRAM, E, 2, 2><<<grid, 256, 0, s>>>(p);
-  else product_kernel<K, GRAM, E, 2, 1><<<grid, 256, 0, s>>>(p);
+template <Kind K, bool GRAM, Epi E> hipError_t product(Prod p, const Choice& c, hipStream_t s) {
+  p.tiles_m = (int)c.tiles_m;
+  p.tiles_n = (int)c.tiles_n;
+  p.splits = c.splits;
+  p.per_split = c.per_split;
+  const dim3 grid((unsigned)blocks_of(c, p.models, p.symmetric));
+  if (c.tile == 0) product_kernel<K, GRAM, E, 2, 4, 4, 2><<<grid, 512, 0, s>>>(p);
+  else if (c.tile == 1) product_kernel<K, GRAM, E, 2, 2, 2, 2><<<grid, 256, 0, s>>>(p);
+  else product_kernel<K, GRAM, E, 2, 2, 1, 1><<<grid, 256, 0, s>>>(p);
   return hipGetLastError();
 }
 
+template <Kind K, int KT, Epi E> int launch_small(const Small& p, const Space& sp, int models, hipStream_t s) {
+  if (sp.small > 48 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&small_kernel<K, KT, E>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)sp.small);
+    if (e != hipSuccess) return (int)e;
+  }
+  small_kernel<K, KT, E><<<dim3((unsigned)models), 256, sp.small, s>>>(p);
+  return (int)hipGetLastError();
+}
+
+template <Kind K, Epi E> int run_small(const mplc_muon_t& t, const Space& sp, const Source& src, hipStream_t s) {
+  Small p = {src, sp.L, sp.k, t.rows >= t.cols, t.steps, sp.phases, t.a, t.b, t.c, t.out, t.out_stride, t.out_ld, 0.f, 0.f};
+  if (E == STEP) {
+    p.dst = t.w;
+    p.dst_stride = t.w_stride;
+    p.dst_ld = t.w_ld;
+    p.keep = (float)(1. - (double)t.lr * t.weight_decay);
+    p.step = t.lr * t.scale;
+  }
+  switch ((sp.k + 15) / 16) {
+    case 1: return launch_small<K, 1, E>(p, sp, t.n_models, s);
+    case 2: return launch_small<K, 2, E>(p, sp, t.n_models, s);
+    case 3: return launch_small<K, 3, E>(p, sp, t.n_models, s);
+    default: return launch_small<K, 4, E>(p, sp, t.n_models, s);
+  }
+}
+
 template <Kind K, Epi LAST> int run(const mplc_muon_t& t, const Space& sp, const Source& src, hipStream_t s) {
+  if (sp.small) return run_small<K, LAST>(t, sp, src, s);
   char* ws = reinterpret_cast<char*>(t.workspace);
   double* sums = reinterpret_cast<double*>(ws);
   ws += sp.sums;
@@ -360,14 +681,19 @@ template <Kind K, Epi LAST> int run(const mplc_muon_t& t, const Space& sp, const
   norm_kernel<K><<<dim3(sp.chunks, t.n_models), 256, 0, s>>>(src, sums);
   if ((err = hipGetLastError()) != hipSuccess) return (int)err;
   const bool tall = t.rows >= t.cols;
-  const dim3 sg((unsigned)ceil_div(sp.L, 32), (unsigned)ceil_div(sp.k, 32), (unsigned)t.n_models);
-  if (tall) start_kernel<K, true><<<sg, 256, 0, s>>>(src, sums, sp.chunks, X[0]);
-  else start_kernel<K, false><<<sg, 256, 0, s>>>(src, sums, sp.chunks, X[0]);
+  if (tall) {
+    const int64_t n = ceil_div((int64_t)t.rows * ceil_div(t.cols, 4), 1024);
+    start_kernel<K><<<dim3((unsigned)(n < 1024 ? n : 1024), (unsigned)t.n_models), 256, 0, s>>>(src, sums, sp.chunks, X[0]);
+  } else {
+    start_wide_kernel<K><<<dim3((unsigned)ceil_div(sp.L, 64), (unsigned)ceil_div(sp.k, 64), (unsigned)t.n_models), 256, 0, s>>>(
+        src, sums, sp.chunks, X[0]);
+  }
   if ((err = hipGetLastError()) != hipSuccess) return (int)err;
 
   Prod base = {};
   base.models = t.n_models;
-  base.splits = 1;
+  const Choice small = shape_for(t.n_models, sp.k, sp.k, sp.k, true, false);
+  const Choice apply = shape_for(t.n_models, sp.L, sp.k, sp.k, false, false);
   const double a = t.a, b = t.b, c = t.c;
   double r = 1.;
   int done = 0, x = 0;
@@ -378,16 +704,17 @@ template <Kind K, Epi LAST> int run(const mplc_muon_t& t, const Space& sp, const
     p.a = p.b = X[x];
     p.m = p.n = sp.k;
     p.r = sp.L;
-    p.splits = sp.gram_splits;
-    p.per_split = sp.gram_per_split;
+    p.symmetric = 1;
     p.alpha = A_SCALE / (X_SCALE * X_SCALE);
     p.out = A;
     p.partial = partial;
-    if (p.splits > 1) {
-      if ((err = product<K, true, PARTIAL>(p, s)) != hipSuccess) return (int)err;
-      join_kernel<<<dim3((unsigned)ceil_div((int64_t)sp.k * (sp.ld / 4), 256), (unsigned)t.n_models), 256, 0, s>>>(p);
+    if (sp.gram.splits > 1) {
+      if ((err = product<F32, true, PARTIAL>(p, sp.gram, s)) != hipSuccess) return (int)err;
+      p.splits = sp.gram.splits;
+      const int64_t jt = ceil_div(sp.k, 64);
+      join_kernel<<<dim3((unsigned)(jt * (jt + 1) / 2), (unsigned)t.n_models), 256, 0, s>>>(p);
       if ((err = hipGetLastError()) != hipSuccess) return (int)err;
-    } else if ((err = product<K, true, PLANES>(p, s)) != hipSuccess) {
+    } else if ((err = product<F32, true, PLANES>(p, sp.gram, s)) != hipSuccess) {
       return (int)err;
     }
     auto square = [&](const Planes& l, float ls, const Planes& m, float ms, const Planes& o, float os) {
@@ -395,9 +722,10 @@ template <Kind K, Epi LAST> int run(const mplc_muon_t& t, const Space& sp, const
       q.a = l;
       q.b = m;
       q.m = q.n = q.r = sp.k;
+      q.symmetric = 1;
       q.alpha = os / (ls * ms);
       q.out = o;
-      return product<K, false, PLANES>(q, s);
+      return product<F32, false, PLANES>(q, small, s);
     };
     double qbound = 1.;
     float q_scale = 1.f;
@@ -410,8 +738,9 @@ template <Kind K, Epi LAST> int run(const mplc_muon_t& t, const Space& sp, const
       q.ca = t.a * p_scale;
       q.cb = t.b * (p_scale / A_SCALE);
       q.cc = t.c * (p_scale / (A_SCALE * A_SCALE));
+      q.symmetric = 1;
       q.out = i == 0 ? Q : P;
-      if ((err = product<K, false, POLY>(q, s)) != hipSuccess) return (int)err;
+      if ((err = product<F32, false, POLY>(q, small, s)) != hipSuccess) return (int)err;
       qbound *= pb;
       const Planes& cur = q.out;
       const float new_scale = i == 0 ? p_scale : scale_for(qbound);
@@ -439,7 +768,7 @@ template <Kind K, Epi LAST> int run(const mplc_muon_t& t, const Space& sp, const
     if (ph + 1 < sp.phases) {
       p.alpha = 1.f / q_scale;
       p.out = X[1 - x];
-      err = product<K, false, PLANES>(p, s);
+      err = product<F32, false, PLANES>(p, apply, s);
       x = 1 - x;
     } else {
       p.alpha = 1.f / (X_SCALE * q_scale);
@@ -448,14 +777,14 @@ template <Kind K, Epi LAST> int run(const mplc_muon_t& t, const Space& sp, const
         p.dst = t.out;
         p.dst_stride = t.out_stride;
         p.dst_ld = t.out_ld;
-        err = product<K, false, OUT>(p, s);
+        err = product<K, false, OUT>(p, apply, s);
       } else {
         p.dst = t.w;
         p.dst_stride = t.w_stride;
         p.dst_ld = t.w_ld;
         p.keep = (float)(1. - (double)t.lr * t.weight_decay);
         p.step = t.lr * t.scale;
-        err = product<F32, false, STEP>(p, s);
+        err = product<F32, false, STEP>(p, apply, s);
       }
     }
     if (err != hipSuccess) return (int)err;
@@ -475,7 +804,7 @@ int check(const mplc_muon_t* t, Space& sp) {
   if (t->n_models == 0) return MPLC_OK;
   if (t->g == nullptr || t->g_ld < t->cols) return MPLC_E_ARG;
   if (((uintptr_t)t->workspace & 15) != 0) return MPLC_E_ARG;
-  if (t->workspace == nullptr || t->workspace_bytes < sp.total) return MPLC_E_WORKSPACE;
+  if (sp.total && (t->workspace == nullptr || t->workspace_bytes < sp.total)) return MPLC_E_WORKSPACE;
   return MPLC_OK;
 }
 

@@ -26,10 +26,10 @@ def dense_t(**kw):
 
 def muon_t(**kw):
     t = muon.MuonT()
-    t.n_models, t.rows, t.cols, t.steps = 2, 6, 4, 5
+    t.n_models, t.rows, t.cols, t.steps = 2, 200, 70, 5
     t.a, t.b, t.c = muon.COEFFICIENTS
     t.g = t.out = t.m = t.w = t.workspace = P
-    t.g_ld = t.out_ld = t.m_ld = t.w_ld = 4
+    t.g_ld = t.out_ld = t.m_ld = t.w_ld = 70
     t.workspace_bytes = 1 << 40
     for k, v in kw.items():
         setattr(t, k, v)
@@ -82,21 +82,21 @@ def test_muon_argument_errors():
         assert f(None, None) == E_ARG
         for kw in ({"n_models": -1}, {"n_models": 65536}, {"rows": 0}, {"cols": 0}, {"dtype": 3}, {"steps": 0},
                    {"steps": 17}, {"a": 4.0, "b": -4.0, "c": 3.0}, {"a": float("nan")}, {"c": float("inf")}, {"g": None},
-                   {"g_ld": 3}, {"workspace": P + 4}):
+                   {"g_ld": 69}, {"workspace": P + 4}):
             assert f(ctypes.byref(muon_t(**kw)), None) == E_ARG, kw
         assert f(ctypes.byref(muon_t(workspace_bytes=16)), None) == E_WS
         assert f(ctypes.byref(muon_t(workspace=None)), None) == E_WS
         assert f(ctypes.byref(muon_t(n_models=0)), None) == 0
-    for kw in ({"out": None}, {"out_ld": 3}):
+    for kw in ({"out": None}, {"out_ld": 69}):
         assert lib.mplc_orthogonalize(ctypes.byref(muon_t(**kw)), None) == E_ARG
-    for kw in ({"m": None}, {"w": None}, {"m_ld": 3}, {"w_ld": 3}):
+    for kw in ({"m": None}, {"w": None}, {"m_ld": 69}, {"w_ld": 69}):
         assert lib.mplc_muon_step(ctypes.byref(muon_t(**kw)), None) == E_ARG
 
 
 def test_workspace_sizes_follow_the_sizes():
     lib = muon._lib()
     size = lambda **kw: lib.mplc_muon_step_workspace_bytes(ctypes.byref(muon_t(**kw)))  # noqa: E731
-    assert size(rows=0) == 0 and 0 < size() < size(n_models=20) and size(rows=64, cols=4000) > 64 * 4000 * 2 * 4
+    assert size(rows=0) == 0 and 0 < size() < size(n_models=20) and size(rows=65, cols=4000) > 65 * 4000 * 4 and size(rows=9, cols=32) == 0
 
 
 def test_singular_range():
