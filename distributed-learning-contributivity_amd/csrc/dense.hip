@@ -116,16 +116,15 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
   const int cnt = seg ? p.m : count_of(p.counts, g, p.count_is_r ? p.r : p.m);
   const int M = p.count_is_r ? p.m : cnt, R = p.count_is_r ? cnt : p.r;
   if (m0 >= M) return;
-  // a split's share: models of a sum over models, tiles of r otherwise
   const int nk = (R + B::BK - 1) / B::BK;
-  const int first = split * p.per_split, last = min(seg ? p.segments : nk, first + p.per_split);
+  const int64_t all = (int64_t)nk * p.segments, first = (int64_t)split * p.per_split;
+  const int64_t last = first + p.per_split < all ? first + p.per_split : all;
   const T* pa = reinterpret_cast<const T*>(p.a) + g * p.a_stride;
   const T* pb = reinterpret_cast<const T*>(p.b) + g * p.b_stride;
   B blk;
   blk.clear();
   if (seg) {
-    blk.run(lds, m0, n0, nk, last - first, [&](int s, Operand<T>& a, Operand<T>& o, int& r0, int& rend) {
-      s += first;
+    blk.run(lds, m0, n0, nk, first, last, [&](int s, Operand<T>& a, Operand<T>& o, int& r0, int& rend) {
       a.p[0] = pa + s * p.a_stride;
       o.p[0] = pb + s * p.b_stride;
       a.ld = p.a_ld;
@@ -138,7 +137,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
     });
   } else {
     const Operand<T> a = {{pa, nullptr}, p.a_ld, M}, o = {{pb, nullptr}, p.b_ld, p.n};
-    blk.run(lds, a, o, m0, n0, first * B::BK, min(R, last * B::BK));
+    blk.run(lds, a, o, m0, n0, (int)first * B::BK, (int)min((int64_t)R, last * B::BK));
   }
   if (p.splits > 1) {
     float* out = p.partial + ((int64_t)split * p.models + g) * p.m * p.n;
@@ -250,7 +249,8 @@ bool plan(const mplc_dense_t& t, Form form, Plan& out) {
   p.count_is_r = form == DW;
   const bool f32 = t.dtype == MPLC_DTYPE_F32;
   p.nk = (int)ceil_div(p.r, f32 ? 32 : 64);
-  const int64_t units = p.segments > 1 ? p.segments : p.nk;
+  const int64_t units = (int64_t)p.nk * p.segments;
+  if (units > INT32_MAX) return false;
   const Choice c = choose(f32 ? SHAPES_F32 : SHAPES_16, 5, p.models, p.m, p.n, (int64_t)p.r * p.segments, units, true);
   out.cfg = c.tile;
   p.splits = c.splits;

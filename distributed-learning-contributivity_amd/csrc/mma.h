@@ -346,7 +346,8 @@ template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int F
   // acc += the sum over r of the whole product; A.rows, B.rows > 0
   __device__ __forceinline__ void run(char* lds, const Operand<T>& A, const Operand<T>& B, int m0, int n0, int r0,
                                       int rend) {
-    run(lds, m0, n0, (rend - r0 + BK - 1) / BK, 1, [&](int, Operand<T>& a, Operand<T>& b, int& first, int& end) {
+    const int n = (rend - r0 + BK - 1) / BK;
+    run(lds, m0, n0, n, 0, n, [&](int, Operand<T>& a, Operand<T>& b, int& first, int& end) {
       a = A;
       b = B;
       first = r0;
@@ -355,22 +356,23 @@ template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int F
     });
   }
 
-  // acc += the sum over `segments` pieces of n tiles each: at(s, A, B, r0, rend) says where piece s is and returns how
-  // many rows of A take part in it (the others contribute nothing)
-  template <typename At> __device__ __forceinline__ void run(char* lds, int m0, int n0, int n, int segments, At at) {
+  // acc += the sum over tiles [from, to) of pieces of n tiles each: at(s, A, B, r0, rend) says where piece s is and
+  // returns how many rows of A take part in it (the others contribute nothing)
+  template <typename At>
+  __device__ __forceinline__ void run(char* lds, int m0, int n0, int n, int64_t from, int64_t to, At at) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave / WN, wn = wave % WN;
-    const int all = n * segments;
-    if (all <= 0) return;
+    if (n <= 0 || to <= from) return;
+    const int all = (int)(to - from);
     TA ta;
     TB tb;
     Operand<T> A, B;
-    int r0, rend, rows, t = 0, s = 0;
+    int r0, rend, rows, s = (int)(from / n), t = (int)(from - (int64_t)s * n);
     bool whole_a, whole_b;
     auto seek = [&]() {
       rows = at(s, A, B, r0, rend);
-      ta.seek(A, m0, r0, tid);
-      tb.seek(B, n0, r0, tid);
+      ta.seek(A, m0, r0 + t * BK, tid);
+      tb.seek(B, n0, r0 + t * BK, tid);
       whole_a = m0 + BM <= A.rows || A.rows % TA::CH == 0;
       whole_b = n0 + BN <= B.rows || B.rows % TB::CH == 0;
     };

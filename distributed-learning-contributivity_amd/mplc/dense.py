@@ -9,6 +9,8 @@ stride; the elements of a row are contiguous.  Work goes to torch's current stre
 """
 import ctypes
 
+import torch
+
 from . import _native
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
@@ -34,6 +36,8 @@ class DenseT(ctypes.Structure):
 
 
 _LIB = None
+_PLANS = {}  # what a call's shapes, strides, types and flags were found to need (_Plan); never an address or a value
+MAX_PLANS = 4096
 
 
 def _lib():
@@ -50,17 +54,73 @@ def _lib():
     return _LIB
 
 
+def _sig(t):
+    """Everything about a tensor that its checks look at."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+class _Plan:
+    """A checked call of given shapes: its struct without addresses, the workspace's size, and the bytes each tensor
+    spans (for the overlap check, which needs the addresses)."""
+
+    def __init__(self, lib, name, struct, device, fields, tensors):
+        self.lib, self.name, self.device = lib, name, device
+        self.fn = getattr(lib, name)
+        self.index = device.index
+        self.fields = fields  # (struct field, position among the call's tensors, is an output)
+        self.size = ctypes.sizeof(struct)
+        self.struct = type(struct)
+        self.workspace = int(getattr(lib, name + "_workspace_bytes")(ctypes.byref(struct)))
+        struct.workspace_bytes = self.workspace
+        self.bytes = bytes(struct)
+        self.spans = [_span(t) for t in tensors]
+        self.outs = [i for _, i, out in fields if out and self.spans[i]]
+        self.ins = [i for _, i, out in fields if not out and self.spans[i]]
+        self.models = struct.n_models
+
+    def run(self, tensors, names, same=(), values=()):
+        """Launch on torch's current stream.  same: pairs of positions that may be one and the same tensor; values:
+        further fields of the struct."""
+        p = [0 if t is None else t.data_ptr() for t in tensors]
+        _no_overlap(tensors, names, p, self.spans, self.outs, self.ins, same)
+        st = self.struct.from_buffer_copy(self.bytes)
+        for f, i, _ in self.fields:
+            if p[i]:
+                setattr(st, f, p[i])
+        for f, v in values:
+            setattr(st, f, v)
+        if self.workspace:
+            ws = torch.empty(self.workspace, dtype=torch.uint8, device=self.device)
+            st.workspace = ws.data_ptr()
+        if torch.cuda.current_device() == self.index:
+            status = self.fn(ctypes.byref(st), _raw_stream(self.index))
+        else:
+            with torch.cuda.device(self.index):
+                status = self.fn(ctypes.byref(st), _raw_stream(self.index))
+        if status:
+            _native.check(status, self.name)
+
+
+def _raw_stream(index):
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _remember(key, plan):
+    if len(_PLANS) >= MAX_PLANS:
+        _PLANS.clear()
+    _PLANS[key] = plan
+    return plan
+
+
 def _tensor(t, name, dtype, device, shape):
-    """A strided [models][rows][columns] (or [models][columns]) view the kernels can address; `shape` entries of None
-    are free."""
-    import torch
+    """A strided [models][rows][columns] (or [models][columns]) view the kernels can address."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
-    if t.dim() != len(shape) or any(s is not None and s != d for s, d in zip(shape, t.shape)):
+    if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must have the shape {list(shape)}, not {list(t.shape)}")
     if any(d > MAX_SIZE for d in t.shape):
         raise ValueError(f"{name} is too large: {list(t.shape)}")
@@ -82,19 +142,20 @@ def _writable(t, name):
             raise ValueError(f"the models of {name} overlap (strides {t.stride()})")
 
 
-def _no_overlap(outs, ins):
-    """Outputs may share no memory with an input or with one another (checked on the spans the tensors cover)."""
-    def span(t):
-        n = 1 + sum((d - 1) * s for d, s in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + n * t.element_size()
-    outs = [(n, t) for n, t in outs if t is not None and t.numel()]
-    ins = [(n, t) for n, t in ins if t is not None and t.numel()]
-    for i, (n, t) in enumerate(outs):
-        a, b = span(t)
-        for m, u in outs[i + 1:] + ins:
-            c, d = span(u)
-            if a < d and c < b and not _interleaved(t, u):
-                raise ValueError(f"{n} and {m} share memory")
+def _span(t):
+    """Bytes from a tensor's first element to behind its last."""
+    return 0 if t is None or not t.numel() else \
+        (1 + sum((d - 1) * s for d, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _no_overlap(tensors, names, ptrs, spans, outs, ins, same=()):
+    """Outputs (positions `outs`) may share no memory with an input or with one another."""
+    for k, i in enumerate(outs):
+        a, b = ptrs[i], ptrs[i] + spans[i]
+        for j in outs[k + 1:] + ins:
+            if a < ptrs[j] + spans[j] and ptrs[j] < b and not _interleaved(tensors[i], tensors[j]):
+                if not ((i, j) in same and a == ptrs[j] and tensors[i].stride() == tensors[j].stride()):
+                    raise ValueError(f"{names[i]} and {names[j]} share memory")
 
 
 def _interleaved(t, u):
@@ -108,6 +169,8 @@ def _interleaved(t, u):
     base = min(t.data_ptr(), u.data_ptr())
     places = []
     for v in (t, u):
+        if (v.data_ptr() - base) % size:
+            return False
         start = (v.data_ptr() - base) // size % s
         n = 1 + sum((d - 1) * k for d, k in zip(v.shape[1:], v.stride()[1:]))
         places.append((start, start + n))
@@ -119,9 +182,12 @@ def _ld(t):
     return max(t.stride(1), t.shape[2]) if t.shape[1] > 1 else t.shape[2]
 
 
+def _three(t):
+    return t if t is None or t.dim() != 2 else t.unsqueeze(0)
+
+
 def _setup(x, w, activation, counts):
-    """The struct's sizes, and the shapes: (t, G, B, K, N, x as [1 or G, B, K])."""
-    import torch
+    """The struct's sizes and the shapes (t, G, B, K, N)."""
     if not isinstance(x, torch.Tensor) or not isinstance(w, torch.Tensor):
         raise TypeError("x and w must be tensors")
     if not w.is_cuda:
@@ -142,7 +208,7 @@ def _setup(x, w, activation, counts):
         raise ValueError(f"x must be [models, rows, in], or [1, rows, in] or [rows, in] shared by all models, "
                          f"not {list(x.shape)}")
     shared = x.dim() == 2 or (x.shape[0] == 1 and G != 1)
-    x3 = x.unsqueeze(0) if x.dim() == 2 else x
+    x3 = _three(x)
     B = x3.shape[1]
     _tensor(x3, "x", w.dtype, w.device, (1 if shared else G, B, K))
     if counts is not None:
@@ -150,26 +216,43 @@ def _setup(x, w, activation, counts):
     t = DenseT()
     t.n_models, t.rows, t.in_, t.out = G, B, K, N
     t.dtype, t.activation, t.x_shared = DTYPES[str(w.dtype)], ACTIVATIONS[activation], int(shared)
-    t.counts = None if counts is None else counts.data_ptr()
-    t.x, t.x_stride, t.x_ld = x3.data_ptr(), (0 if shared else x3.stride(0)), _ld(x3)
-    t.w, t.w_stride, t.w_ld = w.data_ptr(), w.stride(0), _ld(w)
-    return t, G, B, K, N, x3
+    t.x_stride, t.x_ld = (0 if shared else x3.stride(0)), _ld(x3)
+    t.w_stride, t.w_ld = w.stride(0), _ld(w)
+    return t, G, B, K, N
 
 
 def _place(t, field, tensor):
-    setattr(t, field, tensor.data_ptr())
     setattr(t, field + "_stride", tensor.stride(0))
     if tensor.dim() == 3:
         setattr(t, field + "_ld", _ld(tensor))
 
 
-def _run(lib, name, t, device):
-    import torch
-    n = getattr(lib, name + "_workspace_bytes")(ctypes.byref(t))
-    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-    t.workspace, t.workspace_bytes = (ws.data_ptr() if n else None), n
-    with torch.cuda.device(device):
-        _native.check(getattr(lib, name)(ctypes.byref(t), _native.stream_handle(device)), name)
+_FORWARD = ("out", "preact", "x", "w", "bias", "residual", "counts")
+_FORWARD_FIELDS = (("y", 0, True), ("z", 1, True), ("x", 2, False), ("w", 3, False), ("bias", 4, False),
+                   ("residual", 5, False), ("counts", 6, False))
+
+
+def _plan_forward(key, out, preact, x, w, bias, residual, counts, activation):
+    t, G, B, K, N = _setup(x, w, activation, counts)
+    dev, dt = w.device, w.dtype
+    if bias is not None:
+        _tensor(bias, "bias", dt, dev, (G, N))
+        t.bias_stride = bias.stride(0)
+    if residual is not None:
+        _tensor(residual, "residual", dt, dev, (G, B, N))
+        _place(t, "residual", residual)
+    if out is not None:
+        _tensor(out, "out", dt, dev, (G, B, N))
+        _writable(out, "out")
+    if preact is not None:
+        _tensor(preact, "preact", torch.float32, dev, (G, B, N))
+        _writable(preact, "preact")
+        _place(t, "z", preact)
+    if out is None:
+        out = torch.empty((G, B, N), dtype=dt, device=dev)
+    _place(t, "y", out)
+    return _remember(key, _Plan(_lib(), "mplc_dense_forward", t, dev, _FORWARD_FIELDS,
+                                (out, preact, _three(x), w, bias, residual, counts)))
 
 
 def dense_forward(x, w, bias=None, residual=None, activation="none", counts=None, preact=None, out=None):
@@ -180,29 +263,68 @@ def dense_forward(x, w, bias=None, residual=None, activation="none", counts=None
     batch (clamped to [0, B]); rows behind a model's count are not read, and those of `out` and `preact` stay as they
     are.  preact (float32 [G, B, N]): receives x @ w + bias, which dense_backward needs for an activation.
     Returns out [G, B, N] (allocated where not given; then rows behind a count are 0)."""
-    import torch
-    t, G, B, K, N, x3 = _setup(x, w, activation, counts)
-    dev, dt = w.device, w.dtype
-    if bias is not None:
-        _tensor(bias, "bias", dt, dev, (G, N))
-        t.bias, t.bias_stride = bias.data_ptr(), bias.stride(0)
-    if residual is not None:
-        _tensor(residual, "residual", dt, dev, (G, B, N))
-        _place(t, "residual", residual)
+    try:
+        key = (0, activation, _sig(x), _sig(w), _sig(bias), _sig(residual), _sig(counts), _sig(preact), _sig(out))
+        plan = _PLANS.get(key)
+    except (AttributeError, TypeError):  # not tensors: the checks say so
+        key = plan = None
+    if plan is None:
+        plan = _plan_forward(key, out, preact, x, w, bias, residual, counts, activation)
     if out is None:
-        out = (torch.empty if counts is None else torch.zeros)((G, B, N), dtype=dt, device=dev)
-    _tensor(out, "out", dt, dev, (G, B, N))
-    _writable(out, "out")
-    _place(t, "y", out)
-    if preact is not None:
-        _tensor(preact, "preact", torch.float32, dev, (G, B, N))
-        _writable(preact, "preact")
-        _place(t, "z", preact)
-    _no_overlap([("out", out), ("preact", preact)],
-                [("x", x3), ("w", w), ("bias", bias), ("residual", residual), ("counts", counts)])
-    if G and B:
-        _run(_lib(), "mplc_dense_forward", t, dev)
+        out = (torch.empty if counts is None else torch.zeros)((w.shape[0], x.shape[-2], w.shape[2]), dtype=w.dtype,
+                                                               device=w.device)
+    plan.run((out, preact, x, w, bias, residual, counts), _FORWARD)
     return out
+
+
+_BACKWARD = ("dx", "dw", "db", "x", "w", "dout", "preact", "counts")
+_BACKWARD_FIELDS = (("dx", 0, True), ("dw", 1, True), ("db", 2, True), ("x", 3, False), ("w", 4, False),
+                    ("dy", 5, False), ("z", 6, False), ("counts", 7, False))
+
+
+def _plan_backward(key, dx, dw, db, x, w, dout, preact, counts, activation, need):
+    t, G, B, K, N = _setup(x, w, activation, counts)
+    dev, dt = w.device, w.dtype
+    if any(n not in ("dx", "dw", "db") for n in need):
+        raise ValueError(f"need holds 'dx', 'dw' and 'db' only, not {need}")
+    _tensor(dout, "dout", dt, dev, (G, B, N))
+    _place(t, "dy", dout)
+    if activation != "none":
+        if preact is None:
+            raise ValueError(f"the gradient of '{activation}' needs preact (dense_forward(..., preact=))")
+        _tensor(preact, "preact", torch.float32, dev, (G, B, N))
+        _place(t, "z", preact)
+    x3 = _three(x)
+    if "dx" in need:
+        if dx is not None:
+            if not isinstance(dx, torch.Tensor):
+                raise TypeError("dx must be a tensor")
+            if dx.dim() != x.dim():
+                raise ValueError(f"dx must have the shape {list(x.shape)}, not {list(dx.shape)}")
+            _tensor(_three(dx), "dx", dt, dev, tuple(x3.shape))
+            _writable(_three(dx), "dx")
+        else:
+            dx = torch.empty(x.shape, dtype=dt, device=dev)
+        _place(t, "dx", _three(dx))
+        t.dx = 16  # wanted: the workspace query looks at that alone
+    else:
+        dx = None
+    for name, field, v, shape in (("dw", "dw", dw, (G, K, N)), ("db", "db", db, (G, N))):
+        if name in need:
+            if v is not None:
+                _tensor(v, name, dt, dev, shape)
+                _writable(v, name)
+            else:
+                v = torch.empty(shape, dtype=dt, device=dev)
+            _place(t, field, v)
+            setattr(t, field, 16)
+            if name == "dw":
+                dw = v
+            else:
+                db = v
+    plan = _Plan(_lib(), "mplc_dense_backward", t, dev, _BACKWARD_FIELDS,
+                 (_three(dx), dw, db, x3, w, dout, preact if activation != "none" else None, counts))
+    return _remember(key, plan)
 
 
 def dense_backward(dout, x, w, preact=None, activation="none", counts=None, need=("dx", "dw", "db"), dx=None, dw=None,
@@ -213,47 +335,24 @@ def dense_backward(dout, x, w, preact=None, activation="none", counts=None, need
     the models.  need: which of the three are computed (the others are None).  dx, dw, db may be given; where dx is
     allocated here, rows behind a model's count are 0, and a given dx keeps them (a shared x has no such rows: a row that
     no model reaches gets 0)."""
-    import torch
-    t, G, B, K, N, x3 = _setup(x, w, activation, counts)
-    dev, dt = w.device, w.dtype
     need = tuple(need)
-    if any(n not in ("dx", "dw", "db") for n in need):
-        raise ValueError(f"need holds 'dx', 'dw' and 'db' only, not {need}")
-    _tensor(dout, "dout", dt, dev, (G, B, N))
-    _place(t, "dy", dout)
-    if activation != "none":
-        if preact is None:
-            raise ValueError(f"the gradient of '{activation}' needs preact (dense_forward(..., preact=))")
-        _tensor(preact, "preact", torch.float32, dev, (G, B, N))
-        _place(t, "z", preact)
-    if "dx" in need:
-        if dx is None:
-            dx = (torch.empty if counts is None and G else torch.zeros)(x.shape, dtype=dt, device=dev)
-        if dx.dim() != x.dim():
-            raise ValueError(f"dx must have the shape {list(x.shape)}, not {list(dx.shape)}")
-        dx3 = dx.unsqueeze(0) if dx.dim() == 2 else dx
-        _tensor(dx3, "dx", dt, dev, tuple(x3.shape))
-        _writable(dx3, "dx")
-        _place(t, "dx", dx3)
-    else:
-        dx = dx3 = None
-    if "dw" in need:
-        dw = torch.empty((G, K, N), dtype=dt, device=dev) if dw is None else dw
-        _tensor(dw, "dw", dt, dev, (G, K, N))
-        _writable(dw, "dw")
-        _place(t, "dw", dw)
-    else:
-        dw = None
-    if "db" in need:
-        db = torch.empty((G, N), dtype=dt, device=dev) if db is None else db
-        _tensor(db, "db", dt, dev, (G, N))
-        _writable(db, "db")
-        t.db, t.db_stride = db.data_ptr(), db.stride(0)
-    else:
-        db = None
-    _no_overlap([("dx", dx3), ("dw", dw), ("db", db)],
-                [("x", x3), ("w", w), ("dout", dout), ("preact", preact if activation != "none" else None),
-                 ("counts", counts)])
+    dx, dw, db = (v if n in need else None for n, v in (("dx", dx), ("dw", dw), ("db", db)))
+    if activation == "none":
+        preact = None
+    try:
+        key = (1, activation, need, _sig(dout), _sig(x), _sig(w), _sig(preact), _sig(counts), _sig(dx), _sig(dw), _sig(db))
+        plan = _PLANS.get(key)
+    except (AttributeError, TypeError):
+        key = plan = None
+    if plan is None:
+        plan = _plan_backward(key, dx, dw, db, x, w, dout, preact, counts, activation, need)
+    G = w.shape[0]
+    if dx is None and "dx" in need:
+        dx = (torch.empty if counts is None and G else torch.zeros)(x.shape, dtype=w.dtype, device=w.device)
+    if dw is None and "dw" in need:
+        dw = torch.empty(w.shape, dtype=w.dtype, device=w.device)
+    if db is None and "db" in need:
+        db = torch.empty((G, w.shape[2]), dtype=w.dtype, device=w.device)
     if G and need:
-        _run(_lib(), "mplc_dense_backward", t, dev)
+        plan.run((dx, dw, db, x, w, dout, preact, counts), _BACKWARD)
     return dx, dw, db

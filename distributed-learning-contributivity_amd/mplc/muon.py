@@ -8,8 +8,10 @@ round's average (``CoalitionEngine(server_optimizer=...)``).  Work goes to torch
 import ctypes
 import math
 
+import torch
+
 from . import _native
-from .dense import DTYPES, _ld, _no_overlap, _place, _run, _tensor, _writable
+from .dense import _PLANS, DTYPES, _Plan, _ld, _place, _remember, _sig, _tensor, _three, _writable
 
 # a s + b s^3 + c s^5 per step: takes singular values of 0.01 .. 1 to about 0.7 .. 1.2 in five steps
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
@@ -33,7 +35,7 @@ _LIB = None
 
 
 class _Lib:
-    """The two calls under the names _run uses, with their one workspace query."""
+    """The two calls under the names a plan uses, with their one workspace query."""
 
     def __init__(self, lib):
         self.mplc_orthogonalize, self.mplc_muon_step = lib.mplc_orthogonalize, lib.mplc_muon_step
@@ -71,7 +73,6 @@ def singular_range(steps, coefficients):
 
 
 def _setup(g, name, steps, coefficients):
-    import torch
     if not isinstance(g, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     if not g.is_cuda:
@@ -80,7 +81,7 @@ def _setup(g, name, steps, coefficients):
         raise ValueError(f"{name} must be float32, bfloat16 or float16, not {g.dtype}")
     if g.dim() not in (2, 3):
         raise ValueError(f"{name} must be [models, rows, cols] or [rows, cols], not {list(g.shape)}")
-    g3 = g if g.dim() == 3 else g.unsqueeze(0)
+    g3 = _three(g)
     G, m, n = g3.shape
     if m < 1 or n < 1:
         raise ValueError(f"{name} has no elements: {list(g.shape)}")
@@ -97,34 +98,65 @@ def _setup(g, name, steps, coefficients):
     t = MuonT()
     t.n_models, t.rows, t.cols, t.dtype, t.steps = G, m, n, DTYPES[str(g.dtype)], int(steps)
     t.a, t.b, t.c = coefficients
-    t.g, t.g_stride, t.g_ld = g3.data_ptr(), g3.stride(0), _ld(g3)
+    _place(t, "g", g3)
     return t, g3
+
+
+def _key(kind, steps, coefficients, tensors):
+    try:
+        return (kind, steps, tuple(coefficients)) + tuple(_sig(t) for t in tensors)
+    except (AttributeError, TypeError):  # not tensors, not numbers: the checks say so
+        return None
+
+
+def _plan_orthogonalize(key, out, g, steps, coefficients):
+    t, g3 = _setup(g, "g", steps, coefficients)
+    if out is None:
+        out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+    if not isinstance(out, torch.Tensor):
+        raise TypeError("out must be a tensor")
+    if out.dim() != g.dim():
+        raise ValueError(f"out must have the shape {list(g.shape)}, not {list(out.shape)}")
+    _tensor(_three(out), "out", g.dtype, g.device, tuple(g3.shape))
+    _writable(_three(out), "out")
+    _place(t, "out", _three(out))
+    return _remember(key, _Plan(_lib(), "mplc_orthogonalize", t, g.device, (("out", 0, True), ("g", 1, False)),
+                                (_three(out), g3)))
 
 
 def orthogonalize(g, steps=STEPS, coefficients=COEFFICIENTS, out=None):
     """Each matrix of g ([G, m, n] or [m, n]) divided by its Frobenius norm, then `steps` times
     X <- a X + b (X X^T) X + c (X X^T)^2 X.  A zero matrix stays zero; one with an infinity or a NaN becomes NaN.
-    Sums and intermediate matrices keep fp32's accuracy whatever g's type; the result is rounded to it once."""
-    import torch
-    t, g3 = _setup(g, "g", steps, coefficients)
+    Sums and intermediate matrices keep fp32's accuracy whatever g's type; the result is rounded to it once.
+    out may be g itself."""
+    key = _key(2, steps, coefficients, (g, out))
+    plan = _PLANS.get(key) if key is not None else None
+    if plan is None:
+        plan = _plan_orthogonalize(key, out, g, steps, coefficients)
     if out is None:
         out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
-    if out.dim() != g.dim():
-        raise ValueError(f"out must have the shape {list(g.shape)}, not {list(out.shape)}")
-    o3 = out if out.dim() == 3 else out.unsqueeze(0)
-    _tensor(o3, "out", g.dtype, g.device, tuple(g3.shape))
-    _writable(o3, "out")
-    _place(t, "out", o3)
-    if not (out.data_ptr() == g.data_ptr() and out.stride() == g.stride()):  # in place is fine: g is read first
-        _no_overlap([("out", o3)], [("g", g3)])
-    if t.n_models:
-        _run(_lib(), "mplc_orthogonalize", t, g.device)
+    if plan.models:
+        plan.run((out, g), ("out", "g"), same=((0, 1),))  # in place: g is read before anything is written
     return out
 
 
 def update_scale(rows, cols):
     """sqrt(max(1, out / in)) of an [in][out] matrix: a step's size per output does not depend on the shape."""
     return math.sqrt(max(1.0, cols / rows))
+
+
+def _plan_step(key, w, grad, momentum, steps, coefficients):
+    t, g3 = _setup(grad, "grad", steps, coefficients)
+    for name, field, v in (("w", "w", w), ("momentum", "m", momentum)):
+        if not isinstance(v, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor")
+        if v.shape != grad.shape:
+            raise ValueError(f"{name} must have the shape {list(grad.shape)}, not {list(v.shape)}")
+        _tensor(_three(v), name, torch.float32, grad.device, tuple(g3.shape))
+        _writable(_three(v), name)
+        _place(t, field, _three(v))
+    return _remember(key, _Plan(_lib(), "mplc_muon_step", t, grad.device, (("w", 0, True), ("m", 1, True), ("g", 2, False)),
+                                (_three(w), _three(momentum), g3)))
 
 
 def muon_step(w, grad, momentum, lr, beta=0.95, nesterov=True, weight_decay=0.0, steps=STEPS,
@@ -135,25 +167,16 @@ def muon_step(w, grad, momentum, lr, beta=0.95, nesterov=True, weight_decay=0.0,
         w <- (1 - lr weight_decay) w - lr scale orthogonalize(u)
 
     w and momentum are float32, grad any supported type; scale None: update_scale(in, out).  Returns w."""
-    import torch
-    t, g3 = _setup(grad, "grad", steps, coefficients)
-    for name, v in (("w", w), ("momentum", momentum)):
-        if not isinstance(v, torch.Tensor):
-            raise TypeError(f"{name} must be a tensor")
-        if v.shape != grad.shape:
-            raise ValueError(f"{name} must have the shape {list(grad.shape)}, not {list(v.shape)}")
-    w3, m3 = (w, momentum) if w.dim() == 3 else (w.unsqueeze(0), momentum.unsqueeze(0))
-    for name, field, v in (("w", "w", w3), ("momentum", "m", m3)):
-        _tensor(v, name, torch.float32, grad.device, tuple(g3.shape))
-        _writable(v, name)
-        _place(t, field, v)
-    _no_overlap([("w", w3), ("momentum", m3)], [("grad", g3)])
-    scale = update_scale(t.rows, t.cols) if scale is None else float(scale)
-    values = {"lr": float(lr), "beta": float(beta), "weight_decay": float(weight_decay), "scale": scale}
-    if not all(math.isfinite(v) for v in values.values()):
-        raise ValueError(f"lr, beta, weight_decay and scale must be finite: {values}")
-    t.nesterov = int(bool(nesterov))
-    t.lr, t.beta, t.weight_decay, t.scale = float(lr), float(beta), float(weight_decay), scale
-    if t.n_models:
-        _run(_lib(), "mplc_muon_step", t, grad.device)
+    key = _key(3, steps, coefficients, (w, grad, momentum))
+    plan = _PLANS.get(key) if key is not None else None
+    if plan is None:
+        plan = _plan_step(key, w, grad, momentum, steps, coefficients)
+    rows, cols = grad.shape[-2:]
+    scale = update_scale(rows, cols) if scale is None else float(scale)
+    lr, beta, weight_decay = float(lr), float(beta), float(weight_decay)
+    if not math.isfinite(lr * scale) or not math.isfinite(beta) or not math.isfinite(lr * weight_decay):
+        raise ValueError(f"lr, beta, weight_decay and scale must be finite: {lr}, {beta}, {weight_decay}, {scale}")
+    if plan.models:
+        plan.run((w, momentum, grad), ("w", "momentum", "grad"), values=(
+            ("lr", lr), ("beta", beta), ("weight_decay", weight_decay), ("scale", scale), ("nesterov", int(bool(nesterov)))))
     return w

@@ -118,12 +118,18 @@ def test_host_checks_refuse_cpu_tensors():
 
 
 def test_memory_overlap_checks():
+    def check(out, other, same=()):
+        ts = (out, other)
+        dense._no_overlap(ts, ("out", "other"), [t.data_ptr() for t in ts], [dense._span(t) for t in ts], [0], [1], same)
     rows = torch.zeros(3, 100)
     a, b, c = (rows[:, o:o + 12].view(3, 3, 4) for o in (0, 12, 20))
-    dense._no_overlap([("a", a)], [("b", b)])
+    check(a, b)
+    check(a, a, same=((0, 1),))
     for p, q in ((a, a), (b, c), (a, rows)):
         with pytest.raises(ValueError, match="share memory"):
-            dense._no_overlap([("p", p)], [("q", q)])
+            check(p, q)
+    with pytest.raises(ValueError, match="share memory"):
+        check(b, c, same=((0, 1),))
     dense._writable(a, "a")
     dense._writable(torch.zeros(5, 3, 4).transpose(0, 1), "beside")
     for t in (torch.zeros(1, 3, 4).expand(2, 3, 4), torch.zeros(40).as_strided((2, 3, 4), (6, 5, 1))):
