@@ -516,6 +516,489 @@ template <Kind K, int KT, Epi E> __global__ __launch_bounds__(256) void small_ke
   }
 }
 
+// ------------------------------------------------------------------------------------------ narrow matrices: k <= 128
+// U is read three times and nothing of its size but the result is written: the Gram matrix of U itself (whose trace is
+// |U|^2: no pass for the norm), the Gram matrix of U Q1 formed on the way, and the result U (Q1 Q2).  What is between runs
+// on one workgroup per model with all k x k matrices in LDS.  Bound by HBM: 128 KB of matrix per workgroup need 1.2 to
+// 2.3 thousand cycles of matrix instructions and 7.7 thousand of HBM.
+// KP: k padded to 64 or 128; a workgroup of 8 waves takes TR = 16384 / KP rows l of X at a time, the next ones on their
+// way in registers.  TALL: L = rows.  Before |U| is known, a workgroup scales by a power of two that it raises (with what
+// it has summed) when a larger value comes: split fp16 holds any range.
+constexpr int NARROW_THREADS = 512;
+
+struct Narrow {
+  Source src;
+  int L, k, chunks, rows_per;  // chunks per model, rows l of one
+  float* partial;              // [model][chunk][tile][1024]
+  int* exponent;               // [model][chunk]
+  double* inv;                 // [model] 1 / |U|
+  Planes q;                    // [model] Q in the square layout of LDS
+  float q_scale;
+  void* dst;
+  int64_t dst_stride, dst_ld;
+  float keep, step;
+};
+
+// an LDS matrix of 16-bit elements with rows of RB bytes, read along its rows (chunks of 16 bytes exchanged by row)
+template <int RB> __device__ __forceinline__ int along(int row, int elem) {
+  const int s = RB >= 256 ? row & 15 : (row >> 1) & 7;
+  return row * RB + (((elem >> 3) ^ s) << 4) + (elem & 7) * 2;
+}
+template <int RB> __device__ __forceinline__ u32x4 frag_along(const char* m, int row, int ks, int lane) {
+  return *reinterpret_cast<const u32x4*>(m + along<RB>(row + (lane & 31), (2 * ks + (lane >> 5)) * 8));
+}
+// read across its rows (rows of RB + 64 bytes)
+template <int RB> __device__ __forceinline__ u32x4 frag_across(const char* m, int i, int ks, int lane) {
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  const int q = lane & 15, r = (2 * ks + (lane >> 5)) * 8 + (q >> 2);
+  const char* a = m + r * (RB + 64) + (i + (lane & 16) + 4 * (q & 3)) * 2;
+  const u32x2 w0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a)));
+  const u32x2 w1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 4 * (RB + 64))));
+  u32x4 v;
+  v[0] = w0[0]; v[1] = w0[1]; v[2] = w1[0]; v[3] = w1[1];
+  return v;
+}
+__device__ __forceinline__ void put_split(char* hi, char* lo, f32x4 v) {
+  uint16_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split(v[i], h[i], l[i]);
+  u32x2 a, b;
+  a[0] = h[0] | (uint32_t)h[1] << 16;
+  a[1] = h[2] | (uint32_t)h[3] << 16;
+  b[0] = l[0] | (uint32_t)l[1] << 16;
+  b[1] = l[2] | (uint32_t)l[3] << 16;
+  *reinterpret_cast<u32x2*>(hi) = a;
+  *reinterpret_cast<u32x2*>(lo) = b;
+}
+__device__ __forceinline__ void mfma3(f32x16& d, const u32x4* a, const u32x4* b) {  // a, b: hi and lo
+  mfma<F16>(d, b[1], a[0], 0);
+  mfma<F16>(d, b[0], a[1], 0);
+  mfma<F16>(d, b[0], a[0], 0);
+}
+
+// TR rows l of U in registers, as 4-element pieces of U's rows
+template <Kind K, int KP, bool TALL> struct Piece {
+  static constexpr int TR = 16384 / KP, N = 16384 / 4 / NARROW_THREADS;
+  static constexpr int RB = (TALL ? KP : TR) * 2;            // a stored row
+  static constexpr int ACROSS = (TALL ? TR : KP) * (RB + 64);  // bytes of a plane
+  static constexpr int ALONG = (TALL ? TR : KP) * RB;
+  f32x4 u[N];
+  static __device__ __forceinline__ void place(int j, int& row, int& col) {  // of the stored tile
+    constexpr int PER = RB / 8;
+    const int c = threadIdx.x + j * NARROW_THREADS;
+    row = c / PER;
+    col = (c % PER) * 4;
+  }
+  template <bool FIRST> __device__ __forceinline__ void load(const Source& s, int g, int l0, int lend, int k) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      int row, col;
+      place(j, row, col);
+      const int r = TALL ? l0 + row : row, c = TALL ? col : l0 + col;
+      const int rend = TALL ? lend : k, cend = TALL ? k : lend;
+      u[j] = r < rend && c < cend ? update4<K, FIRST>(s, g, r, c, cend - c) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // planes for a sum over l (GRAM) or over k: whichever of the stored rows' directions that is
+  template <bool GRAM, typename F> __device__ __forceinline__ void store(char* lds, F scaled) const {
+    constexpr bool IS_ACROSS = GRAM == TALL;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      int row, col;
+      place(j, row, col);
+      const int at = IS_ACROSS ? row * (RB + 64) + col * 2 : along<RB>(row, col);
+      f32x4 v = u[j];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = scaled(v[e]);
+      put_split(lds + at, lds + (IS_ACROSS ? ACROSS : ALONG) + at, v);
+    }
+  }
+};
+
+// Gram tiles of 32 x 32 at and below the diagonal, at most 3 per wave; KP = 64: every wave has all 3 and its own l,
+// KP = 128: two groups of 4 waves halve the l
+template <int KP> struct GramTiles {
+  static constexpr int TILES = KP == 128 ? 10 : 3, GROUPS = KP == 128 ? 2 : 8, STEP = KP == 128 ? 4 : 1;
+  static constexpr int KS = 16384 / KP / 16 / GROUPS;  // k-steps of a wave
+  f32x16 acc[3];
+  int ti[3], tj[3], n, group;
+  __device__ __forceinline__ void init() {
+    const int wave = threadIdx.x >> 6, member = KP == 128 ? wave & 3 : 0;
+    group = KP == 128 ? wave >> 2 : wave;
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const int t = member + i * STEP;
+      ti[i] = tj[i] = 0;
+      if (t < TILES) {
+        lower_tile(t, ti[i], tj[i]);
+        n = i + 1;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+    }
+  }
+  // frag(plane, i, ks): of rows i .. i + 31 of X^T
+  template <typename F> __device__ __forceinline__ void add(F frag) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int ks = group * KS + s;
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (i < n) {
+          const u32x4 a[2] = {frag(0, ti[i] * 32, ks), frag(1, ti[i] * 32, ks)};
+          const u32x4 b[2] = {frag(0, tj[i] * 32, ks), frag(1, tj[i] * 32, ks)};
+          mfma3(acc[i], a, b);
+        }
+    }
+  }
+  // the groups' sums, added in order, to out [tile][1024]: value (m, n) of a tile at lane (m | ..) * 16 + ..
+  __device__ __forceinline__ void finish(char* lds, float* out) {
+    float* buf = reinterpret_cast<float*>(lds);
+    const int lane = threadIdx.x & 63, member = KP == 128 ? (threadIdx.x >> 6) & 3 : 0;
+    for (int gr = 0; gr < GROUPS; ++gr) {
+      __syncthreads();
+      if (group == gr)
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (i < n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              f32x4* at = reinterpret_cast<f32x4*>(buf + (member + i * STEP) * 1024 + q * 256 + lane * 4);
+              f32x4 v;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = acc[i][4 * q + e];
+              *at = gr ? *at + v : v;
+            }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x * 4; i < TILES * 1024; i += NARROW_THREADS * 4)
+      *reinterpret_cast<f32x4*>(out + i) = *reinterpret_cast<const f32x4*>(buf + i);
+  }
+};
+
+// pass 1: the momentum; partial Gram matrices of U
+template <Kind K, int KP, bool TALL> __global__ __launch_bounds__(NARROW_THREADS) void narrow_gram_kernel(const Narrow p) {
+  typedef Piece<K, KP, TALL> Pc;
+  constexpr int BYTES = 2 * (TALL ? Pc::ACROSS : Pc::ALONG), SUM = GramTiles<KP>::TILES * 4096;
+  __shared__ __attribute__((aligned(16))) char lds[BYTES > SUM ? BYTES : SUM];
+  __shared__ float most[8];
+  const int g = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 63;
+  const int begin = chunk * p.rows_per, end = min(p.L, begin + p.rows_per);
+  Pc pc;
+  GramTiles<KP> gt;
+  gt.init();
+  int exponent = -300;  // values are below 2^(exponent + 14); nothing seen yet
+  pc.template load<true>(p.src, g, begin, end, p.k);
+  for (int l0 = begin; l0 < end; l0 += Pc::TR) {
+    float mx = 0.f;
+#pragma unroll
+    for (int j = 0; j < Pc::N; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(pc.u[j][e]));
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
+    if (lane == 0) most[threadIdx.x >> 6] = mx;
+    __syncthreads();  // also: the last tile's planes are read
+#pragma unroll
+    for (int w = 0; w < 8; ++w) mx = fmaxf(mx, most[w]);
+    int e;
+    frexpf(mx, &e);  // mx < 2^e
+    e = mx > 0.f ? (mx < INFINITY ? e : 128) - 14 : -300;
+    if (e > exponent) {
+      if (exponent > -300)
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) gt.acc[i][v] = ldexpf(gt.acc[i][v], 2 * (exponent - e));
+      exponent = e;
+    }
+    const int down = exponent > -300 ? -exponent : 0;
+    pc.template store<true>(lds, [&](float v) { return ldexpf(v, down); });
+    __syncthreads();
+    if (l0 + Pc::TR < end) pc.template load<true>(p.src, g, l0 + Pc::TR, end, p.k);
+    gt.add([&](int plane, int i, int ks) {
+      if constexpr (TALL) return frag_across<Pc::RB>(lds + plane * Pc::ACROSS, i, ks, lane);
+      else return frag_along<Pc::RB>(lds + plane * Pc::ALONG, i, ks, lane);
+    });
+  }
+  const int64_t slot = (int64_t)g * p.chunks + chunk;
+  gt.finish(lds, p.partial + slot * (GramTiles<KP>::TILES * 1024));
+  if (threadIdx.x == 0) p.exponent[slot] = exponent;
+}
+
+// Q (planes in the square layout) to LDS
+template <int KP> __device__ __forceinline__ void load_square(char* lds, const Planes& q, int g) {
+  constexpr int BYTES = KP * KP * 2;
+  for (int i = threadIdx.x * 16; i < BYTES; i += blockDim.x * 16) {
+    *reinterpret_cast<u32x4*>(lds + i) = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(q.hi + g * q.stride) + i);
+    *reinterpret_cast<u32x4*>(lds + BYTES + i) = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(q.lo + g * q.stride) + i);
+  }
+}
+
+// passes 2 and 3: Y = U Q / |U| by TR rows.  GRAM: partial Gram matrices of Y; otherwise Y is the result.
+template <Kind K, int KP, bool TALL, bool GRAM, Epi E>
+__global__ __launch_bounds__(NARROW_THREADS) void narrow_apply_kernel(const Narrow p) {
+  typedef Piece<K, KP, TALL> Pc;
+  constexpr int TR = Pc::TR, QB = KP * KP * 2, YB = TR * (KP * 2 + 64);
+  constexpr int XB = TALL ? Pc::ALONG : Pc::ACROSS;  // a plane of U
+  constexpr int OUT_LD = TALL ? 68 : 36, OUT = 8 * (TALL ? 32 : 64) * OUT_LD * 4;
+  constexpr int A = 2 * XB, B = GRAM ? 2 * YB : OUT, SUM = GRAM ? GramTiles<KP>::TILES * 4096 : 0;
+  constexpr int REST = A > B ? A : B;
+  __shared__ __attribute__((aligned(16))) char lds[2 * QB + (REST > SUM ? REST : SUM)];
+  char* const xs = lds + 2 * QB;
+  const int g = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int begin = chunk * p.rows_per, end = min(p.L, begin + p.rows_per);
+  const int wr = KP == 128 ? wave >> 1 : wave, wc = KP == 128 ? wave & 1 : 0;  // 32 rows l, 64 columns
+  const double inv = p.inv[g] * (double)X_SCALE;
+  const float back = GRAM ? 1.f / p.q_scale : 1.f / (X_SCALE * p.q_scale);
+  Pc pc;
+  GramTiles<KP> gt;
+  if constexpr (GRAM) gt.init();
+  pc.template load<false>(p.src, g, begin, end, p.k);
+  load_square<KP>(lds, p.q, g);
+  for (int l0 = begin; l0 < end; l0 += TR) {
+    __syncthreads();  // the last tile is done with
+    pc.template store<false>(xs, [&](float v) { return (float)((double)v * inv); });
+    __syncthreads();
+    if (l0 + TR < end) pc.template load<false>(p.src, g, l0 + TR, end, p.k);
+    f32x16 acc[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KP / 16; ++ks) {
+      u32x4 x[2];
+#pragma unroll
+      for (int pl = 0; pl < 2; ++pl) {
+        if constexpr (TALL) x[pl] = frag_along<Pc::RB>(xs + pl * XB, wr * 32, ks, lane);
+        else x[pl] = frag_across<Pc::RB>(xs + pl * XB, wr * 32, ks, lane);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const u32x4 q[2] = {frag_along<KP * 2>(lds, wc * 64 + j * 32, ks, lane), frag_along<KP * 2>(lds + QB, wc * 64 + j * 32, ks, lane)};
+        // a lane gets 4 consecutive columns of a row l; the result of a wide matrix: 4 consecutive l of a column
+        if (GRAM || TALL) mfma3(acc[j], x, q);
+        else mfma3(acc[j], q, x);
+      }
+    }
+    __syncthreads();  // U is read: its place takes Y
+    if constexpr (GRAM) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[j][4 * q + e] * back;
+          const int at = (wr * 32 + (lane & 31)) * (KP * 2 + 64) + (wc * 64 + j * 32 + 8 * q + 4 * (lane >> 5)) * 2;
+          put_split(xs + at, xs + YB + at, v);
+        }
+      __syncthreads();
+      gt.add([&](int plane, int i, int ks) { return frag_across<KP * 2>(xs + plane * YB, i, ks, lane); });
+    } else {
+      typedef typename Elem<E == STEP ? F32 : K>::T O;
+      O* dst = reinterpret_cast<O*>(p.dst) + g * p.dst_stride;
+      float* buf = reinterpret_cast<float*>(xs) + wave * (TALL ? 32 : 64) * OUT_LD;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[j][4 * q + e] * back;
+          // TALL: row l, columns j; otherwise row n of 64, columns l
+          const int row = (TALL ? 0 : j * 32) + (lane & 31), col = (TALL ? j * 32 : 0) + 8 * q + 4 * (lane >> 5);
+          *reinterpret_cast<f32x4*>(buf + row * OUT_LD + col) = v;
+        }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      constexpr int PERROW = TALL ? 16 : 8;
+#pragma unroll
+      for (int i = 0; i < (TALL ? 32 : 64); i += 64 / PERROW) {
+        const int row = i + lane / PERROW, col = (lane % PERROW) * 4;
+        f32x4 v = *reinterpret_cast<const f32x4*>(buf + row * OUT_LD + col);
+        const int r = TALL ? l0 + wr * 32 + row : wc * 64 + row, c = TALL ? wc * 64 + col : l0 + wr * 32 + col;
+        const int rend = TALL ? end : p.k, cend = TALL ? p.k : end;
+        if (r < rend && c < cend) {
+          O* at = dst + r * p.dst_ld + c;
+          if constexpr (E == STEP) {
+            const f32x4 old = load4<F32>(at, cend - c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = p.keep * old[e] - p.step * v[e];
+            store4<F32>(at, v, cend - c);
+          } else {
+            store4<K>(at, v, cend - c);
+          }
+        }
+      }
+    }
+  }
+  if constexpr (GRAM) gt.finish(xs, p.partial + ((int64_t)g * p.chunks + chunk) * (GramTiles<KP>::TILES * 1024));
+}
+
+// The steps of a phase on one workgroup.  Matrices live in registers (as the matrix instruction leaves them) and, as
+// planes, in the two places of LDS when they are operands.
+struct Chain {
+  const float* partial;
+  const int* exponent;  // first phase: A = sum / trace; NULL: A = sum / X_SCALE^2
+  int chunks, n;
+  double* inv;
+  float a, b, c;
+  float p_scale[3], q_scale[3];  // of step i
+  Planes before;                 // Q of the phase before (before.hi = NULL: none), in the square layout
+  float before_scale;
+  Planes q;                      // the product of all Q so far
+  float total_scale;
+};
+
+template <int KP> __global__ __launch_bounds__(KP * 4) void chain_kernel(const Chain p) {
+  constexpr int NT = KP * 4, F = KP == 128 ? 2 : 1, RB = KP * 2, MAT = KP * RB;
+  constexpr int TILES = GramTiles<KP>::TILES;
+  __shared__ __attribute__((aligned(16))) char lds[4 * MAT];
+  const int g = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  char *const s1 = lds, *const s2 = lds + 2 * MAT;
+  const int mb = (wave / 2) * 32, nb = (wave % 2) * 32 * F;
+  const int row = mb + (lane & 31), col0 = nb + 4 * (lane >> 5);
+  typedef f32x16 Mat[F];
+  auto put = [&](char* to, const Mat& v, float scale) {
+#pragma unroll
+    for (int j = 0; j < F; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = v[j][4 * q + e] * scale;
+        const int at = along<RB>(row, col0 + j * 32 + 8 * q);
+        put_split(to + at, to + MAT + at, x);
+      }
+  };
+  auto multiply = [&](Mat& v, const char* x, const char* y, float scale) {
+#pragma unroll
+    for (int j = 0; j < F; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[j][e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KP / 16; ++ks) {
+      const u32x4 a[2] = {frag_along<RB>(x, mb, ks, lane), frag_along<RB>(x + MAT, mb, ks, lane)};
+#pragma unroll
+      for (int j = 0; j < F; ++j) {
+        const u32x4 b[2] = {frag_along<RB>(y, nb + j * 32, ks, lane), frag_along<RB>(y + MAT, nb + j * 32, ks, lane)};
+        mfma3(v[j], a, b);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < F; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[j][e] *= scale;
+  };
+
+  // A: the partial sums of the tiles at and below the diagonal, mirrored through LDS
+  int top = -300;
+  if (p.exponent)
+    for (int c = 0; c < p.chunks; ++c) top = max(top, p.exponent[(int64_t)g * p.chunks + c]);
+  float* sum = reinterpret_cast<float*>(lds);  // [KP][KP + 4]
+  static_assert(KP * (KP + 4) * 4 <= 4 * MAT, "the Gram matrix fits");
+  for (int i = threadIdx.x * 4; i < TILES * 1024; i += NT * 4) {
+    const int tile = i >> 10, in = i & 1023, q = in >> 8, ln = (in & 255) >> 2;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < p.chunks; ++c) {
+      const int64_t slot = (int64_t)g * p.chunks + c;
+      f32x4 x = *reinterpret_cast<const f32x4*>(p.partial + slot * (TILES * 1024) + i);
+      if (p.exponent) {
+        const int d = 2 * (p.exponent[slot] - top);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = ldexpf(x[e], d);
+      }
+      v += x;
+    }
+    int ti, tj;
+    lower_tile(tile, ti, tj);
+    const int m = ti * 32 + (ln & 31), n = tj * 32 + 8 * q + 4 * (ln >> 5);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (ti != tj || n + e <= m) sum[m * (KP + 4) + n + e] = v[e];
+      if (ti != tj || n + e < m) sum[(n + e) * (KP + 4) + m] = v[e];
+    }
+  }
+  __syncthreads();
+  float unit = 1.f / (X_SCALE * X_SCALE);
+  if (p.exponent) {
+    double trace = 0.;
+    for (int i = 0; i < KP; ++i) trace += (double)sum[i * (KP + 4) + i];
+    double inv = 0.;
+    unit = 0.f;
+    if (!(trace < (double)INFINITY)) inv = unit = NAN;
+    else if (trace > 0.) {
+      unit = (float)(1. / trace);
+      inv = ldexp(1. / sqrt(trace), -top);
+    }
+    if (threadIdx.x == 0) p.inv[g] = inv;
+  }
+  Mat A, Q, T;
+#pragma unroll
+  for (int j = 0; j < F; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(sum + row * (KP + 4) + col0 + j * 32 + 8 * q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) A[j][4 * q + e] = x[e] * unit;
+    }
+  __syncthreads();
+  put(s1, A, A_SCALE);
+  __syncthreads();
+  float q_scale = 1.f;
+  for (int i = 0; i < p.n; ++i) {
+    Mat P;
+    const float ps = p.p_scale[i];
+    multiply(P, s1, s1, 1.f / (A_SCALE * A_SCALE));  // P = a I + b A + c A^2
+#pragma unroll
+    for (int j = 0; j < F; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int col = col0 + j * 32 + 8 * (e >> 2) + (e & 3);
+        P[j][e] = p.c * P[j][e] + (p.b * A[j][e] + (row == col ? p.a : 0.f));
+      }
+    put(s2, P, ps);
+    __syncthreads();
+    if (i + 1 < p.n) multiply(T, s2, s1, 1.f / (ps * A_SCALE));  // T = P A
+    if (i == 0) {
+#pragma unroll
+      for (int j = 0; j < F; ++j) Q[j] = P[j];
+    } else {  // Q = P Q
+      __syncthreads();
+      put(s1, Q, q_scale);
+      __syncthreads();
+      multiply(Q, s2, s1, 1.f / (ps * q_scale));
+    }
+    q_scale = p.q_scale[i];
+    if (i + 1 < p.n) {  // A = T P
+      __syncthreads();
+      put(s1, T, A_SCALE);
+      __syncthreads();
+      multiply(A, s1, s2, 1.f / (A_SCALE * ps));
+      __syncthreads();
+      put(s1, A, A_SCALE);
+      __syncthreads();
+    }
+  }
+  if (p.before.hi) {  // times the phase before
+    __syncthreads();
+    load_square<KP>(s1, p.before, g);
+    put(s2, Q, q_scale);
+    __syncthreads();
+    multiply(Q, s2, s1, 1.f / (q_scale * p.before_scale));
+  }
+  __syncthreads();
+  put(s1, Q, p.total_scale);
+  __syncthreads();
+  for (int i = threadIdx.x * 16; i < MAT; i += NT * 16) {
+    *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(p.q.hi + g * p.q.stride) + i) = *reinterpret_cast<const u32x4*>(s1 + i);
+    *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(p.q.lo + g * p.q.stride) + i) = *reinterpret_cast<const u32x4*>(s1 + MAT + i);
+  }
+}
+
 // ------------------------------------------------------------------------------------------ host
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align16(size_t v) { return (v + 15) & ~(size_t)15; }
@@ -534,6 +1017,7 @@ size_t small_bytes(int L, int k) {
 struct Space {
   int k, L, ld, phases, chunks;
   size_t small;
+  int narrow, rows_per;  // KP of the narrow form (0: not used), rows l of a chunk
   Choice gram;
   size_t sums, x, square, partial, total;  // bytes of one of each
   int n_x;
@@ -574,6 +1058,22 @@ bool space(const mplc_muon_t& t, Space& s) {
   s.small = small_bytes(s.L, s.k);
   if (s.small) {  // reading X again costs nothing here: phases of two steps lose less to the Gram matrix's error
     s.phases = (t.steps + 1) / 2;
+    return true;
+  }
+  if (s.k <= 128 && t.steps <= 6 && t.n_models <= 65535) {  // two phases of three steps at most
+    s.narrow = s.k <= 64 ? 64 : 128;
+    s.phases = (t.steps + 2) / 3;
+    const int64_t tr = 16384 / s.narrow, pieces = ceil_div(s.L, tr);
+    // about one workgroup per CU and round, whole pieces, at least two per workgroup where there are many
+    int64_t per = ceil_div(pieces * t.n_models, 512);
+    if (per > pieces) per = pieces;
+    s.rows_per = (int)((per < 1 ? 1 : per) * tr);
+    s.chunks = (int)ceil_div(s.L, s.rows_per);
+    const size_t G = (size_t)t.n_models, tiles = s.narrow == 128 ? 10 : 3;
+    s.sums = align16(G * s.chunks * sizeof(int)) + align16(G * sizeof(double));
+    s.partial = align16(G * s.chunks * tiles * 4096);
+    s.square = align16(G * s.narrow * s.narrow * 2) * 2;
+    s.total = s.sums + s.partial + 2 * s.square;
     return true;
   }
   s.n_x = s.phases > 1 ? 2 : 1;
@@ -663,8 +1163,81 @@ template <Kind K, Epi E> int run_small(const mplc_muon_t& t, const Space& sp, co
   }
 }
 
+template <Kind K, int KP, bool TALL, Epi E>
+int launch_narrow(const mplc_muon_t& t, const Space& sp, const Source& src, hipStream_t s) {
+  char* ws = reinterpret_cast<char*>(t.workspace);
+  Narrow p = {};
+  p.src = src;
+  p.L = sp.L;
+  p.k = sp.k;
+  p.chunks = sp.chunks;
+  p.rows_per = sp.rows_per;
+  p.exponent = reinterpret_cast<int*>(ws);
+  ws += align16((size_t)t.n_models * sp.chunks * sizeof(int));
+  p.inv = reinterpret_cast<double*>(ws);
+  ws += align16((size_t)t.n_models * sizeof(double));
+  p.partial = reinterpret_cast<float*>(ws);
+  ws += sp.partial;
+  Planes q[2];
+  for (int i = 0; i < 2; ++i) {
+    q[i] = Planes{reinterpret_cast<uint16_t*>(ws), reinterpret_cast<uint16_t*>(ws + sp.square / 2), KP * KP, KP};
+    ws += sp.square;
+  }
+  if (E == STEP) {
+    p.dst = t.w;
+    p.dst_stride = t.w_stride;
+    p.dst_ld = t.w_ld;
+    p.keep = (float)(1. - (double)t.lr * t.weight_decay);
+    p.step = t.lr * t.scale;
+  } else {
+    p.dst = t.out;
+    p.dst_stride = t.out_stride;
+    p.dst_ld = t.out_ld;
+  }
+  const dim3 grid((unsigned)sp.chunks, (unsigned)t.n_models);
+  hipError_t err;
+  double r = 1., total = 1.;
+  int done = 0;
+  for (int ph = 0; ph < sp.phases; ++ph) {
+    if (ph == 0) narrow_gram_kernel<K, KP, TALL><<<grid, NARROW_THREADS, 0, s>>>(p);
+    else narrow_apply_kernel<K, KP, TALL, true, E><<<grid, NARROW_THREADS, 0, s>>>(p);
+    if ((err = hipGetLastError()) != hipSuccess) return (int)err;
+    Chain c = {p.partial, ph == 0 ? p.exponent : nullptr, sp.chunks, (t.steps - done + (sp.phases - ph) - 1) / (sp.phases - ph),
+               p.inv, t.a, t.b, t.c, {}, {}, {}, 0.f, {}, 0.f};
+    double bound = 1.;
+    for (int i = 0; i < c.n; ++i) {
+      const double pb = factor_bound(t.a, t.b, t.c, r);
+      bound *= pb;
+      c.p_scale[i] = scale_for(pb);
+      c.q_scale[i] = scale_for(bound);
+      r = poly_bound(t.a, t.b, t.c, r);
+    }
+    total *= bound;
+    if (ph > 0) {
+      c.before = q[0];
+      c.before_scale = p.q_scale;
+    }
+    c.q = q[ph];
+    c.total_scale = scale_for(total);
+    chain_kernel<KP><<<dim3((unsigned)t.n_models), KP * 4, 0, s>>>(c);
+    if ((err = hipGetLastError()) != hipSuccess) return (int)err;
+    p.q = q[ph];
+    p.q_scale = c.total_scale;
+    done += c.n;
+  }
+  narrow_apply_kernel<K, KP, TALL, false, E><<<grid, NARROW_THREADS, 0, s>>>(p);
+  return (int)hipGetLastError();
+}
+
+template <Kind K, Epi E> int run_narrow(const mplc_muon_t& t, const Space& sp, const Source& src, hipStream_t s) {
+  const bool tall = t.rows >= t.cols;
+  if (sp.narrow == 64) return tall ? launch_narrow<K, 64, true, E>(t, sp, src, s) : launch_narrow<K, 64, false, E>(t, sp, src, s);
+  return tall ? launch_narrow<K, 128, true, E>(t, sp, src, s) : launch_narrow<K, 128, false, E>(t, sp, src, s);
+}
+
 template <Kind K, Epi LAST> int run(const mplc_muon_t& t, const Space& sp, const Source& src, hipStream_t s) {
   if (sp.small) return run_small<K, LAST>(t, sp, src, s);
+  if (sp.narrow) return run_narrow<K, LAST>(t, sp, src, s);
   char* ws = reinterpret_cast<char*>(t.workspace);
   double* sums = reinterpret_cast<double*>(ws);
   ws += sp.sums;

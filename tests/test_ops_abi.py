@@ -26,7 +26,7 @@ def dense_t(**kw):
 
 def muon_t(**kw):
     t = muon.MuonT()
-    t.n_models, t.rows, t.cols, t.steps = 2, 200, 70, 5
+    t.n_models, t.rows, t.cols, t.steps = 2, 400, 70, 5
     t.a, t.b, t.c = muon.COEFFICIENTS
     t.g = t.out = t.m = t.w = t.workspace = P
     t.g_ld = t.out_ld = t.m_ld = t.w_ld = 70
