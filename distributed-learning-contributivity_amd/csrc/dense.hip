@@ -160,8 +160,16 @@ template <Kind K> __global__ __launch_bounds__(256) void join_kernel(const Produ
   if (!p.count_is_r && p.segments == 1 && m >= count_of(p.counts, g, p.m)) return;
   const float* src = p.partial + (int64_t)g * p.m * p.n + (int64_t)m * p.n + n;
   const int64_t step = (int64_t)p.models * p.m * p.n;
-  f32x4 v = load4<F32>(src, p.n - n);
-  for (int s = 1; s < p.splits; ++s) v += load4<F32>(src + s * step, p.n - n);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < p.splits; s0 += 8) {  // 8 loads in flight
+    f32x4 x[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (s0 + s < p.splits) x[s] = load4<F32>(src + (s0 + s) * step, p.n - n);
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (s0 + s < p.splits) v += x[s];
+  }
   finish<K>(e, g, m, n, p.n, v);
 }
 

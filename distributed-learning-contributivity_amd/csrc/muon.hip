@@ -524,7 +524,8 @@ template <Kind K, int KT, Epi E> __global__ __launch_bounds__(256) void small_ke
 // KP: k padded to 64 or 128; a workgroup of 8 waves takes TR = 16384 / KP rows l of X at a time, the next ones on their
 // way in registers.  TALL: L = rows.  Before |U| is known, a workgroup scales by a power of two that it raises (with what
 // it has summed) when a larger value comes: split fp16 holds any range.
-constexpr int NARROW_THREADS = 512;
+constexpr int NARROW_THREADS = 512;  // with Q in LDS: one workgroup per CU
+constexpr int GRAM_THREADS = 256;    // without: several, whose conversions and products overlap
 
 struct Narrow {
   Source src;
@@ -577,15 +578,15 @@ __device__ __forceinline__ void mfma3(f32x16& d, const u32x4* a, const u32x4* b)
 }
 
 // TR rows l of U in registers, as 4-element pieces of U's rows
-template <Kind K, int KP, bool TALL> struct Piece {
-  static constexpr int TR = 16384 / KP, N = 16384 / 4 / NARROW_THREADS;
+template <Kind K, int KP, bool TALL, int NT> struct Piece {
+  static constexpr int TR = 32 * NT / KP, N = 8;
   static constexpr int RB = (TALL ? KP : TR) * 2;            // a stored row
   static constexpr int ACROSS = (TALL ? TR : KP) * (RB + 64);  // bytes of a plane
   static constexpr int ALONG = (TALL ? TR : KP) * RB;
   f32x4 u[N];
   static __device__ __forceinline__ void place(int j, int& row, int& col) {  // of the stored tile
     constexpr int PER = RB / 8;
-    const int c = threadIdx.x + j * NARROW_THREADS;
+    const int c = threadIdx.x + j * NT;
     row = c / PER;
     col = (c % PER) * 4;
   }
@@ -616,10 +617,10 @@ template <Kind K, int KP, bool TALL> struct Piece {
 };
 
 // Gram tiles of 32 x 32 at and below the diagonal, at most 3 per wave; KP = 64: every wave has all 3 and its own l,
-// KP = 128: two groups of 4 waves halve the l
-template <int KP> struct GramTiles {
-  static constexpr int TILES = KP == 128 ? 10 : 3, GROUPS = KP == 128 ? 2 : 8, STEP = KP == 128 ? 4 : 1;
-  static constexpr int KS = 16384 / KP / 16 / GROUPS;  // k-steps of a wave
+// KP = 128: groups of 4 waves share the tiles and have their own l
+template <int KP, int NT> struct GramTiles {
+  static constexpr int TILES = KP == 128 ? 10 : 3, GROUPS = KP == 128 ? NT / 256 : NT / 64, STEP = KP == 128 ? 4 : 1;
+  static constexpr int KS = 32 * NT / KP / 16 / GROUPS;  // k-steps of a wave
   f32x16 acc[3];
   int ti[3], tj[3], n, group;
   __device__ __forceinline__ void init() {
@@ -672,21 +673,22 @@ template <int KP> struct GramTiles {
             }
     }
     __syncthreads();
-    for (int i = threadIdx.x * 4; i < TILES * 1024; i += NARROW_THREADS * 4)
+    for (int i = threadIdx.x * 4; i < TILES * 1024; i += NT * 4)
       *reinterpret_cast<f32x4*>(out + i) = *reinterpret_cast<const f32x4*>(buf + i);
   }
 };
 
 // pass 1: the momentum; partial Gram matrices of U
-template <Kind K, int KP, bool TALL> __global__ __launch_bounds__(NARROW_THREADS) void narrow_gram_kernel(const Narrow p) {
-  typedef Piece<K, KP, TALL> Pc;
-  constexpr int BYTES = 2 * (TALL ? Pc::ACROSS : Pc::ALONG), SUM = GramTiles<KP>::TILES * 4096;
+template <Kind K, int KP, bool TALL> __global__ __launch_bounds__(GRAM_THREADS) void narrow_gram_kernel(const Narrow p) {
+  typedef Piece<K, KP, TALL, GRAM_THREADS> Pc;
+  typedef GramTiles<KP, GRAM_THREADS> Gt;
+  constexpr int BYTES = 2 * (TALL ? Pc::ACROSS : Pc::ALONG), SUM = Gt::TILES * 4096;
   __shared__ __attribute__((aligned(16))) char lds[BYTES > SUM ? BYTES : SUM];
-  __shared__ float most[8];
+  __shared__ float most[GRAM_THREADS / 64];
   const int g = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 63;
   const int begin = chunk * p.rows_per, end = min(p.L, begin + p.rows_per);
   Pc pc;
-  GramTiles<KP> gt;
+  Gt gt;
   gt.init();
   int exponent = -300;  // values are below 2^(exponent + 14); nothing seen yet
   pc.template load<true>(p.src, g, begin, end, p.k);
@@ -701,7 +703,7 @@ template <Kind K, int KP, bool TALL> __global__ __launch_bounds__(NARROW_THREADS
     if (lane == 0) most[threadIdx.x >> 6] = mx;
     __syncthreads();  // also: the last tile's planes are read
 #pragma unroll
-    for (int w = 0; w < 8; ++w) mx = fmaxf(mx, most[w]);
+    for (int w = 0; w < GRAM_THREADS / 64; ++w) mx = fmaxf(mx, most[w]);
     int e;
     frexpf(mx, &e);  // mx < 2^e
     e = mx > 0.f ? (mx < INFINITY ? e : 128) - 14 : -300;
@@ -723,8 +725,36 @@ template <Kind K, int KP, bool TALL> __global__ __launch_bounds__(NARROW_THREADS
     });
   }
   const int64_t slot = (int64_t)g * p.chunks + chunk;
-  gt.finish(lds, p.partial + slot * (GramTiles<KP>::TILES * 1024));
+  gt.finish(lds, p.partial + slot * (Gt::TILES * 1024));
   if (threadIdx.x == 0) p.exponent[slot] = exponent;
+}
+
+// the chunks' partial sums, added in order at the largest exponent, into the first chunk's place
+__global__ __launch_bounds__(256) void narrow_join_kernel(float* partial, const int* exponent, int chunks, int n) {
+  const int g = blockIdx.y, i = (blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  float* at = partial + (int64_t)g * chunks * n + i;
+  int top = -300;
+  if (exponent)
+    for (int c = 0; c < chunks; ++c) top = max(top, exponent[(int64_t)g * chunks + c]);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int c0 = 0; c0 < chunks; c0 += 8) {
+    f32x4 x[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c0 + c < chunks) x[c] = *reinterpret_cast<const f32x4*>(at + (int64_t)(c0 + c) * n);
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c0 + c < chunks) {
+        if (exponent) {
+          const int d = 2 * (exponent[(int64_t)g * chunks + c0 + c] - top);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[c][e] = ldexpf(x[c][e], d);
+        }
+        v += x[c];
+      }
+  }
+  *reinterpret_cast<f32x4*>(at) = v;
 }
 
 // Q (planes in the square layout) to LDS
@@ -739,11 +769,12 @@ template <int KP> __device__ __forceinline__ void load_square(char* lds, const P
 // passes 2 and 3: Y = U Q / |U| by TR rows.  GRAM: partial Gram matrices of Y; otherwise Y is the result.
 template <Kind K, int KP, bool TALL, bool GRAM, Epi E>
 __global__ __launch_bounds__(NARROW_THREADS) void narrow_apply_kernel(const Narrow p) {
-  typedef Piece<K, KP, TALL> Pc;
+  typedef Piece<K, KP, TALL, NARROW_THREADS> Pc;
+  typedef GramTiles<KP, NARROW_THREADS> Gt;
   constexpr int TR = Pc::TR, QB = KP * KP * 2, YB = TR * (KP * 2 + 64);
   constexpr int XB = TALL ? Pc::ALONG : Pc::ACROSS;  // a plane of U
   constexpr int OUT_LD = TALL ? 68 : 36, OUT = 8 * (TALL ? 32 : 64) * OUT_LD * 4;
-  constexpr int A = 2 * XB, B = GRAM ? 2 * YB : OUT, SUM = GRAM ? GramTiles<KP>::TILES * 4096 : 0;
+  constexpr int A = 2 * XB, B = GRAM ? 2 * YB : OUT, SUM = GRAM ? Gt::TILES * 4096 : 0;
   constexpr int REST = A > B ? A : B;
   __shared__ __attribute__((aligned(16))) char lds[2 * QB + (REST > SUM ? REST : SUM)];
   char* const xs = lds + 2 * QB;
@@ -753,7 +784,7 @@ __global__ __launch_bounds__(NARROW_THREADS) void narrow_apply_kernel(const Narr
   const double inv = p.inv[g] * (double)X_SCALE;
   const float back = GRAM ? 1.f / p.q_scale : 1.f / (X_SCALE * p.q_scale);
   Pc pc;
-  GramTiles<KP> gt;
+  Gt gt;
   if constexpr (GRAM) gt.init();
   pc.template load<false>(p.src, g, begin, end, p.k);
   load_square<KP>(lds, p.q, g);
@@ -835,13 +866,13 @@ __global__ __launch_bounds__(NARROW_THREADS) void narrow_apply_kernel(const Narr
       }
     }
   }
-  if constexpr (GRAM) gt.finish(xs, p.partial + ((int64_t)g * p.chunks + chunk) * (GramTiles<KP>::TILES * 1024));
+  if constexpr (GRAM) gt.finish(xs, p.partial + ((int64_t)g * p.chunks + chunk) * (Gt::TILES * 1024));
 }
 
 // The steps of a phase on one workgroup.  Matrices live in registers (as the matrix instruction leaves them) and, as
 // planes, in the two places of LDS when they are operands.
 struct Chain {
-  const float* partial;
+  const float* partial;  // [model][chunk], joined into the first chunk's
   const int* exponent;  // first phase: A = sum / trace; NULL: A = sum / X_SCALE^2
   int chunks, n;
   double* inv;
@@ -855,7 +886,7 @@ struct Chain {
 
 template <int KP> __global__ __launch_bounds__(KP * 4) void chain_kernel(const Chain p) {
   constexpr int NT = KP * 4, F = KP == 128 ? 2 : 1, RB = KP * 2, MAT = KP * RB;
-  constexpr int TILES = GramTiles<KP>::TILES;
+  constexpr int TILES = GramTiles<KP, 256>::TILES;
   __shared__ __attribute__((aligned(16))) char lds[4 * MAT];
   const int g = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   char *const s1 = lds, *const s2 = lds + 2 * MAT;
@@ -894,7 +925,7 @@ template <int KP> __global__ __launch_bounds__(KP * 4) void chain_kernel(const C
       for (int e = 0; e < 16; ++e) v[j][e] *= scale;
   };
 
-  // A: the partial sums of the tiles at and below the diagonal, mirrored through LDS
+  // A: the tiles at and below the diagonal, mirrored through LDS
   int top = -300;
   if (p.exponent)
     for (int c = 0; c < p.chunks; ++c) top = max(top, p.exponent[(int64_t)g * p.chunks + c]);
@@ -902,17 +933,7 @@ template <int KP> __global__ __launch_bounds__(KP * 4) void chain_kernel(const C
   static_assert(KP * (KP + 4) * 4 <= 4 * MAT, "the Gram matrix fits");
   for (int i = threadIdx.x * 4; i < TILES * 1024; i += NT * 4) {
     const int tile = i >> 10, in = i & 1023, q = in >> 8, ln = (in & 255) >> 2;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; c < p.chunks; ++c) {
-      const int64_t slot = (int64_t)g * p.chunks + c;
-      f32x4 x = *reinterpret_cast<const f32x4*>(p.partial + slot * (TILES * 1024) + i);
-      if (p.exponent) {
-        const int d = 2 * (p.exponent[slot] - top);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = ldexpf(x[e], d);
-      }
-      v += x;
-    }
+    const f32x4 v = *reinterpret_cast<const f32x4*>(p.partial + (int64_t)g * p.chunks * (TILES * 1024) + i);
     int ti, tj;
     lower_tile(tile, ti, tj);
     const int m = ti * 32 + (ln & 31), n = tj * 32 + 8 * q + 4 * (ln >> 5);
@@ -1199,9 +1220,15 @@ int launch_narrow(const mplc_muon_t& t, const Space& sp, const Source& src, hipS
   double r = 1., total = 1.;
   int done = 0;
   for (int ph = 0; ph < sp.phases; ++ph) {
-    if (ph == 0) narrow_gram_kernel<K, KP, TALL><<<grid, NARROW_THREADS, 0, s>>>(p);
+    if (ph == 0) narrow_gram_kernel<K, KP, TALL><<<grid, GRAM_THREADS, 0, s>>>(p);
     else narrow_apply_kernel<K, KP, TALL, true, E><<<grid, NARROW_THREADS, 0, s>>>(p);
     if ((err = hipGetLastError()) != hipSuccess) return (int)err;
+    if (sp.chunks > 1) {
+      constexpr int n = GramTiles<KP, 256>::TILES * 1024;
+      narrow_join_kernel<<<dim3(n / 1024, (unsigned)t.n_models), 256, 0, s>>>(p.partial, ph == 0 ? p.exponent : nullptr,
+                                                                              sp.chunks, n);
+      if ((err = hipGetLastError()) != hipSuccess) return (int)err;
+    }
     Chain c = {p.partial, ph == 0 ? p.exponent : nullptr, sp.chunks, (t.steps - done + (sp.phases - ph) - 1) / (sp.phases - ph),
                p.inv, t.a, t.b, t.c, {}, {}, {}, 0.f, {}, 0.f};
     double bound = 1.;
