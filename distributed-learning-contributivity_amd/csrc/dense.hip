@@ -43,7 +43,8 @@ struct Product {
   int models, segments;  // segments > 1: one product, r runs over (model, r)
   const int32_t* counts;
   int count_is_r;        // counts limit r (dw), not m
-  int tiles_m, tiles_n, nk, splits, per_split;
+  int tiles_m, tiles_n, nk, splits, per_split;  // nk: units of r; per_split: units of a split
+  int aligned;           // 16-byte rows: tiles go straight into LDS
   float* partial;        // [split][model][m][n] where splits > 1
 };
 
@@ -100,10 +101,12 @@ __device__ __forceinline__ void tile_of(int idx, int tm, int tn, int& m, int& n)
   n = in / size;
 }
 
-template <Kind K, bool AA, bool BA, int WM, int WN, int FM, int FN>
+constexpr int unit_of(Kind k) { return k == F32 ? 32 : 64; }  // what a split takes whole numbers of
+
+template <Kind K, bool AA, bool BA, int WM, int WN, int FM, int FN, int BKB, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, const Epilogue e) {
   typedef typename Elem<K>::T T;
-  typedef Block<K, AA, BA, WM, WN, FM, FN, 128, 1> B;
+  typedef Block<K, AA, BA, WM, WN, FM, FN, BKB, 1, STAGES> B;
   __shared__ __attribute__((aligned(16))) char lds[B::LDS_BYTES];
   int64_t b = xcd_block();
   const int tiles = p.tiles_m * p.tiles_n;
@@ -116,15 +119,20 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
   const int cnt = seg ? p.m : count_of(p.counts, g, p.count_is_r ? p.r : p.m);
   const int M = p.count_is_r ? p.m : cnt, R = p.count_is_r ? cnt : p.r;
   if (m0 >= M) return;
-  const int nk = (R + B::BK - 1) / B::BK;
-  const int64_t all = (int64_t)nk * p.segments, first = (int64_t)split * p.per_split;
-  const int64_t last = first + p.per_split < all ? first + p.per_split : all;
+  const int64_t first = (int64_t)split * p.per_split, last = first + p.per_split;  // units of r
   const T* pa = reinterpret_cast<const T*>(p.a) + g * p.a_stride;
   const T* pb = reinterpret_cast<const T*>(p.b) + g * p.b_stride;
   B blk;
   blk.clear();
   if (seg) {
-    blk.run(lds, m0, n0, nk, first, last, [&](int s, Operand<T>& a, Operand<T>& o, int& r0, int& rend) {
+    // unit u of (model, r) as a tile of (model, r)
+    const int nk = (R + B::BK - 1) / B::BK;
+    auto tile_at = [&](int64_t u) {
+      const int64_t s = u / p.nk;
+      return s >= p.segments ? (int64_t)p.segments * nk : s * nk + min(nk, (int)(u - s * p.nk) * (unit_of(K) / B::BK));
+    };
+    const int64_t from = tile_at(first), to = tile_at(last);
+    auto at = [&](int s, Operand<T>& a, Operand<T>& o, int& r0) {
       a.p[0] = pa + s * p.a_stride;
       o.p[0] = pb + s * p.b_stride;
       a.ld = p.a_ld;
@@ -132,12 +140,19 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
       a.rows = p.m;
       o.rows = p.n;
       r0 = 0;
-      rend = R;
-      return count_of(p.counts, s, p.m);
-    });
+    };
+    if (p.aligned && p.counts == nullptr && R % B::BK == 0) {
+      if (from < to) blk.ring(lds, m0, n0, nk, from, to, at);
+    } else {
+      blk.through_registers(lds, m0, n0, nk, from, to, [&](int s, Operand<T>& a, Operand<T>& o, int& r0, int& rend) {
+        at(s, a, o, r0);
+        rend = R;
+        return count_of(p.counts, s, p.m);
+      });
+    }
   } else {
     const Operand<T> a = {{pa, nullptr}, p.a_ld, M}, o = {{pb, nullptr}, p.b_ld, p.n};
-    blk.run(lds, a, o, m0, n0, (int)first * B::BK, (int)min((int64_t)R, last * B::BK));
+    blk.run(lds, a, o, m0, n0, (int)min((int64_t)R, first * unit_of(K)), (int)min((int64_t)R, last * unit_of(K)), p.aligned);
   }
   if (p.splits > 1) {
     float* out = p.partial + ((int64_t)split * p.models + g) * p.m * p.n;
@@ -256,7 +271,7 @@ bool plan(const mplc_dense_t& t, Form form, Plan& out) {
   p.counts = t.counts;
   p.count_is_r = form == DW;
   const bool f32 = t.dtype == MPLC_DTYPE_F32;
-  p.nk = (int)ceil_div(p.r, f32 ? 32 : 64);
+  p.nk = (int)ceil_div(p.r, f32 ? unit_of(F32) : unit_of(BF16));
   const int64_t units = (int64_t)p.nk * p.segments;
   if (units > INT32_MAX) return false;
   const Choice c = choose(f32 ? SHAPES_F32 : SHAPES_16, 5, p.models, p.m, p.n, (int64_t)p.r * p.segments, units, true);
@@ -273,15 +288,21 @@ bool plan(const mplc_dense_t& t, Form form, Plan& out) {
   return true;
 }
 
-template <Kind K, bool AA, bool BA> hipError_t launch(const Plan& pl, const Epilogue& e, hipStream_t s) {
+template <Kind K, bool AA, bool BA> hipError_t launch(Plan& pl, const Epilogue& e, hipStream_t s) {
+  const int ch = K == F32 ? 4 : 8;
+  auto fits = [&](const void* base, int64_t stride, int64_t ld) {
+    return ((uintptr_t)base & 15) == 0 && stride % ch == 0 && ld % ch == 0;
+  };
+  pl.p.aligned = fits(pl.p.a, pl.p.a_stride, pl.p.a_ld) && fits(pl.p.b, pl.p.b_stride, pl.p.b_ld) &&
+                 (!AA || pl.p.m % ch == 0) && (!BA || pl.p.n % ch == 0);
   const dim3 grid((unsigned)pl.blocks);
-  if (pl.cfg == 0) product_kernel<K, AA, BA, 2, 2, 2, 2><<<grid, 256, 0, s>>>(pl.p, e);
-  else if (pl.cfg == 1) product_kernel<K, AA, BA, 2, 2, 1, 1><<<grid, 256, 0, s>>>(pl.p, e);
-  else if (pl.cfg == 4) product_kernel<K, AA, BA, 1, 4, 2, 1><<<grid, 256, 0, s>>>(pl.p, e);
+  if (pl.cfg == 0) product_kernel<K, AA, BA, 2, 2, 2, 2, 128, 2><<<grid, 256, 0, s>>>(pl.p, e);
+  else if (pl.cfg == 1) product_kernel<K, AA, BA, 2, 2, 1, 1, 128, 3><<<grid, 256, 0, s>>>(pl.p, e);
+  else if (pl.cfg == 4) product_kernel<K, AA, BA, 1, 4, 2, 1, 128, 3><<<grid, 256, 0, s>>>(pl.p, e);
   else if (pl.cfg == 3) {
-    if constexpr (K != F32) product_kernel<K, AA, BA, 2, 4, 4, 2><<<grid, 512, 0, s>>>(pl.p, e);
+    if constexpr (K != F32) product_kernel<K, AA, BA, 2, 4, 4, 2, 128, 2><<<grid, 512, 0, s>>>(pl.p, e);
   }
-  else product_kernel<K, AA, BA, 1, 4, 1, 1><<<grid, 256, 0, s>>>(pl.p, e);
+  else product_kernel<K, AA, BA, 1, 4, 1, 1, 128, 3><<<grid, 256, 0, s>>>(pl.p, e);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || pl.p.splits == 1) return err;
   const dim3 jg((unsigned)ceil_div((int64_t)pl.p.m * ((pl.p.n + 3) / 4), 256), (unsigned)pl.p.models);

@@ -9,12 +9,14 @@
 // takes three matrix instructions (hi hi, hi lo, lo hi; lo lo is below 2^-24 of the product).  Values must be scaled
 // into fp16's range by the caller.  It reaches fp32's accuracy at a third of the fp16 rate, about twice the fp32 rate.
 //
-// One workgroup computes a BM x BN tile.  Tiles of both operands go through registers into LDS, two buffers deep: the
-// loads of the next tile are in flight while the matrix cores work on this one, one barrier per tile.  A tile row "along
-// r" is BKB bytes and its 16-byte chunks are exchanged (XOR with the row) so that the 16 rows that one pass of
-// ds_read_b128 touches fall on different banks.  A tile "across r" keeps its rows as they are, with a pad that puts
-// the rows that one pass touches on different banks; 16-bit fragments are gathered with ds_read_b64_tr_b16, which
-// transposes 4 x 16 elements inside 16 lanes, fp32 fragments with four ds_read_b32.
+// One workgroup computes a BM x BN tile over tiles of r, BKB bytes of an operand "along r" long.  Where the operands'
+// rows are 16-byte aligned their tiles go from memory into LDS directly (global_load_lds, no registers), in a ring of
+// STAGES tiles, whose loads run ahead by STAGES - 1 tiles; one barrier per tile.  Other operands, and the last tile of an r that no tile divides, go through registers.
+//
+// LDS.  A tile is a sequence of 16-byte chunks, row by row; which chunk of a row is at which place is exchanged by row
+// (XOR), so that the rows that one pass of a read touches fall on different banks: along r, the 16 rows of a
+// ds_read_b128; across r, the 4 rows of a ds_read_b64_tr_b16 (which transposes 4 x 16 elements inside 16 lanes) or the
+// two of an fp32 fragment's ds_read_b32.
 //
 // The matrix instruction is issued as B A^T, so that a lane ends up with 4 consecutive columns n of one row m (wide
 // stores and wide reads of the residual) instead of 4 rows of one column.
@@ -158,21 +160,26 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
   static constexpr int CH = 16 / sizeof(T);              // elements of a chunk
   static constexpr int BK = BKB / sizeof(T);             // r per tile
   static constexpr int RPC = ACROSS ? BT / CH : BK / CH; // chunks of a stored row
+  static constexpr int ROWB = RPC * 16;
   static constexpr int CHUNKS = BT * BK / CH;
-  static constexpr int PER = (CHUNKS + NT - 1) / NT;
-  static constexpr int PAD = K == F32 ? 32 : 64;
-  static constexpr int ROWB = ACROSS ? BT * (int)sizeof(T) + PAD : BKB;
-  static constexpr int PLANE_BYTES = ACROSS ? BK * ROWB : BT * BKB;
+  static constexpr int PER = CHUNKS / NT;
+  static constexpr int PLANE_BYTES = CHUNKS * 16;
   static constexpr int BYTES = PL * PLANE_BYTES;
   static_assert(CHUNKS % NT == 0, "whole chunks per thread");
 
-  u32x4 reg[PL][PER];
   const T* ptr[PL][PER];
   int live[PER];  // ACROSS: valid elements of the chunk's columns
 
+  // place of chunk ch of a row, and the chunk at a place
   __device__ __forceinline__ static int swz(int row, int ch) {
-    if constexpr (BKB == 128) return ch ^ ((row >> 1) & 7);
-    else return ch ^ ((row >> 2) & 3);
+    if constexpr (!ACROSS) return BKB == 128 ? ch ^ ((row >> 1) & 7) : ch ^ ((row >> 2) & 3);
+    else if constexpr (K == F32) return RPC >= 16 ? ch ^ (((row >> 2) & 1) << 3) : ch;
+    else return RPC >= 16 ? ch ^ ((row & 3) << 2) : RPC == 8 ? ch ^ (((row >> 1) & 1) << 2) : ch;
+  }
+  __device__ __forceinline__ static void place(int j, int tid, int& row, int& ch) {
+    const int c = tid + j * NT;
+    row = c / RPC;
+    ch = swz(row, c % RPC);
   }
 
   // Points at the tile of rows [i0, i0 + BT) and r = r0 ...  Rows behind o.rows (never stored) repeat the last one, so
@@ -180,8 +187,8 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
   __device__ __forceinline__ void seek(const Operand<T>& o, int i0, int r0, int tid) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const int c = tid + j * NT;
-      const int row = c / RPC, ch = c % RPC;
+      int row, ch;
+      place(j, tid, row, ch);
       int64_t off;
       if constexpr (ACROSS) {
         const int i = i0 + ch * CH;
@@ -200,42 +207,53 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
 #pragma unroll
       for (int j = 0; j < PER; ++j) ptr[p][j] += ACROSS ? BK * ld : BK;
   }
-  // the tile at ptr, of which `left` r are valid (left >= BK: all); `whole`: no chunk of columns is cut (uniform)
-  __device__ __forceinline__ void load(int left, bool whole, int tid) {
+  // the whole tile at ptr into LDS; counts as PL * PER loads of the wave
+  __device__ __forceinline__ void fetch(char* lds, int tid) const {
+    typedef __attribute__((address_space(3))) uint32_t lds_u32;
+    typedef __attribute__((address_space(1))) const uint32_t glb_u32;
+#pragma unroll
+    for (int p = 0; p < PL; ++p)
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        __builtin_amdgcn_global_load_lds((glb_u32*)ptr[p][j], (lds_u32*)(lds + p * PLANE_BYTES + (j * NT + (tid & ~63)) * 16), 16, 0, 0);
+  }
+  // the tile at ptr, of which `left` r are valid (left >= BK: all); `whole`: no chunk of columns is cut (uniform); rows
+  // at or behind `rows` contribute nothing
+  struct Regs {
+    u32x4 v[PL][PER];
+  };
+  __device__ __forceinline__ void load(Regs& reg, int left, bool whole, int i0, int rows, bool drop, int tid) const {
     if (left >= BK && (!ACROSS || whole)) {
 #pragma unroll
       for (int p = 0; p < PL; ++p)
 #pragma unroll
-        for (int j = 0; j < PER; ++j) reg[p][j] = load16(ptr[p][j]);
-      return;
-    }
+        for (int j = 0; j < PER; ++j) reg.v[p][j] = load16(ptr[p][j]);
+    } else {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int c = tid + j * NT;
-      const int row = c / RPC, ch = c % RPC;
-      const int n = ACROSS ? (row < left ? (live[j] > 0 ? live[j] : (whole ? CH : 0)) : 0) : left - ch * CH;
+      for (int j = 0; j < PER; ++j) {
+        int row, ch;
+        place(j, tid, row, ch);
+        const int n = ACROSS ? (row < left ? (live[j] > 0 ? live[j] : (whole ? CH : 0)) : 0) : left - ch * CH;
 #pragma unroll
-      for (int p = 0; p < PL; ++p) reg[p][j] = load16_edge<K>(ptr[p][j], n);
+        for (int p = 0; p < PL; ++p) reg.v[p][j] = load16_edge<K>(ptr[p][j], n);
+      }
     }
-  }
-  // rows at or behind `rows` are not part of this sum
-  __device__ __forceinline__ void drop_rows(int i0, int rows, int tid) {
     if constexpr (!ACROSS)
+      if (drop)
 #pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (i0 + (tid + j * NT) / RPC >= rows)
+        for (int j = 0; j < PER; ++j) {
+          int row, ch;
+          place(j, tid, row, ch);
+          if (i0 + row >= rows)
 #pragma unroll
-          for (int p = 0; p < PL; ++p) reg[p][j] = u32x4{0, 0, 0, 0};
+            for (int p = 0; p < PL; ++p) reg.v[p][j] = u32x4{0, 0, 0, 0};
+        }
   }
-  __device__ __forceinline__ void store(char* lds, int tid) const {
+  __device__ __forceinline__ static void store(const Regs& reg, char* lds, int tid) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int c = tid + j * NT;
-      const int row = c / RPC, ch = c % RPC;
-      const int at = ACROSS ? row * ROWB + ch * 16 : row * ROWB + swz(row, ch) * 16;
+    for (int j = 0; j < PER; ++j)
 #pragma unroll
-      for (int p = 0; p < PL; ++p) *reinterpret_cast<u32x4*>(lds + p * PLANE_BYTES + at) = reg[p][j];
-    }
+      for (int p = 0; p < PL; ++p) *reinterpret_cast<u32x4*>(lds + p * PLANE_BYTES + (tid + j * NT) * 16) = reg.v[p][j];
   }
   // the fragment of rows [i, i + 32) for k-step ks (2 chunks of r)
   __device__ __forceinline__ static u32x4 frag(const char* lds, int plane, int i, int ks, int lane) {
@@ -244,8 +262,8 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
       const int row = i + (lane & 31);
       return *reinterpret_cast<const u32x4*>(base + row * ROWB + swz(row, 2 * ks + (lane >> 5)) * 16);
     } else if constexpr (K == F32) {
-      const int r = (2 * ks + (lane >> 5)) * 4;
-      const float* f = reinterpret_cast<const float*>(base + r * ROWB + (i + (lane & 31)) * 4);
+      const int r = (2 * ks + (lane >> 5)) * 4, col = i + (lane & 31);
+      const float* f = reinterpret_cast<const float*>(base + r * ROWB + swz(r, col >> 2) * 16) + (col & 3);
       u32x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(f[e * (ROWB / 4)]);
@@ -254,8 +272,8 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
       // 16 lanes fetch 4 rows of 16 elements (lane q of them: row q / 4, elements 4 (q % 4) ..) and lane q receives
       // element q of the 4 rows; twice, for 8 r
       const int q = lane & 15;
-      const int r = (2 * ks + (lane >> 5)) * 8 + (q >> 2);
-      const char* a = base + r * ROWB + (i + (lane & 16) + 4 * (q & 3)) * 2;
+      const int r = (2 * ks + (lane >> 5)) * 8 + (q >> 2), col = i + (lane & 16) + 4 * (q & 3);
+      const char* a = base + r * ROWB + swz(r, col >> 3) * 16 + (col & 7) * 2;
       typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
       const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a));
       const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 4 * ROWB));
@@ -267,8 +285,26 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
   }
 };
 
+// Waits for the wave's own LDS accesses.
+__device__ __forceinline__ void wait_lds() {
+  __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+// Waits until at most N of the wave's loads are on their way, and keeps later LDS accesses behind that.
+template <int N> __device__ __forceinline__ void wait_loads() {
+  static_assert(N < 64, "six bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+  asm volatile("" ::: "memory");
+}
+
 // A workgroup of WM x WN waves, each FM x FN fragments of 32 x 32.
-template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int FN_, int BKB, int PL> struct Block {
+template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int FN_, int BKB, int PL, int STAGES>
+struct Block {
   typedef typename Elem<K>::T T;
   static constexpr int WM = WM_, WN = WN_, FM = FM_, FN = FN_;
   static constexpr int NT = 64 * WM * WN;
@@ -277,7 +313,8 @@ template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int F
   typedef Tile<K, B_ACROSS, BN, BKB, NT, PL> TB;
   static constexpr int BK = TA::BK;
   static constexpr int STAGE = TA::BYTES + TB::BYTES;
-  static constexpr int LDS_BYTES = 2 * STAGE;
+  static constexpr int LDS_BYTES = STAGES * STAGE;
+  static_assert(STAGES >= 2, "one tile in use, one on its way");
 
   f32x16 acc[FM][FN];
 
@@ -312,26 +349,38 @@ template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int F
     for (int e = 0; e < (K == F32 ? 4 : 1); ++e)
       each_pair([&](int i, int j) { mfma<K>(acc[i][j], f.b[0][j], f.a[0][i], e); });
   }
-  // One tile: the fragments of step ks + 1 are on their way while the matrix cores work on step ks.  Left to itself the
-  // compiler reads each fragment right before its use and waits (fp32 128 x 128: 72 % of the cycles busy).
-  __device__ __forceinline__ void compute(const char* la, const char* lb, int lane, int wm, int wn) {
-    constexpr int KS = BKB / 32;
-    if constexpr (PL * (FM + FN) > 8) {  // no registers for two sets: many instructions per fragment hide the reads
+  // One tile's products.  The fragments of step ks + 1 are on their way while the matrix cores work on step ks, across
+  // the tile's end too: turn() - called once every read of this tile has arrived - makes the next tile's LDS ready and
+  // returns it (nullptr: no more), so neither its barrier nor its first reads leave the matrix cores idle.  (Reads at
+  // the start of each tile, after the barrier: 40 % of the cycles busy at 256 x 256.)
+  static constexpr int KS = BKB / 32;
+  static constexpr bool PIPE = PL * (FM + FN) <= 8;  // registers for two sets of fragments
+  static_assert(KS % 2 == 0, "the sets alternate");
+  Frags f[PIPE ? 2 : 1];
+  __device__ __forceinline__ void first(const char* cur, int lane, int wm, int wn) {
+    if constexpr (PIPE) read(f[0], cur, cur + TA::BYTES, 0, lane, wm, wn);
+  }
+  template <typename Turn> __device__ __forceinline__ void compute(const char* cur, int lane, int wm, int wn, Turn turn) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        Frags f;
-        read(f, la, lb, ks, lane, wm, wn);
-        multiply(f);
-      }
-    } else {
-      Frags f[2];
-      read(f[0], la, lb, 0, lane, wm, wn);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        if (ks + 1 < KS) read(f[(ks + 1) & 1], la, lb, ks + 1, lane, wm, wn);
+    for (int ks = 0; ks < KS; ++ks) {
+      if constexpr (PIPE) {
+        if (ks + 1 < KS) {
+          read(f[(ks + 1) & 1], cur, cur + TA::BYTES, ks + 1, lane, wm, wn);
+        } else {
+          wait_lds();
+          const char* next = turn();
+          if (next) read(f[0], next, next + TA::BYTES, 0, lane, wm, wn);
+        }
         __builtin_amdgcn_sched_barrier(0);
         multiply(f[ks & 1]);
         __builtin_amdgcn_sched_barrier(0);
+      } else {
+        read(f[0], cur, cur + TA::BYTES, ks, lane, wm, wn);
+        if (ks + 1 == KS) {
+          wait_lds();
+          turn();
+        }
+        multiply(f[0]);
       }
     }
   }
@@ -343,11 +392,24 @@ template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int F
       for (int j = 0; j < FN; ++j) f(i, j);
   }
 
-  // acc += the sum over r of the whole product; A.rows, B.rows > 0
+  // acc += the sum over [r0, rend); A.rows, B.rows > 0.  aligned: bases and lds are multiples of 16 bytes, and the
+  // columns of an operand across r whole chunks.
   __device__ __forceinline__ void run(char* lds, const Operand<T>& A, const Operand<T>& B, int m0, int n0, int r0,
-                                      int rend) {
+                                      int rend, bool aligned) {
+    const int tid = threadIdx.x;
+    if (r0 >= rend) return;
+    if (aligned) {
+      const int n = (rend - r0) / BK;
+      if (n > 0) ring(lds, m0, n0, n, 0, n, [&](int, Operand<T>& a, Operand<T>& b, int& first) {
+          a = A;
+          b = B;
+          first = r0;
+        });
+      r0 += n * BK;
+      if (r0 >= rend) return;
+    }
     const int n = (rend - r0 + BK - 1) / BK;
-    run(lds, m0, n0, n, 0, n, [&](int, Operand<T>& a, Operand<T>& b, int& first, int& end) {
+    through_registers(lds, m0, n0, n, 0, n, [&](int, Operand<T>& a, Operand<T>& b, int& first, int& end) {
       a = A;
       b = B;
       first = r0;
@@ -356,16 +418,72 @@ template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int F
     });
   }
 
-  // acc += the sum over tiles [from, to) of pieces of n tiles each: at(s, A, B, r0, rend) says where piece s is and
-  // returns how many rows of A take part in it (the others contribute nothing)
+  // acc += the sum over tiles [from, to) of pieces of n whole tiles each: at(s, A, B, r0) says where piece s is
   template <typename At>
-  __device__ __forceinline__ void run(char* lds, int m0, int n0, int n, int64_t from, int64_t to, At at) {
+  __device__ __forceinline__ void ring(char* lds, int m0, int n0, int n, int64_t from, int64_t to, At at) {
+    constexpr int LOADS = PL * (TA::PER + TB::PER);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave / WN, wn = wave % WN;
+    const int all = (int)(to - from);
+    TA ta;
+    TB tb;
+    Operand<T> A, B;
+    int r0, s = (int)(from / n), t = (int)(from - (int64_t)s * n), issued = 0;
+    auto seek = [&]() {
+      at(s, A, B, r0);
+      ta.seek(A, m0, r0 + t * BK, tid);
+      tb.seek(B, n0, r0 + t * BK, tid);
+    };
+    auto fetch = [&](char* to) {
+      ta.fetch(to, tid);
+      tb.fetch(to + TA::BYTES, tid);
+      ++issued;
+      if (++t == n) {
+        t = 0;
+        ++s;
+        if (issued < all) seek();
+      } else {
+        ta.advance(A.ld);
+        tb.advance(B.ld);
+      }
+    };
+    seek();
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i)
+      if (i < all) fetch(lds + i * STAGE);
+    if (issued == STAGES) wait_loads<(STAGES - 1) * LOADS>();  // the first tile's
+    else wait_loads<0>();
+    barrier();
+    first(lds, lane, wm, wn);
+    int stage = 0;
+    for (int it = 0; it < all; ++it) {
+      char* cur = lds + stage * STAGE;
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      char* nxt = lds + stage * STAGE;
+      compute(cur, lane, wm, wn, [&]() -> const char* {
+        if (it + 1 == all) return nullptr;
+        if (issued - it == STAGES) wait_loads<(STAGES - 2) * LOADS>();  // the next tile's, not the ones behind it
+        else wait_loads<0>();
+        barrier();  // everyone's part of the next tile is there, and everyone has read this one
+        if (issued < all) fetch(cur);
+        return nxt;
+      });
+    }
+    __syncthreads();
+  }
+
+  // The same through registers, pieces of n tiles of which the last may be cut: at(s, A, B, r0, rend) returns how many
+  // rows of A take part in piece s (the others contribute nothing).
+  template <typename At>
+  __device__ __forceinline__ void through_registers(char* lds, int m0, int n0, int n, int64_t from, int64_t to, At at) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave / WN, wn = wave % WN;
     if (n <= 0 || to <= from) return;
     const int all = (int)(to - from);
     TA ta;
     TB tb;
+    typename TA::Regs ra;
+    typename TB::Regs rb;
     Operand<T> A, B;
     int r0, rend, rows, s = (int)(from / n), t = (int)(from - (int64_t)s * n);
     bool whole_a, whole_b;
@@ -378,15 +496,15 @@ template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int F
     };
     auto load = [&]() {
       const int left = rend - r0 - t * BK;
-      ta.load(left, whole_a, tid);
-      tb.load(left, whole_b, tid);
-      if (rows < min(A.rows, m0 + BM)) ta.drop_rows(m0, rows, tid);
+      ta.load(ra, left, whole_a, m0, rows, rows < min(A.rows, m0 + BM), tid);
+      tb.load(rb, left, whole_b, n0, 0, false, tid);
     };
     seek();
     load();
-    ta.store(lds, tid);
-    tb.store(lds + TA::BYTES, tid);
+    TA::store(ra, lds, tid);
+    TB::store(rb, lds + TA::BYTES, tid);
     __syncthreads();
+    first(lds, lane, wm, wn);
     for (int it = 0; it < all; ++it) {
       char* cur = lds + (it & 1) * STAGE;
       char* nxt = lds + ((it + 1) & 1) * STAGE;
@@ -402,13 +520,16 @@ template <Kind K, bool A_ACROSS, bool B_ACROSS, int WM_, int WN_, int FM_, int F
         }
         load();
       }
-      compute(cur, cur + TA::BYTES, lane, wm, wn);
-      if (more) {
-        ta.store(nxt, tid);
-        tb.store(nxt + TA::BYTES, tid);
-      }
-      __syncthreads();
+      compute(cur, lane, wm, wn, [&]() -> const char* {
+        if (!more) return nullptr;
+        TA::store(ra, nxt, tid);  // everyone has read what was there: the tile before this one
+        TB::store(rb, nxt + TA::BYTES, tid);
+        wait_lds();
+        barrier();
+        return nxt;
+      });
     }
+    __syncthreads();
   }
 
   // f(m, n, v): 4 consecutive columns n .. n + 3 of row m, as the accumulators hold them: the 32 lanes of a half wave

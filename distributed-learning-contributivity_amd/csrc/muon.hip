@@ -236,7 +236,7 @@ __device__ __forceinline__ void store_planes_mirrored(const Planes& p, int g, in
 // GRAM: both operands are X and the sum runs over its rows
 template <Kind K, bool GRAM, Epi E, int WM, int WN, int FM, int FN>
 __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Prod p) {
-  typedef Block<F16, GRAM, GRAM, WM, WN, FM, FN, 64, 2> B;
+  typedef Block<F16, GRAM, GRAM, WM, WN, FM, FN, 64, 2, FM * FN == 1 ? 4 : 2> B;
   __shared__ __attribute__((aligned(16))) char lds[B::LDS_BYTES];
   int64_t b = xcd_block();
   int tm, tn;
@@ -258,14 +258,14 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Prod p) {
   oa.p[0] = p.a.hi + g * p.a.stride;
   oa.p[1] = p.a.lo + g * p.a.stride;
   oa.ld = p.a.ld;
-  oa.rows = p.m;
+  oa.rows = GRAM ? p.a.ld : p.m;  // whole chunks of columns: the planes' padding is zero
   ob.p[0] = p.b.hi + g * p.b.stride;
   ob.p[1] = p.b.lo + g * p.b.stride;
   ob.ld = p.b.ld;
-  ob.rows = p.n;
+  ob.rows = GRAM ? p.b.ld : p.n;
   B blk;
   blk.clear();
-  blk.run(lds, oa, ob, m0, n0, first * B::BK, min(p.r, last * B::BK));
+  blk.run(lds, oa, ob, m0, n0, first * B::BK, min(p.r, last * B::BK), true);
   auto value = [&](int m, int n, f32x4 v) {
     if constexpr (E == POLY) {
       const f32x4 a = load_planes(p.add, g, m, n);
