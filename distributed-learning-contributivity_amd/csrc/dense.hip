@@ -11,7 +11,7 @@
 // sums go through the workspace and a second kernel adds them in order and applies the epilogue.
 //
 // act'(z) needs dz as an operand of two products: one pass computes it, rounds it to the operands' type and sums its
-// columns (db) on the way, in fp32, per 128 rows, the blocks of rows added in order.
+// columns (db) on the way, in fp32, per 64 rows, the blocks of rows added in order.
 #include <math.h>
 
 #include "mma.h"
@@ -45,6 +45,7 @@ struct Product {
   int count_is_r;        // counts limit r (dw), not m
   int tiles_m, tiles_n, nk, splits, per_split;  // nk: units of r; per_split: units of a split
   int aligned;           // 16-byte rows: tiles go straight into LDS
+  int b_cols;            // across r: columns of B that may be read (n, or its padding too)
   float* partial;        // [split][model][m][n] where splits > 1
 };
 
@@ -54,11 +55,27 @@ __device__ __forceinline__ int count_of(const int32_t* counts, int g, int most) 
   return c < 0 ? 0 : (c > most ? most : c);
 }
 
-// a finite z far in the negative tail gives 0, so -infinity does too
+// Standard normal: the probability of values below z and its density.  The tail below -|z| is half of
+// erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), x = |z| / sqrt 2 (Abramowitz and Stegun 7.1.26, off by at
+// most 1.5e-7): a tenth of erff's instructions, and the exponential is the density's.
+__device__ __forceinline__ float normal(float z, float& density) {
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float e = __expf(-x * x);
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+  const float tail = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  density = 0.39894228040143268f * e;
+  return z < 0.f ? tail : 1.f - tail;
+}
+
+// far in the negative tail the result is 0, at -infinity too
 __device__ __forceinline__ float activate(int act, float z) {
   switch (act) {
     case MPLC_ACT_RELU: return z < 0.f ? 0.f : z;
-    case MPLC_ACT_GELU: return z < -64.f ? 0.f : 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case MPLC_ACT_GELU: {
+      float density;
+      const float p = normal(z, density);
+      return z < -64.f ? 0.f : z * p;
+    }
     case MPLC_ACT_SILU: return z < -1e4f ? 0.f : z / (1.f + __expf(-z));
     default: return z;
   }
@@ -66,9 +83,12 @@ __device__ __forceinline__ float activate(int act, float z) {
 __device__ __forceinline__ float slope(int act, float z) {
   switch (act) {
     case MPLC_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case MPLC_ACT_GELU:
+    case MPLC_ACT_GELU: {
       if (fabsf(z) > 64.f) return z > 0.f ? 1.f : 0.f;
-      return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+      float density;
+      const float p = normal(z, density);
+      return p + z * density;
+    }
     case MPLC_ACT_SILU: {
       if (fabsf(z) > 1e4f) return z > 0.f ? 1.f : 0.f;
       const float s = 1.f / (1.f + __expf(-z));
@@ -78,16 +98,26 @@ __device__ __forceinline__ float slope(int act, float z) {
   }
 }
 
-// z of 4 columns n .. of row m of model g -> z, y
-template <Kind K> __device__ __forceinline__ void finish(const Epilogue& e, int g, int m, int n, int N, f32x4 v) {
+template <Kind K> __device__ __forceinline__ f32x4 residual_at(const Epilogue& e, int g, int m, int n, int N) {
+  typedef typename Elem<K>::T T;
+  return e.res ? load4<K>(reinterpret_cast<const T*>(e.res) + g * e.res_stride + m * e.res_ld + n, N - n)
+               : f32x4{0.f, 0.f, 0.f, 0.f};
+}
+template <Kind K> __device__ __forceinline__ f32x4 bias_at(const Epilogue& e, int g, int n, int N) {
+  typedef typename Elem<K>::T T;
+  return e.bias ? load4<K>(reinterpret_cast<const T*>(e.bias) + g * e.bias_stride + n, N - n) : f32x4{0.f, 0.f, 0.f, 0.f};
+}
+// x w of 4 columns n .. of row m of model g -> z, y
+template <Kind K>
+__device__ __forceinline__ void finish(const Epilogue& e, int g, int m, int n, int N, f32x4 v, f32x4 bias, f32x4 res) {
   typedef typename Elem<K>::T T;
   const int valid = N - n;
-  if (e.bias) v += load4<K>(reinterpret_cast<const T*>(e.bias) + g * e.bias_stride + n, valid);
+  if (e.bias) v += bias;
   if (e.z) store4<F32>(e.z + g * e.z_stride + m * e.z_ld + n, v, valid);
   if (e.act != MPLC_ACT_NONE)
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = activate(e.act, v[i]);
-  if (e.res) v += load4<K>(reinterpret_cast<const T*>(e.res) + g * e.res_stride + m * e.res_ld + n, valid);
+  if (e.res) v += res;
   store4<K>(reinterpret_cast<T*>(e.out) + g * e.out_stride + m * e.out_ld + n, v, valid);
 }
 
@@ -151,18 +181,23 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
       });
     }
   } else {
-    const Operand<T> a = {{pa, nullptr}, p.a_ld, M}, o = {{pb, nullptr}, p.b_ld, p.n};
+    const Operand<T> a = {{pa, nullptr}, p.a_ld, M}, o = {{pb, nullptr}, p.b_ld, BA ? p.b_cols : p.n};
     blk.run(lds, a, o, m0, n0, (int)min((int64_t)R, first * unit_of(K)), (int)min((int64_t)R, last * unit_of(K)), p.aligned);
   }
   if (p.splits > 1) {
     float* out = p.partial + ((int64_t)split * p.models + g) * p.m * p.n;
-    blk.each_row(lds, m0, n0, [&](int m, int n, f32x4 v) {
+    blk.each_row(lds, m0, n0, [](int, int) { return 0; }, [&](int m, int n, f32x4 v, int) {
       if (m < M && n < p.n) store4<F32>(out + (int64_t)m * p.n + n, v, p.n - n);
     });
   } else {
-    blk.each_row(lds, m0, n0, [&](int m, int n, f32x4 v) {
-      if (m < M && n < p.n) finish<K>(e, g, m, n, p.n, v);
-    });
+    const int nl = n0 + B::lane_column();
+    const f32x4 bias = nl < p.n ? bias_at<K>(e, g, nl, p.n) : f32x4{0.f, 0.f, 0.f, 0.f};
+    blk.each_row(
+        lds, m0, n0,
+        [&](int m, int n) { return m < M && n < p.n ? residual_at<K>(e, g, m, n, p.n) : f32x4{0.f, 0.f, 0.f, 0.f}; },
+        [&](int m, int n, f32x4 v, f32x4 res) {
+          if (m < M && n < p.n) finish<K>(e, g, m, n, p.n, v, bias, res);
+        });
   }
 }
 
@@ -185,10 +220,10 @@ template <Kind K> __global__ __launch_bounds__(256) void join_kernel(const Produ
     for (int s = 0; s < 8; ++s)
       if (s0 + s < p.splits) v += x[s];
   }
-  finish<K>(e, g, m, n, p.n, v);
+  finish<K>(e, g, m, n, p.n, v, bias_at<K>(e, g, n, p.n), residual_at<K>(e, g, m, n, p.n));
 }
 
-constexpr int DZ_ROWS = 128;  // rows summed by one workgroup
+constexpr int DZ_ROWS = 64;  // rows summed by one workgroup: 16 a wave, 4 of them on their way at a time
 
 // dz = dy act'(z) and the sums of its columns over DZ_ROWS rows
 template <Kind K>
@@ -206,15 +241,24 @@ __global__ __launch_bounds__(256) void dz_kernel(const void* dy_, int64_t dy_str
   T* dz = dz_ ? reinterpret_cast<T*>(dz_) + (int64_t)g * rows * dz_ld : nullptr;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
   if (c < n)
-    for (int r = r0 + wave; r < r1; r += 4) {
-      f32x4 d = load4<K>(dy + r * dy_ld + c, n - c);
-      if (act != MPLC_ACT_NONE) {
-        const f32x4 zz = load4<F32>(z + g * z_stride + r * z_ld + c, n - c);
+    for (int r = r0 + wave; r < r1; r += 16) {
+      f32x4 d[4], zz[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] *= slope(act, zz[i]);
-        if (dz) store4<K>(dz + (int64_t)r * dz_ld + c, d, n - c);
-      }
-      sum += d;
+      for (int i = 0; i < 4; ++i)
+        if (r + 4 * i < r1) {
+          d[i] = load4<K>(dy + (r + 4 * i) * dy_ld + c, n - c);
+          if (act != MPLC_ACT_NONE) zz[i] = load4<F32>(z + g * z_stride + (r + 4 * i) * z_ld + c, n - c);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (r + 4 * i < r1) {
+          if (act != MPLC_ACT_NONE) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[i][e] *= slope(act, zz[i][e]);
+            if (dz) store4<K>(dz + (int64_t)(r + 4 * i) * dz_ld + c, d[i], n - c);
+          }
+          sum += d[i];
+        }
     }
   if (sums == nullptr && db_ == nullptr) return;
   part[wave][lane] = sum;
@@ -227,17 +271,28 @@ __global__ __launch_bounds__(256) void dz_kernel(const void* dy_, int64_t dy_str
   }
 }
 
+// db from the blocks' sums: 64 columns a workgroup, its waves take every fourth block
 template <Kind K>
-__global__ __launch_bounds__(256) void db_kernel(const float* sums, int blocks, int n, int used_rows,
-                                                 const int32_t* counts, void* db_, int64_t db_stride) {
+__global__ __launch_bounds__(256) void db_kernel(const float* sums, int blocks, int n, int rows, const int32_t* counts,
+                                                 void* db_, int64_t db_stride) {
   typedef typename Elem<K>::T T;
-  const int g = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= n) return;
-  const int cnt = count_of(counts, g, used_rows);
-  const int nb = min(blocks, (cnt + DZ_ROWS - 1) / DZ_ROWS);
+  __shared__ float part[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = blockIdx.y, c = blockIdx.x * 64 + lane;
+  const int nb = min(blocks, (count_of(counts, g, rows) + DZ_ROWS - 1) / DZ_ROWS);
   float v = 0.f;
-  for (int i = 0; i < nb; ++i) v += sums[((int64_t)g * blocks + i) * n + c];
-  reinterpret_cast<T*>(db_)[g * db_stride + c] = from_f32<K>(v);
+  if (c < n)
+    for (int i = wave; i < nb; i += 32) {
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = i + 4 * k < nb ? sums[((int64_t)g * blocks + i + 4 * k) * n + c] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v += x[k];
+    }
+  part[wave][lane] = v;
+  __syncthreads();
+  if (wave == 0 && c < n)
+    reinterpret_cast<T*>(db_)[g * db_stride + c] = from_f32<K>((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
 }
 
 // ---------------------------------------------------------------------------------------------- host
@@ -294,7 +349,7 @@ template <Kind K, bool AA, bool BA> hipError_t launch(Plan& pl, const Epilogue& 
     return ((uintptr_t)base & 15) == 0 && stride % ch == 0 && ld % ch == 0;
   };
   pl.p.aligned = fits(pl.p.a, pl.p.a_stride, pl.p.a_ld) && fits(pl.p.b, pl.p.b_stride, pl.p.b_ld) &&
-                 (!AA || pl.p.m % ch == 0) && (!BA || pl.p.n % ch == 0);
+                 (!AA || pl.p.m % ch == 0) && (!BA || pl.p.b_cols % ch == 0);
   const dim3 grid((unsigned)pl.blocks);
   if (pl.cfg == 0) product_kernel<K, AA, BA, 2, 2, 2, 2, 128, 2><<<grid, 256, 0, s>>>(pl.p, e);
   else if (pl.cfg == 1) product_kernel<K, AA, BA, 2, 2, 1, 1, 128, 3><<<grid, 256, 0, s>>>(pl.p, e);
@@ -356,6 +411,7 @@ template <Kind K> int forward(const mplc_dense_t& t, const Plan& pl0, hipStream_
   pl.p.b = t.w;
   pl.p.b_stride = t.w_stride;
   pl.p.b_ld = t.w_ld;
+  pl.p.b_cols = pl.p.n;
   pl.p.partial = reinterpret_cast<float*>(t.workspace);
   Epilogue e = {t.bias, t.bias_stride, t.residual, t.residual_stride, t.residual_ld, t.y, t.y_stride, t.y_ld,
                 t.z, t.z_stride, t.z_ld, t.activation};
@@ -374,7 +430,7 @@ template <Kind K> int backward(const mplc_dense_t& t, BackwardSpace& sp, hipStre
                                       t.counts, dz, sp.dz_ld, sums, sums ? nullptr : t.db, t.db_stride);
     if ((err = hipGetLastError()) != hipSuccess) return (int)err;
     if (sums) {
-      db_kernel<K><<<dim3((unsigned)ceil_div(t.out, 256), (unsigned)t.n_models), 256, 0, s>>>(
+      db_kernel<K><<<dim3((unsigned)ceil_div(t.out, 64), (unsigned)t.n_models), 256, 0, s>>>(
           sums, sp.blocks, t.out, t.rows, t.counts, t.db, t.db_stride);
       if ((err = hipGetLastError()) != hipSuccess) return (int)err;
     }
@@ -401,6 +457,7 @@ template <Kind K> int backward(const mplc_dense_t& t, BackwardSpace& sp, hipStre
     pl.p.a = t.x;
     pl.p.a_stride = t.x_shared ? 0 : t.x_stride;
     pl.p.a_ld = t.x_ld;
+    pl.p.b_cols = dz ? sp.dz_ld : pl.p.n;
     pl.p.b = d;
     pl.p.b_stride = d_stride;
     pl.p.b_ld = d_ld;

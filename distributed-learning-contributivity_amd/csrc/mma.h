@@ -249,11 +249,13 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
             for (int p = 0; p < PL; ++p) reg.v[p][j] = u32x4{0, 0, 0, 0};
         }
   }
-  __device__ __forceinline__ static void store(const Regs& reg, char* lds, int tid) {
+  __device__ __forceinline__ void store(const Regs& reg, char* lds, int tid) const {
 #pragma unroll
     for (int j = 0; j < PER; ++j)
 #pragma unroll
-      for (int p = 0; p < PL; ++p) *reinterpret_cast<u32x4*>(lds + p * PLANE_BYTES + (tid + j * NT) * 16) = reg.v[p][j];
+      for (int p = 0; p < PL; ++p) {
+        *reinterpret_cast<u32x4*>(lds + p * PLANE_BYTES + (tid + j * NT) * 16) = reg.v[p][j];
+      }
   }
   // the fragment of rows [i, i + 32) for k-step ks (2 chunks of r)
   __device__ __forceinline__ static u32x4 frag(const char* lds, int plane, int i, int ks, int lane) {
@@ -396,26 +398,49 @@ struct Block {
   // columns of an operand across r whole chunks.
   __device__ __forceinline__ void run(char* lds, const Operand<T>& A, const Operand<T>& B, int m0, int n0, int r0,
                                       int rend, bool aligned) {
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (r0 >= rend) return;
-    if (aligned) {
-      const int n = (rend - r0) / BK;
-      if (n > 0) ring(lds, m0, n0, n, 0, n, [&](int, Operand<T>& a, Operand<T>& b, int& first) {
-          a = A;
-          b = B;
-          first = r0;
-        });
-      r0 += n * BK;
-      if (r0 >= rend) return;
+    const int n = (rend - r0) / BK;
+    if (!aligned) {
+      through_registers(lds, m0, n0, (rend - r0 + BK - 1) / BK, 0, (rend - r0 + BK - 1) / BK,
+                        [&](int, Operand<T>& a, Operand<T>& b, int& first, int& end) {
+                          a = A;
+                          b = B;
+                          first = r0;
+                          end = rend;
+                          return A.rows;
+                        });
+      return;
     }
-    const int n = (rend - r0 + BK - 1) / BK;
-    through_registers(lds, m0, n0, n, 0, n, [&](int, Operand<T>& a, Operand<T>& b, int& first, int& end) {
-      a = A;
-      b = B;
-      first = r0;
-      end = rend;
-      return A.rows;
-    });
+    // the cut tile's loads go first, where there are registers for them: they have arrived when the others are done
+    const int cut = r0 + n * BK;
+    typename TA::Regs ra;
+    typename TB::Regs rb;
+    TA ta;
+    TB tb;
+    constexpr bool EARLY = PL == 1 && BM * BN < 256 * 256;
+    auto load_cut = [&]() {
+      ta.seek(A, m0, cut, tid);
+      tb.seek(B, n0, cut, tid);
+      ta.load(ra, rend - cut, true, m0, 0, false, tid);
+      tb.load(rb, rend - cut, true, n0, 0, false, tid);
+    };
+    if (EARLY && cut < rend) load_cut();
+    if (n > 0)
+      ring(lds, m0, n0, n, 0, n, [&](int, Operand<T>& a, Operand<T>& b, int& first) {
+        a = A;
+        b = B;
+        first = r0;
+      });
+    if (cut < rend) {
+      if (!EARLY) load_cut();
+      ta.store(ra, lds, tid);
+      tb.store(rb, lds + TA::BYTES, tid);
+      __syncthreads();
+      first(lds, lane, wave / WN, wave % WN);
+      compute(lds, lane, wave / WN, wave % WN, []() -> const char* { return nullptr; });
+      __syncthreads();
+    }
   }
 
   // acc += the sum over tiles [from, to) of pieces of n whole tiles each: at(s, A, B, r0) says where piece s is
@@ -501,8 +526,8 @@ struct Block {
     };
     seek();
     load();
-    TA::store(ra, lds, tid);
-    TB::store(rb, lds + TA::BYTES, tid);
+    ta.store(ra, lds, tid);
+    tb.store(rb, lds + TA::BYTES, tid);
     __syncthreads();
     first(lds, lane, wm, wn);
     for (int it = 0; it < all; ++it) {
@@ -522,14 +547,20 @@ struct Block {
       }
       compute(cur, lane, wm, wn, [&]() -> const char* {
         if (!more) return nullptr;
-        TA::store(ra, nxt, tid);  // everyone has read what was there: the tile before this one
-        TB::store(rb, nxt + TA::BYTES, tid);
+        ta.store(ra, nxt, tid);  // everyone has read what was there: the tile before this one
+        tb.store(rb, nxt + TA::BYTES, tid);
         wait_lds();
         barrier();
         return nxt;
       });
     }
     __syncthreads();
+  }
+
+  // the first of the columns, from n0, that each_row() gives this lane
+  static __device__ __forceinline__ int lane_column() {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    return (wave % WN) * FN * 32 + (lane % (8 * FN)) * 4;
   }
 
   // f(m, n, v): 4 consecutive columns n .. n + 3 of row m, as the accumulators hold them: the 32 lanes of a half wave
@@ -551,16 +582,22 @@ struct Block {
   }
 
   // The same with neighbouring lanes at neighbouring columns, 32 FN of a row, through the wave's own part of LDS (which
-  // run() has left): stores and the residual's loads cover whole lines.
-  template <typename F> __device__ __forceinline__ void each_row(char* lds, int m0, int n0, F f) const {
+  // run() has left): stores cover whole lines.  pre(m, n) loads what f(m, n, v, x) adds, for all rows of a pass before
+  // any of them is stored.
+  template <typename P, typename F> __device__ __forceinline__ void each_row(char* lds, int m0, int n0, P pre, F f) const {
     constexpr int LD = 32 * FN + 4;  // floats; the rows one pass writes fall on different banks
-    constexpr int PERROW = 8 * FN, ROWS = 64 / PERROW;
+    constexpr int PERROW = 8 * FN, ROWS = 64 / PERROW, N = 32 / ROWS;
     static_assert(WM * WN * 32 * LD * 4 <= LDS_BYTES, "the epilogue's rows fit");
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave / WN, wn = wave % WN;
     float* buf = reinterpret_cast<float*>(lds) + wave * 32 * LD;
+    const int col = (lane % PERROW) * 4, n = n0 + wn * FN * 32 + col;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
+      const int mi = m0 + (wm * FM + i) * 32 + lane / PERROW;
+      decltype(pre(0, 0)) x[N];
+#pragma unroll
+      for (int r = 0; r < N; ++r) x[r] = pre(mi + r * ROWS, n);
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -573,11 +610,8 @@ struct Block {
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int r = 0; r < 32; r += ROWS) {
-        const int row = r + lane / PERROW, col = (lane % PERROW) * 4;
-        const f32x4 v = *reinterpret_cast<const f32x4*>(buf + row * LD + col);
-        f(m0 + (wm * FM + i) * 32 + row, n0 + wn * FN * 32 + col, v);
-      }
+      for (int r = 0; r < N; ++r)
+        f(mi + r * ROWS, n, *reinterpret_cast<const f32x4*>(buf + (r * ROWS + lane / PERROW) * LD + col), x[r]);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }

@@ -193,25 +193,30 @@ struct Prod {
   float keep, step;  // STEP: w = keep w - step value
 };
 
-template <Kind K, Epi E> __device__ __forceinline__ void write_result(const Prod& p, int g, int m, int n, f32x4 v) {
+// what the result at (m, n .. n + 3) is added to (STEP)
+template <Kind K, Epi E> __device__ __forceinline__ f32x4 before_result(const Prod& p, int g, int m, int n) {
+  f32x4 w = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (E == STEP) {
+    const float* dst = reinterpret_cast<const float*>(p.dst) + g * p.dst_stride;
+    if (!p.transposed) return load4<F32>(dst + m * p.dst_ld + n, p.n - n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < p.n) w[i] = dst[(n + i) * p.dst_ld + m];
+  }
+  return w;
+}
+template <Kind K, Epi E> __device__ __forceinline__ void write_result(const Prod& p, int g, int m, int n, f32x4 v, f32x4 w) {
   typedef typename Elem<K>::T T;
   T* dst = reinterpret_cast<T*>(p.dst) + g * p.dst_stride;
-  if (!p.transposed) {
-    T* at = dst + m * p.dst_ld + n;
-    if constexpr (E == STEP) {
-      const f32x4 w = load4<K>(at, p.n - n);
+  if constexpr (E == STEP)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = p.keep * w[i] - p.step * v[i];
-    }
-    store4<K>(at, v, p.n - n);
+    for (int i = 0; i < 4; ++i) v[i] = p.keep * w[i] - p.step * v[i];
+  if (!p.transposed) {
+    store4<K>(dst + m * p.dst_ld + n, v, p.n - n);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (n + i < p.n) {
-        T* at = dst + (n + i) * p.dst_ld + m;
-        if constexpr (E == STEP) *at = from_f32<K>(p.keep * to_f32<K>(*at) - p.step * v[i]);
-        else *at = from_f32<K>(v[i]);
-      }
+      if (n + i < p.n) dst[(n + i) * p.dst_ld + m] = from_f32<K>(v[i]);
   }
 }
 
@@ -266,12 +271,19 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Prod p) {
   B blk;
   blk.clear();
   blk.run(lds, oa, ob, m0, n0, first * B::BK, min(p.r, last * B::BK), true);
-  auto value = [&](int m, int n, f32x4 v) {
+  auto before = [&](int m, int n) {
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (m < p.m && n < p.n) {
+      if constexpr (E == POLY) x = load_planes(p.add, g, m, n);
+      else if constexpr (E == STEP) x = before_result<K, E>(p, g, m, n);
+    }
+    return x;
+  };
+  auto value = [&](int m, int n, f32x4 v, f32x4 x) {
     if constexpr (E == POLY) {
-      const f32x4 a = load_planes(p.add, g, m, n);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        v[i] = p.cc * v[i] + p.cb * a[i];
+        v[i] = p.cc * v[i] + p.cb * x[i];
         if (n + i == m) v[i] += p.ca;
       }
     } else if constexpr (E != PARTIAL) {
@@ -283,20 +295,22 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Prod p) {
         if (n + i >= p.n) v[i] = 0.f;
     return v;
   };
-  auto result = [&](int m, int n, f32x4 v) {
+  auto result = [&](int m, int n, f32x4 v, f32x4 x) {
     if (m >= p.m || n >= p.n) return;
-    v = value(m, n, v);
+    v = value(m, n, v, x);
     if constexpr (E == PARTIAL)
       store4<F32>(p.partial + ((int64_t)sp * p.models + g) * p.m * p.n + (int64_t)m * p.n + n, v, p.n - n);
     else if constexpr (E == PLANES || E == POLY) store_planes(p.out, g, m, n, v);
-    else write_result<K, E>(p, g, m, n, v);
+    else write_result<K, E>(p, g, m, n, v, x);
   };
-  if ((E == OUT || E == STEP) && p.transposed) blk.each(m0, n0, result);
-  else blk.each_row(lds, m0, n0, result);
+  if ((E == OUT || E == STEP) && p.transposed)
+    blk.each(m0, n0, [&](int m, int n, f32x4 v) { result(m, n, v, before(m, n)); });
+  else
+    blk.each_row(lds, m0, n0, before, result);
   if constexpr (E == PLANES || E == POLY)
     if (p.symmetric && tm != tn)
       blk.each(m0, n0, [&](int m, int n, f32x4 v) {
-        if (m < p.m && n < p.n) store_planes_mirrored(p.out, g, m, n, p.n, value(m, n, v));
+        if (m < p.m && n < p.n) store_planes_mirrored(p.out, g, m, n, p.n, value(m, n, v, before(m, n)));
       });
 }
 
