@@ -163,8 +163,8 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
     };
     const int64_t from = tile_at(first), to = tile_at(last);
     auto at = [&](int s, Operand<T>& a, Operand<T>& o, int& r0) {
-      a.p[0] = pa + s * p.a_stride;
-      o.p[0] = pb + s * p.b_stride;
+      a.p = pa + s * p.a_stride;
+      o.p = pb + s * p.b_stride;
       a.ld = p.a_ld;
       o.ld = p.b_ld;
       a.rows = p.m;
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
       });
     }
   } else {
-    const Operand<T> a = {{pa, nullptr}, p.a_ld, M}, o = {{pb, nullptr}, p.b_ld, BA ? p.b_cols : p.n};
+    const Operand<T> a = {pa, p.a_ld, M}, o = {pb, p.b_ld, BA ? p.b_cols : p.n};
     blk.run(lds, a, o, m0, n0, (int)min((int64_t)R, first * unit_of(K)), (int)min((int64_t)R, last * unit_of(K)), p.aligned);
   }
   if (p.splits > 1) {
@@ -223,47 +223,53 @@ template <Kind K> __global__ __launch_bounds__(256) void join_kernel(const Produ
   finish<K>(e, g, m, n, p.n, v, bias_at<K>(e, g, n, p.n), residual_at<K>(e, g, m, n, p.n));
 }
 
-constexpr int DZ_ROWS = 64;  // rows summed by one workgroup: 16 a wave, 4 of them on their way at a time
+constexpr int DZ_ROWS = 64;  // rows summed by one workgroup
 
-// dz = dy act'(z) and the sums of its columns over DZ_ROWS rows
-template <Kind K>
+// dz = dy act'(z) and the sums of its columns over DZ_ROWS rows.  A wave takes LANES groups of 4 columns of 64 / LANES
+// rows at a time (a narrow matrix would leave lanes idle), 4 such passes in flight.
+template <Kind K, int LANES>
 __global__ __launch_bounds__(256) void dz_kernel(const void* dy_, int64_t dy_stride, int64_t dy_ld, const float* z,
                                                  int64_t z_stride, int64_t z_ld, int act, int rows, int n,
                                                  const int32_t* counts, void* dz_, int dz_ld, float* sums, void* db_,
                                                  int64_t db_stride) {
   typedef typename Elem<K>::T T;
-  __shared__ f32x4 part[4][64];
+  constexpr int STEP = 4 * (64 / LANES);  // rows of a pass of the workgroup
+  __shared__ f32x4 part[4][LANES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int g = blockIdx.z, c = (blockIdx.x * 64 + lane) * 4;
+  const int g = blockIdx.z, c = (blockIdx.x * LANES + lane % LANES) * 4;
   const int cnt = count_of(counts, g, rows);
   const int r0 = blockIdx.y * DZ_ROWS, r1 = min(cnt, r0 + DZ_ROWS);
   const T* dy = reinterpret_cast<const T*>(dy_) + g * dy_stride;
   T* dz = dz_ ? reinterpret_cast<T*>(dz_) + (int64_t)g * rows * dz_ld : nullptr;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
   if (c < n)
-    for (int r = r0 + wave; r < r1; r += 16) {
+    for (int r = r0 + wave * (64 / LANES) + lane / LANES; r < r1; r += 4 * STEP) {
       f32x4 d[4], zz[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (r + 4 * i < r1) {
-          d[i] = load4<K>(dy + (r + 4 * i) * dy_ld + c, n - c);
-          if (act != MPLC_ACT_NONE) zz[i] = load4<F32>(z + g * z_stride + (r + 4 * i) * z_ld + c, n - c);
+        if (r + STEP * i < r1) {
+          d[i] = load4<K>(dy + (r + STEP * i) * dy_ld + c, n - c);
+          if (act != MPLC_ACT_NONE) zz[i] = load4<F32>(z + g * z_stride + (r + STEP * i) * z_ld + c, n - c);
         }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (r + 4 * i < r1) {
+        if (r + STEP * i < r1) {
           if (act != MPLC_ACT_NONE) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[i][e] *= slope(act, zz[i][e]);
-            if (dz) store4<K>(dz + (int64_t)(r + 4 * i) * dz_ld + c, d[i], n - c);
+            if (dz) store4<K>(dz + (int64_t)(r + STEP * i) * dz_ld + c, d[i], n - c);
           }
           sum += d[i];
         }
     }
   if (sums == nullptr && db_ == nullptr) return;
-  part[wave][lane] = sum;
+#pragma unroll
+  for (int d = 32; d >= LANES; d >>= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], d, 64);
+  if (lane < LANES) part[wave][lane] = sum;
   __syncthreads();
-  if (wave == 0 && c < n) {
+  if (wave == 0 && lane < LANES && c < n) {
     f32x4 v = part[0][lane] + part[1][lane];
     v += part[2][lane] + part[3][lane];
     if (sums) store4<F32>(sums + ((int64_t)g * gridDim.y + blockIdx.y) * n + c, v, n - c);
@@ -309,8 +315,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Multiply-adds per cycle and CU (measured on large products; 0: shape not built).  256 x 256 in fp32 would leave one
 // wave per SIMD without gaining anything: the fp32 matrix rate is reached by 128 x 128.
-constexpr TileShape SHAPES_16[5] = {{128, 128, 2, 640.f}, {64, 64, 3, 330.f}, {32, 128, 2, 280.f}, {256, 256, 1, 840.f},
-                                    {64, 128, 2, 450.f}};
+constexpr TileShape SHAPES_16[5] = {{128, 128, 2, 640.f}, {64, 64, 3, 330.f}, {32, 128, 2, 280.f}, {256, 256, 1, 900.f},
+                                    {64, 128, 3, 450.f}};
 constexpr TileShape SHAPES_F32[5] = {{128, 128, 2, 115.f}, {64, 64, 4, 105.f}, {32, 128, 3, 95.f}, {256, 256, 1, 0.f},
                                      {64, 128, 3, 108.f}};
 
@@ -331,6 +337,9 @@ bool plan(const mplc_dense_t& t, Form form, Plan& out) {
   if (units > INT32_MAX) return false;
   const Choice c = choose(f32 ? SHAPES_F32 : SHAPES_16, 5, p.models, p.m, p.n, (int64_t)p.r * p.segments, units, true);
   out.cfg = c.tile;
+  // A short sum is bound by its operands' latency and its result's stores: tiles of half the length leave LDS for three
+  // workgroups per CU (45 x 9216 x 128 from 51 rows: 103 us against 142).  Operands along r would fetch half lines.
+  if (form == DW && c.tile == 0 && p.nk <= 2) out.cfg = 5;
   p.splits = c.splits;
   p.per_split = c.per_split;
   const int64_t tiles = c.tiles_m * c.tiles_n * p.models;
@@ -353,9 +362,12 @@ template <Kind K, bool AA, bool BA> hipError_t launch(Plan& pl, const Epilogue& 
   const dim3 grid((unsigned)pl.blocks);
   if (pl.cfg == 0) product_kernel<K, AA, BA, 2, 2, 2, 2, 128, 2><<<grid, 256, 0, s>>>(pl.p, e);
   else if (pl.cfg == 1) product_kernel<K, AA, BA, 2, 2, 1, 1, 128, 3><<<grid, 256, 0, s>>>(pl.p, e);
-  else if (pl.cfg == 4) product_kernel<K, AA, BA, 1, 4, 2, 1, 128, 3><<<grid, 256, 0, s>>>(pl.p, e);
+  else if (pl.cfg == 4) product_kernel<K, AA, BA, 1, 4, 2, 1, 128, 2><<<grid, 256, 0, s>>>(pl.p, e);
   else if (pl.cfg == 3) {
     if constexpr (K != F32) product_kernel<K, AA, BA, 2, 4, 4, 2, 128, 2><<<grid, 512, 0, s>>>(pl.p, e);
+  }
+  else if (pl.cfg == 5) {
+    if constexpr (AA && BA) product_kernel<K, AA, BA, 2, 2, 2, 2, 64, 3><<<grid, 256, 0, s>>>(pl.p, e);
   }
   else product_kernel<K, AA, BA, 1, 4, 1, 1, 128, 3><<<grid, 256, 0, s>>>(pl.p, e);
   hipError_t err = hipGetLastError();
@@ -425,9 +437,15 @@ template <Kind K> int backward(const mplc_dense_t& t, BackwardSpace& sp, hipStre
   float* partial = reinterpret_cast<float*>(ws + sp.dz + sp.sums);
   hipError_t err;
   if (dz || t.db) {
-    const dim3 grid((unsigned)ceil_div(t.out, 256), (unsigned)(sp.blocks ? sp.blocks : 1), (unsigned)t.n_models);
-    dz_kernel<K><<<grid, 256, 0, s>>>(t.dy, t.dy_stride, t.dy_ld, t.z, t.z_stride, t.z_ld, t.activation, t.rows, t.out,
-                                      t.counts, dz, sp.dz_ld, sums, sums ? nullptr : t.db, t.db_stride);
+    const int lanes = t.out > 128 ? 64 : t.out > 64 ? 32 : 16;
+    const dim3 grid((unsigned)ceil_div(t.out, 4 * lanes), (unsigned)(sp.blocks ? sp.blocks : 1), (unsigned)t.n_models);
+    auto go = [&](auto kernel) {
+      kernel<<<grid, 256, 0, s>>>(t.dy, t.dy_stride, t.dy_ld, t.z, t.z_stride, t.z_ld, t.activation, t.rows, t.out,
+                                  t.counts, dz, sp.dz_ld, sums, sums ? nullptr : t.db, t.db_stride);
+    };
+    if (lanes == 64) go(dz_kernel<K, 64>);
+    else if (lanes == 32) go(dz_kernel<K, 32>);
+    else go(dz_kernel<K, 16>);
     if ((err = hipGetLastError()) != hipSuccess) return (int)err;
     if (sums) {
       db_kernel<K><<<dim3((unsigned)ceil_div(t.out, 64), (unsigned)t.n_models), 256, 0, s>>>(

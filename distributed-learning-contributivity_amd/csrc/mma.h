@@ -147,9 +147,10 @@ template <Kind K> __device__ __forceinline__ void mfma(f32x16& d, const u32x4& a
   }
 }
 
-// One operand of the product as the kernel sees it.
+// One operand of the product as the kernel sees it.  Two planes lie in one row, in blocks of 32 elements of the one and
+// then of the other.
 template <typename T> struct Operand {
-  const T* p[2];   // planes (p[1] only where PL = 2)
+  const T* p;
   int64_t ld;
   int rows;        // valid i
 };
@@ -193,20 +194,22 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
       if constexpr (ACROSS) {
         const int i = i0 + ch * CH;
         live[j] = o.rows - i;
-        off = (int64_t)(r0 + row) * o.ld + (live[j] > 0 ? i : 0);
+        off = (int64_t)(r0 + row) * o.ld + (live[j] > 0 ? column(i) : 0);
       } else {
-        off = (int64_t)min(i0 + row, o.rows - 1) * o.ld + r0 + ch * CH;
+        off = (int64_t)min(i0 + row, o.rows - 1) * o.ld + column(r0 + ch * CH);
       }
 #pragma unroll
-      for (int p = 0; p < PL; ++p) ptr[p][j] = o.p[p] + off;
+      for (int p = 0; p < PL; ++p) ptr[p][j] = o.p + off + 32 * p;
     }
   }
   __device__ __forceinline__ void advance(int64_t ld) {
 #pragma unroll
     for (int p = 0; p < PL; ++p)
 #pragma unroll
-      for (int j = 0; j < PER; ++j) ptr[p][j] += ACROSS ? BK * ld : BK;
+      for (int j = 0; j < PER; ++j) ptr[p][j] += ACROSS ? BK * ld : BK * PL;
   }
+  static_assert(PL == 1 || BK == 32, "a tile along r is a block of each plane");
+  __device__ __forceinline__ static int column(int c) { return PL == 1 ? c : ((c >> 5) << 6) + (c & 31); }
   // the whole tile at ptr into LDS; counts as PL * PER loads of the wave
   __device__ __forceinline__ void fetch(char* lds, int tid) const {
     typedef __attribute__((address_space(3))) uint32_t lds_u32;

@@ -29,12 +29,16 @@ constexpr float X_SCALE = 16384.f;  // |X| <= 2
 constexpr float A_SCALE = 8192.f;   // |A|, |P A| <= 4
 constexpr int NORM_CHUNKS = 256;
 
-struct Planes {  // split fp16 of a matrix times its scale
-  uint16_t* hi;
-  uint16_t* lo;
+// Split fp16 of a matrix times its scale.  Rows of 32-column blocks, 32 hi then 32 lo: both planes' pieces of a tile lie in
+// one 128-byte line (planes of their own cost each operand along r half a line, fetched twice).
+struct Planes {
+  uint16_t* p;
   int64_t stride;  // elements of one model
-  int ld;
+  int ld;          // elements of a row: 2 * (columns rounded up to 32)
 };
+__device__ __forceinline__ int64_t plane_at(const Planes& p, int g, int64_t m, int n) {
+  return g * p.stride + m * p.ld + ((n >> 5) << 6) + (n & 31);
+}
 
 __device__ __forceinline__ void split(float v, uint16_t& hi, uint16_t& lo) {
   hi = f32_to_f16(v);
@@ -44,18 +48,18 @@ __device__ __forceinline__ void store_planes(const Planes& p, int g, int64_t m, 
   uint16_t h[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) split(v[i], h[i], l[i]);
-  const int64_t at = g * p.stride + m * p.ld + n;  // n and ld are multiples of 4: 8-byte aligned
+  uint16_t* at = p.p + plane_at(p, g, m, n);  // n is a multiple of 4: 8-byte aligned
   u32x2 a, b;
   a[0] = h[0] | (uint32_t)h[1] << 16;
   a[1] = h[2] | (uint32_t)h[3] << 16;
   b[0] = l[0] | (uint32_t)l[1] << 16;
   b[1] = l[2] | (uint32_t)l[3] << 16;
-  *reinterpret_cast<u32x2*>(p.hi + at) = a;
-  *reinterpret_cast<u32x2*>(p.lo + at) = b;
+  *reinterpret_cast<u32x2*>(at) = a;
+  *reinterpret_cast<u32x2*>(at + 32) = b;
 }
 __device__ __forceinline__ f32x4 load_planes(const Planes& p, int g, int64_t m, int n) {
-  const int64_t at = g * p.stride + m * p.ld + n;
-  const u32x2 a = *reinterpret_cast<const u32x2*>(p.hi + at), b = *reinterpret_cast<const u32x2*>(p.lo + at);
+  const uint16_t* at = p.p + plane_at(p, g, m, n);
+  const u32x2 a = *reinterpret_cast<const u32x2*>(at), b = *reinterpret_cast<const u32x2*>(at + 32);
   f32x4 v;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -138,13 +142,14 @@ template <Kind K> __global__ __launch_bounds__(256) void norm_kernel(const Sourc
   if (threadIdx.x == 0) sums[(int64_t)g * gridDim.x + blockIdx.x] = sum;
 }
 
-// X_0 as planes [L][ld]; L = rows
+// X_0 as planes of L = rows rows, the columns behind k zero
 template <Kind K> __global__ __launch_bounds__(256) void start_kernel(const Source s, const double* sums, int chunks, const Planes x) {
   __shared__ double part[4];
   const int g = blockIdx.y;
   const double inv = inverse_norm(block_sum(threadIdx.x < chunks ? sums[(int64_t)g * chunks + threadIdx.x] : 0., part));
-  for (Walk w(blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, (s.cols + 3) >> 2); w.r < s.rows; w.next()) {
-    f32x4 v = update4<K, false>(s, g, w.r, w.c4 * 4, s.cols - w.c4 * 4);
+  for (Walk w(blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, x.ld >> 3); w.r < s.rows; w.next()) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (w.c4 * 4 < s.cols) v = update4<K, false>(s, g, w.r, w.c4 * 4, s.cols - w.c4 * 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (float)((double)v[i] * inv);
     store_planes(x, g, w.r, w.c4 * 4, v);
@@ -167,7 +172,7 @@ template <Kind K> __global__ __launch_bounds__(256) void start_wide_kernel(const
   }
   __syncthreads();
   for (int i = ty; i < 64; i += 16)
-    if (l0 + i < s.cols && k0 + q < x.ld) {
+    if (l0 + i < s.cols && k0 + q < (x.ld >> 1)) {
       f32x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = k0 + q + e < s.rows ? tile[i][q + e] : 0.f;
@@ -233,15 +238,15 @@ __device__ __forceinline__ void store_planes_mirrored(const Planes& p, int g, in
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (n + i < N) {
-      const int64_t at = g * p.stride + (int64_t)(n + i) * p.ld + m;
-      split(v[i], p.hi[at], p.lo[at]);
+      uint16_t* at = p.p + plane_at(p, g, n + i, m);
+      split(v[i], at[0], at[32]);
     }
 }
 
 // GRAM: both operands are X and the sum runs over its rows
-template <Kind K, bool GRAM, Epi E, int WM, int WN, int FM, int FN>
+template <Kind K, bool GRAM, Epi E, int WM, int WN, int FM, int FN, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Prod p) {
-  typedef Block<F16, GRAM, GRAM, WM, WN, FM, FN, 64, 2, FM * FN == 1 ? 4 : 2> B;
+  typedef Block<F16, GRAM, GRAM, WM, WN, FM, FN, 64, 2, STAGES> B;
   __shared__ __attribute__((aligned(16))) char lds[B::LDS_BYTES];
   int64_t b = xcd_block();
   int tm, tn;
@@ -257,24 +262,23 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Prod p) {
   }
   const int sp = (int)(b % p.splits), g = (int)(b / p.splits);
   const int m0 = tm * B::BM, n0 = tn * B::BN;
-  const int nk = (p.r + B::BK - 1) / B::BK;
+  const int rend = GRAM ? p.r : p.a.ld / 2;  // along r: zeros behind p.r
+  const int nk = (rend + B::BK - 1) / B::BK;
   const int first = sp * p.per_split, last = min(nk, first + p.per_split);
   Operand<uint16_t> oa, ob;
-  oa.p[0] = p.a.hi + g * p.a.stride;
-  oa.p[1] = p.a.lo + g * p.a.stride;
+  oa.p = p.a.p + g * p.a.stride;
   oa.ld = p.a.ld;
-  oa.rows = GRAM ? p.a.ld : p.m;  // whole chunks of columns: the planes' padding is zero
-  ob.p[0] = p.b.hi + g * p.b.stride;
-  ob.p[1] = p.b.lo + g * p.b.stride;
+  oa.rows = GRAM ? p.a.ld / 2 : p.m;  // whole chunks of columns: the planes' padding is zero
+  ob.p = p.b.p + g * p.b.stride;
   ob.ld = p.b.ld;
-  ob.rows = GRAM ? p.b.ld : p.n;
+  ob.rows = GRAM ? p.b.ld / 2 : p.n;
   B blk;
   blk.clear();
-  blk.run(lds, oa, ob, m0, n0, first * B::BK, min(p.r, last * B::BK), true);
+  blk.run(lds, oa, ob, m0, n0, first * B::BK, min(rend, last * B::BK), true);
   auto before = [&](int m, int n) {
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     if (m < p.m && n < p.n) {
-      if constexpr (E == POLY) x = load_planes(p.add, g, m, n);
+      if constexpr (E == POLY) x = load_planes(p.add, g, m, n);  // zeros behind the last column
       else if constexpr (E == STEP) x = before_result<K, E>(p, g, m, n);
     }
     return x;
@@ -296,7 +300,8 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Prod p) {
     return v;
   };
   auto result = [&](int m, int n, f32x4 v, f32x4 x) {
-    if (m >= p.m || n >= p.n) return;
+    // planes: zeros behind the last column too
+    if (m >= p.m || n >= (E == PLANES || E == POLY ? p.out.ld / 2 : p.n)) return;
     v = value(m, n, v, x);
     if constexpr (E == PARTIAL)
       store4<F32>(p.partial + ((int64_t)sp * p.models + g) * p.m * p.n + (int64_t)m * p.n + n, v, p.n - n);
@@ -310,7 +315,8 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Prod p) {
   if constexpr (E == PLANES || E == POLY)
     if (p.symmetric && tm != tn)
       blk.each(m0, n0, [&](int m, int n, f32x4 v) {
-        if (m < p.m && n < p.n) store_planes_mirrored(p.out, g, m, n, p.n, value(m, n, v, before(m, n)));
+        if (m < p.out.ld / 2 && n < p.n)  // its zeros behind the last column too
+          store_planes_mirrored(p.out, g, m, n, p.n, m < p.m ? value(m, n, v, before(m, n)) : f32x4{0.f, 0.f, 0.f, 0.f});
       });
 }
 
@@ -332,8 +338,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Prod p) {
       v = load4<F32>(at, p.n - n);
       for (int s = 1; s < p.splits; ++s) v += load4<F32>(at + s * step, p.n - n);
       v *= p.alpha;
-      store_planes(p.out, g, m, n, v);
     }
+    if (m < p.m && n < p.out.ld / 2) store_planes(p.out, g, m, n, v);
 #pragma unroll
     for (int e = 0; e < 4; ++e) tile[q + e][i] = v[e];
   }
@@ -343,7 +349,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Prod p) {
     f32x4 v;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = tile[i][q + e];
-    if (n0 + i < p.n && m0 + q < p.m) store_planes(p.out, g, n0 + i, m0 + q, v);
+    if (n0 + i < p.n && m0 + q < p.out.ld / 2) store_planes(p.out, g, n0 + i, m0 + q, v);
   }
 }
 
@@ -541,13 +547,17 @@ template <Kind K, int KT, Epi E> __global__ __launch_bounds__(256) void small_ke
 constexpr int NARROW_THREADS = 512;  // with Q in LDS: one workgroup per CU
 constexpr int GRAM_THREADS = 256;    // without: several, whose conversions and products overlap
 
+struct Square {  // planes of a KP x KP matrix as they lie in LDS, hi then lo, one after the other for each model
+  char* p;
+};
+
 struct Narrow {
   Source src;
   int L, k, chunks, rows_per;  // chunks per model, rows l of one
   float* partial;              // [model][chunk][tile][1024]
   int* exponent;               // [model][chunk]
   double* inv;                 // [model] 1 / |U|
-  Planes q;                    // [model] Q in the square layout of LDS
+  Square q;                    // [model] Q
   float q_scale;
   void* dst;
   int64_t dst_stride, dst_ld;
@@ -771,13 +781,11 @@ __global__ __launch_bounds__(256) void narrow_join_kernel(float* partial, const 
   *reinterpret_cast<f32x4*>(at) = v;
 }
 
-// Q (planes in the square layout) to LDS
-template <int KP> __device__ __forceinline__ void load_square(char* lds, const Planes& q, int g) {
-  constexpr int BYTES = KP * KP * 2;
-  for (int i = threadIdx.x * 16; i < BYTES; i += blockDim.x * 16) {
-    *reinterpret_cast<u32x4*>(lds + i) = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(q.hi + g * q.stride) + i);
-    *reinterpret_cast<u32x4*>(lds + BYTES + i) = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(q.lo + g * q.stride) + i);
-  }
+template <int KP> __device__ __forceinline__ void load_square(char* lds, const Square& q, int g) {
+  constexpr int BYTES = KP * KP * 4;
+  const char* src = q.p + (int64_t)g * BYTES;
+  for (int i = threadIdx.x * 16; i < BYTES; i += blockDim.x * 16)
+    *reinterpret_cast<u32x4*>(lds + i) = *reinterpret_cast<const u32x4*>(src + i);
 }
 
 // passes 2 and 3: Y = U Q / |U| by TR rows.  GRAM: partial Gram matrices of Y; otherwise Y is the result.
@@ -892,9 +900,9 @@ struct Chain {
   double* inv;
   float a, b, c;
   float p_scale[3], q_scale[3];  // of step i
-  Planes before;                 // Q of the phase before (before.hi = NULL: none), in the square layout
+  Square before;                 // Q of the phase before (NULL: none)
   float before_scale;
-  Planes q;                      // the product of all Q so far
+  Square q;                      // the product of all Q so far
   float total_scale;
 };
 
@@ -1018,7 +1026,7 @@ template <int KP> __global__ __launch_bounds__(KP * 4) void chain_kernel(const C
       __syncthreads();
     }
   }
-  if (p.before.hi) {  // times the phase before
+  if (p.before.p) {  // times the phase before
     __syncthreads();
     load_square<KP>(s1, p.before, g);
     put(s2, Q, q_scale);
@@ -1028,10 +1036,9 @@ template <int KP> __global__ __launch_bounds__(KP * 4) void chain_kernel(const C
   __syncthreads();
   put(s1, Q, p.total_scale);
   __syncthreads();
-  for (int i = threadIdx.x * 16; i < MAT; i += NT * 16) {
-    *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(p.q.hi + g * p.q.stride) + i) = *reinterpret_cast<const u32x4*>(s1 + i);
-    *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(p.q.lo + g * p.q.stride) + i) = *reinterpret_cast<const u32x4*>(s1 + MAT + i);
-  }
+  char* out = p.q.p + (int64_t)g * (2 * MAT);
+  for (int i = threadIdx.x * 16; i < 2 * MAT; i += NT * 16)
+    *reinterpret_cast<u32x4*>(out + i) = *reinterpret_cast<const u32x4*>(s1 + i);
 }
 
 // ------------------------------------------------------------------------------------------ host
@@ -1039,7 +1046,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align16(size_t v) { return (v + 15) & ~(size_t)15; }
 
 // Multiply-adds per cycle and CU of split products (measured on large ones)
-constexpr TileShape SHAPES[3] = {{256, 256, 1, 280.f}, {128, 128, 2, 205.f}, {64, 64, 3, 120.f}};
+// The last: one workgroup per CU with twice the tiles in flight, for products too small for two.
+constexpr TileShape SHAPES[4] = {{256, 256, 1, 300.f}, {128, 128, 2, 250.f}, {64, 64, 2, 130.f}, {128, 128, 1, 220.f}};
 
 // LDS of small_kernel, 0 where the matrix does not fit
 size_t small_bytes(int L, int k) {
@@ -1061,7 +1069,7 @@ struct Space {
 Choice shape_for(int64_t models, int64_t m, int64_t n, int64_t r, bool symmetric, bool can_split) {
   Choice best = {};
   double least = 0;
-  for (int s = 0; s < 3; ++s) {  // choose() per shape, its tiles halved where the result is symmetric
+  for (int s = 0; s < 4; ++s) {  // choose() per shape, its tiles halved where the result is symmetric
     TileShape one = SHAPES[s];
     const int64_t t = ceil_div(m, one.bm);
     const int64_t tiles = symmetric ? t * (t + 1) / 2 : t * ceil_div(n, one.bn);
@@ -1088,7 +1096,7 @@ bool space(const mplc_muon_t& t, Space& s) {
   s = Space{};
   s.k = t.rows < t.cols ? t.rows : t.cols;
   s.L = t.rows < t.cols ? t.cols : t.rows;
-  s.ld = (s.k + 7) & ~7;
+  s.ld = 2 * ((s.k + 31) & ~31);
   s.phases = 2 * (int64_t)s.L >= 3 * (int64_t)s.k ? (t.steps + 2) / 3 : t.steps;
   s.small = small_bytes(s.L, s.k);
   if (s.small) {  // reading X again costs nothing here: phases of two steps lose less to the Gram matrix's error
@@ -1107,7 +1115,7 @@ bool space(const mplc_muon_t& t, Space& s) {
     const size_t G = (size_t)t.n_models, tiles = s.narrow == 128 ? 10 : 3;
     s.sums = align16(G * s.chunks * sizeof(int)) + align16(G * sizeof(double));
     s.partial = align16(G * s.chunks * tiles * 4096);
-    s.square = align16(G * s.narrow * s.narrow * 2) * 2;
+    s.square = G * s.narrow * s.narrow * 4;
     s.total = s.sums + s.partial + 2 * s.square;
     return true;
   }
@@ -1119,8 +1127,8 @@ bool space(const mplc_muon_t& t, Space& s) {
   s.gram = shape_for(t.n_models, s.k, s.k, s.L, true, true);
   const size_t G = (size_t)t.n_models;
   s.sums = align16(G * s.chunks * sizeof(double));
-  s.x = align16(G * s.L * s.ld * 2) * 2;       // both planes
-  s.square = align16(G * s.k * s.ld * 2) * 2;
+  s.x = align16(G * s.L * s.ld * 2);
+  s.square = align16(G * s.k * s.ld * 2);
   s.partial = s.gram.splits > 1 ? align16(G * s.gram.splits * (size_t)s.k * s.k * sizeof(float)) : 0;
   s.total = s.sums + s.n_x * s.x + 6 * s.square + s.partial;
   return ceil_div(s.L, 64) * ceil_div(s.k, 64) * (int64_t)t.n_models <= (1 << 23) &&
@@ -1165,9 +1173,10 @@ template <Kind K, bool GRAM, Epi E> hipError_t product(Prod p, const Choice& c, 
   p.splits = c.splits;
   p.per_split = c.per_split;
   const dim3 grid((unsigned)blocks_of(c, p.models, p.symmetric));
-  if (c.tile == 0) product_kernel<K, GRAM, E, 2, 4, 4, 2><<<grid, 512, 0, s>>>(p);
-  else if (c.tile == 1) product_kernel<K, GRAM, E, 2, 2, 2, 2><<<grid, 256, 0, s>>>(p);
-  else product_kernel<K, GRAM, E, 2, 2, 1, 1><<<grid, 256, 0, s>>>(p);
+  if (c.tile == 0) product_kernel<K, GRAM, E, 2, 4, 4, 2, 2><<<grid, 512, 0, s>>>(p);
+  else if (c.tile == 1) product_kernel<K, GRAM, E, 2, 2, 2, 2, 2><<<grid, 256, 0, s>>>(p);
+  else if (c.tile == 2) product_kernel<K, GRAM, E, 2, 2, 1, 1, 4><<<grid, 256, 0, s>>>(p);
+  else product_kernel<K, GRAM, E, 2, 2, 2, 2, 4><<<grid, 256, 0, s>>>(p);
   return hipGetLastError();
 }
 
@@ -1213,9 +1222,9 @@ int launch_narrow(const mplc_muon_t& t, const Space& sp, const Source& src, hipS
   ws += align16((size_t)t.n_models * sizeof(double));
   p.partial = reinterpret_cast<float*>(ws);
   ws += sp.partial;
-  Planes q[2];
+  Square q[2];
   for (int i = 0; i < 2; ++i) {
-    q[i] = Planes{reinterpret_cast<uint16_t*>(ws), reinterpret_cast<uint16_t*>(ws + sp.square / 2), KP * KP, KP};
+    q[i].p = ws;
     ws += sp.square;
   }
   if (E == STEP) {
@@ -1283,7 +1292,7 @@ template <Kind K, Epi LAST> int run(const mplc_muon_t& t, const Space& sp, const
   double* sums = reinterpret_cast<double*>(ws);
   ws += sp.sums;
   auto planes = [&](size_t bytes, int64_t stride) {
-    Planes p = {reinterpret_cast<uint16_t*>(ws), reinterpret_cast<uint16_t*>(ws + bytes / 2), stride, sp.ld};
+    Planes p = {reinterpret_cast<uint16_t*>(ws), stride, sp.ld};
     ws += bytes;
     return p;
   };
