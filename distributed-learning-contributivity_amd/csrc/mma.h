@@ -344,15 +344,25 @@ struct Block {
       for (int j = 0; j < FN; ++j) f.b[p][j] = TB::frag(lb, p, (wn * FN + j) * 32, ks, lane);
     }
   }
-  __device__ __forceinline__ void multiply(const Frags& f) {
-    // consecutive instructions write different accumulators: none waits for the one before it
+  // The products of one step, in two parts: what follows the first part is issued behind instructions that are already
+  // under way.  Consecutive instructions write different accumulators: none waits for the one before it.
+  template <bool FIRST> __device__ __forceinline__ void multiply(const Frags& f) {
     if constexpr (PL == 2) {  // small terms first
-      each_pair([&](int i, int j) { mfma<K>(acc[i][j], f.b[1][j], f.a[0][i], 0); });
-      each_pair([&](int i, int j) { mfma<K>(acc[i][j], f.b[0][j], f.a[1][i], 0); });
-    }
+      if constexpr (FIRST) {
+        each_pair([&](int i, int j) { mfma<K>(acc[i][j], f.b[1][j], f.a[0][i], 0); });
+      } else {
+        each_pair([&](int i, int j) { mfma<K>(acc[i][j], f.b[0][j], f.a[1][i], 0); });
+        each_pair([&](int i, int j) { mfma<K>(acc[i][j], f.b[0][j], f.a[0][i], 0); });
+      }
+    } else if constexpr (K == F32) {
 #pragma unroll
-    for (int e = 0; e < (K == F32 ? 4 : 1); ++e)
-      each_pair([&](int i, int j) { mfma<K>(acc[i][j], f.b[0][j], f.a[0][i], e); });
+      for (int e = FIRST ? 0 : 1; e < (FIRST ? 1 : 4); ++e)
+        each_pair([&](int i, int j) { mfma<K>(acc[i][j], f.b[0][j], f.a[0][i], e); });
+    } else {
+      each_pair([&](int i, int j) {
+        if ((i == 0) == FIRST) mfma<K>(acc[i][j], f.b[0][j], f.a[0][i], 0);
+      });
+    }
   }
   // One tile's products.  The fragments of step ks + 1 are on their way while the matrix cores work on step ks, across
   // the tile's end too: turn() - called once every read of this tile has arrived - makes the next tile's LDS ready and
@@ -369,6 +379,9 @@ struct Block {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       if constexpr (PIPE) {
+        // the wait for this step's fragments stands before the next one's are asked for, so it is for them alone
+        multiply<true>(f[ks & 1]);
+        __builtin_amdgcn_sched_barrier(0);
         if (ks + 1 < KS) {
           read(f[(ks + 1) & 1], cur, cur + TA::BYTES, ks + 1, lane, wm, wn);
         } else {
@@ -377,7 +390,7 @@ struct Block {
           if (next) read(f[0], next, next + TA::BYTES, 0, lane, wm, wn);
         }
         __builtin_amdgcn_sched_barrier(0);
-        multiply(f[ks & 1]);
+        multiply<false>(f[ks & 1]);
         __builtin_amdgcn_sched_barrier(0);
       } else {
         read(f[0], cur, cur + TA::BYTES, ks, lane, wm, wn);
@@ -385,7 +398,8 @@ struct Block {
           wait_lds();
           turn();
         }
-        multiply(f[0]);
+        multiply<true>(f[0]);
+        multiply<false>(f[0]);
       }
     }
   }
@@ -566,26 +580,8 @@ struct Block {
     return (wave % WN) * FN * 32 + (lane % (8 * FN)) * 4;
   }
 
-  // f(m, n, v): 4 consecutive columns n .. n + 3 of row m, as the accumulators hold them: the 32 lanes of a half wave
-  // have consecutive m
-  template <typename F> __device__ __forceinline__ void each(int m0, int n0, F f) const {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = wave / WN, wn = wave % WN;
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          f32x4 v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
-          f(m0 + (wm * FM + i) * 32 + (lane & 31), n0 + (wn * FN + j) * 32 + 8 * q + 4 * (lane >> 5), v);
-        }
-  }
-
-  // The same with neighbouring lanes at neighbouring columns, 32 FN of a row, through the wave's own part of LDS (which
-  // run() has left): stores cover whole lines.  pre(m, n) loads what f(m, n, v, x) adds, for all rows of a pass before
+  // f(m, n, v, x): 4 consecutive columns n .. n + 3 of row m, neighbouring lanes at neighbouring columns, 32 FN of a row,
+  // through the wave's own part of LDS (which run() has left): stores cover whole lines.  pre(m, n) loads what f(m, n, v, x) adds, for all rows of a pass before
   // any of them is stored.
   template <typename P, typename F> __device__ __forceinline__ void each_row(char* lds, int m0, int n0, P pre, F f) const {
     constexpr int LD = 32 * FN + 4;  // floats; the rows one pass writes fall on different banks
@@ -618,6 +614,38 @@ struct Block {
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
+  }
+
+  // The same for the transposed result: f(n, m, v, x) with 4 consecutive rows m .. m + 3 of column n.
+  template <typename P, typename F> __device__ __forceinline__ void each_column(char* lds, int m0, int n0, P pre, F f) const {
+    constexpr int W = FM < 2 ? FM : 2;  // 32 W rows at a time
+    constexpr int LD = 32 * W + 4, PERROW = 8 * W, ROWS = 64 / PERROW, N = 32 / ROWS;
+    static_assert(WM * WN * 32 * LD * 4 <= LDS_BYTES && FM % W == 0, "the epilogue's rows fit");
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave / WN, wn = wave % WN;
+    float* buf = reinterpret_cast<float*>(lds) + wave * 32 * LD;
+    const int col = (lane % PERROW) * 4;
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; i += W) {
+        const int m = m0 + (wm * FM + i) * 32 + col, nj = n0 + (wn * FN + j) * 32 + lane / PERROW;
+        decltype(pre(0, 0)) x[N];
+#pragma unroll
+        for (int r = 0; r < N; ++r) x[r] = pre(nj + r * ROWS, m);
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            buf[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * LD + w * 32 + (lane & 31)] = acc[i + w][j][e];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < N; ++r)
+          f(nj + r * ROWS, m, *reinterpret_cast<const f32x4*>(buf + (r * ROWS + lane / PERROW) * LD + col), x[r]);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
   }
 };
 

@@ -198,49 +198,12 @@ struct Prod {
   float keep, step;  // STEP: w = keep w - step value
 };
 
-// what the result at (m, n .. n + 3) is added to (STEP)
-template <Kind K, Epi E> __device__ __forceinline__ f32x4 before_result(const Prod& p, int g, int m, int n) {
-  f32x4 w = {0.f, 0.f, 0.f, 0.f};
-  if constexpr (E == STEP) {
-    const float* dst = reinterpret_cast<const float*>(p.dst) + g * p.dst_stride;
-    if (!p.transposed) return load4<F32>(dst + m * p.dst_ld + n, p.n - n);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < p.n) w[i] = dst[(n + i) * p.dst_ld + m];
-  }
-  return w;
-}
-template <Kind K, Epi E> __device__ __forceinline__ void write_result(const Prod& p, int g, int m, int n, f32x4 v, f32x4 w) {
-  typedef typename Elem<K>::T T;
-  T* dst = reinterpret_cast<T*>(p.dst) + g * p.dst_stride;
-  if constexpr (E == STEP)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = p.keep * w[i] - p.step * v[i];
-  if (!p.transposed) {
-    store4<K>(dst + m * p.dst_ld + n, v, p.n - n);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < p.n) dst[(n + i) * p.dst_ld + m] = from_f32<K>(v[i]);
-  }
-}
-
 // tile i of those at and below the diagonal: (0,0) (1,0) (1,1) (2,0) ...
 __device__ __forceinline__ void lower_tile(int i, int& tm, int& tn) {
   tm = (int)((sqrtf(8.f * i + 1.f) - 1.f) * 0.5f);
   while (tm * (tm + 1) / 2 > i) --tm;
   while ((tm + 1) * (tm + 2) / 2 <= i) ++tm;
   tn = i - tm * (tm + 1) / 2;
-}
-
-// planes at (n .. n + 3, m): the mirror image of a tile below the diagonal
-__device__ __forceinline__ void store_planes_mirrored(const Planes& p, int g, int m, int n, int N, f32x4 v) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (n + i < N) {
-      uint16_t* at = p.p + plane_at(p, g, n + i, m);
-      split(v[i], at[0], at[32]);
-    }
 }
 
 // GRAM: both operands are X and the sum runs over its rows
@@ -275,49 +238,50 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Prod p) {
   B blk;
   blk.clear();
   blk.run(lds, oa, ob, m0, n0, first * B::BK, min(rend, last * B::BK), true);
-  auto before = [&](int m, int n) {
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    if (m < p.m && n < p.n) {
-      if constexpr (E == POLY) x = load_planes(p.add, g, m, n);  // zeros behind the last column
-      else if constexpr (E == STEP) x = before_result<K, E>(p, g, m, n);
-    }
-    return x;
-  };
-  auto value = [&](int m, int n, f32x4 v, f32x4 x) {
-    if constexpr (E == POLY) {
+  if constexpr (E == PARTIAL) {
+    float* out = p.partial + ((int64_t)sp * p.models + g) * p.m * p.n;
+    blk.each_row(lds, m0, n0, [](int, int) { return 0; }, [&](int m, int n, f32x4 v, int) {
+      if (m < p.m && n < p.n) store4<F32>(out + (int64_t)m * p.n + n, v, p.n - n);
+    });
+  } else if constexpr (E == PLANES || E == POLY) {
+    // the same for a tile and its mirror image; zeros behind the last column
+    auto before = [&](int m, int n) {
+      return E == POLY && m < p.m && n < p.n ? load_planes(p.add, g, m, n) : f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    auto result = [&](int m, int n, f32x4 v, f32x4 x) {
+      if (m >= p.m || n >= p.out.ld / 2) return;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        v[i] = p.cc * v[i] + p.cb * x[i];
-        if (n + i == m) v[i] += p.ca;
-      }
-    } else if constexpr (E != PARTIAL) {
-      v *= p.alpha;
-    }
-    if constexpr (E == PLANES || E == POLY)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
+        if (E == POLY) v[i] = p.cc * v[i] + (p.cb * x[i] + (n + i == m ? p.ca : 0.f));
+        else v[i] *= p.alpha;
         if (n + i >= p.n) v[i] = 0.f;
-    return v;
-  };
-  auto result = [&](int m, int n, f32x4 v, f32x4 x) {
-    // planes: zeros behind the last column too
-    if (m >= p.m || n >= (E == PLANES || E == POLY ? p.out.ld / 2 : p.n)) return;
-    v = value(m, n, v, x);
-    if constexpr (E == PARTIAL)
-      store4<F32>(p.partial + ((int64_t)sp * p.models + g) * p.m * p.n + (int64_t)m * p.n + n, v, p.n - n);
-    else if constexpr (E == PLANES || E == POLY) store_planes(p.out, g, m, n, v);
-    else write_result<K, E>(p, g, m, n, v, x);
-  };
-  if ((E == OUT || E == STEP) && p.transposed)
-    blk.each(m0, n0, [&](int m, int n, f32x4 v) { result(m, n, v, before(m, n)); });
-  else
+      }
+      store_planes(p.out, g, m, n, v);
+    };
     blk.each_row(lds, m0, n0, before, result);
-  if constexpr (E == PLANES || E == POLY)
-    if (p.symmetric && tm != tn)
-      blk.each(m0, n0, [&](int m, int n, f32x4 v) {
-        if (m < p.out.ld / 2 && n < p.n)  // its zeros behind the last column too
-          store_planes_mirrored(p.out, g, m, n, p.n, m < p.m ? value(m, n, v, before(m, n)) : f32x4{0.f, 0.f, 0.f, 0.f});
-      });
+    if (p.symmetric && tm != tn) {
+      __syncthreads();
+      blk.each_column(lds, m0, n0, before, result);
+    }
+  } else {
+    typedef typename Elem<K>::T T;
+    T* dst = reinterpret_cast<T*>(p.dst) + g * p.dst_stride;
+    const int rows = p.transposed ? p.n : p.m, cols = p.transposed ? p.m : p.n;
+    auto before = [&](int r, int c) {
+      if constexpr (E == STEP) return r < rows && c < cols ? load4<K>(dst + r * p.dst_ld + c, cols - c) : f32x4{0.f, 0.f, 0.f, 0.f};
+      else return 0;
+    };
+    auto result = [&](int r, int c, f32x4 v, auto w) {
+      if (r >= rows || c >= cols) return;
+      v *= p.alpha;
+      if constexpr (E == STEP)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = p.keep * w[i] - p.step * v[i];
+      store4<K>(dst + r * p.dst_ld + c, v, cols - c);
+    };
+    if (p.transposed) blk.each_column(lds, m0, n0, before, result);
+    else blk.each_row(lds, m0, n0, before, result);
+  }
 }
 
 // the Gram matrix from its partial sums, added in order: 64 x 64 tiles at and below the diagonal, the others mirrored
@@ -1047,7 +1011,7 @@ size_t align16(size_t v) { return (v + 15) & ~(size_t)15; }
 
 // Multiply-adds per cycle and CU of split products (measured on large ones)
 // The last: one workgroup per CU with twice the tiles in flight, for products too small for two.
-constexpr TileShape SHAPES[4] = {{256, 256, 1, 300.f}, {128, 128, 2, 250.f}, {64, 64, 2, 130.f}, {128, 128, 1, 220.f}};
+constexpr TileShape SHAPES[4] = {{256, 256, 1, 300.f}, {128, 128, 2, 250.f}, {64, 64, 2, 140.f}, {128, 128, 1, 200.f}};
 
 // LDS of small_kernel, 0 where the matrix does not fit
 size_t small_bytes(int L, int k) {
