@@ -1023,6 +1023,7 @@ size_t small_bytes(int L, int k) {
 
 struct Space {
   int k, L, ld, phases, chunks;
+  int planned;  // the number of models that sums are split for
   size_t small;
   int narrow, rows_per;  // KP of the narrow form (0: not used), rows l of a chunk
   Choice gram;
@@ -1058,6 +1059,7 @@ bool space(const mplc_muon_t& t, Space& s) {
   if (t.n_models < 0 || t.n_models > 65535 || t.rows < 1 || t.cols < 1 || t.dtype < 0 || t.dtype > 2) return false;
   if (t.steps < 1 || t.steps > 16) return false;
   s = Space{};
+  s.planned = t.invariant ? 16 : t.n_models;
   s.k = t.rows < t.cols ? t.rows : t.cols;
   s.L = t.rows < t.cols ? t.cols : t.rows;
   s.ld = 2 * ((s.k + 31) & ~31);
@@ -1072,7 +1074,7 @@ bool space(const mplc_muon_t& t, Space& s) {
     s.phases = (t.steps + 2) / 3;
     const int64_t tr = 16384 / s.narrow, pieces = ceil_div(s.L, tr);
     // about one workgroup per CU and round, whole pieces, at least two per workgroup where there are many
-    int64_t per = ceil_div(pieces * t.n_models, 512);
+    int64_t per = ceil_div(pieces * s.planned, 512);
     if (per > pieces) per = pieces;
     s.rows_per = (int)((per < 1 ? 1 : per) * tr);
     s.chunks = (int)ceil_div(s.L, s.rows_per);
@@ -1086,9 +1088,9 @@ bool space(const mplc_muon_t& t, Space& s) {
   s.n_x = s.phases > 1 ? 2 : 1;
   const int64_t groups = (int64_t)t.rows * ceil_div(t.cols, 4);
   if (groups > (int64_t)1 << 30) return false;
-  const int64_t most = t.n_models >= 16 ? 64 : NORM_CHUNKS;
+  const int64_t most = s.planned >= 16 ? 64 : NORM_CHUNKS;
   s.chunks = (int)(ceil_div(groups, 1024) < most ? ceil_div(groups, 1024) : most);
-  s.gram = shape_for(t.n_models, s.k, s.k, s.L, true, true);
+  s.gram = shape_for(s.planned, s.k, s.k, s.L, true, true);
   const size_t G = (size_t)t.n_models;
   s.sums = align16(G * s.chunks * sizeof(double));
   s.x = align16(G * s.L * s.ld * 2);
@@ -1279,8 +1281,8 @@ template <Kind K, Epi LAST> int run(const mplc_muon_t& t, const Space& sp, const
 
   Prod base = {};
   base.models = t.n_models;
-  const Choice small = shape_for(t.n_models, sp.k, sp.k, sp.k, true, false);
-  const Choice apply = shape_for(t.n_models, sp.L, sp.k, sp.k, false, false);
+  const Choice small = shape_for(sp.planned, sp.k, sp.k, sp.k, true, false);
+  const Choice apply = shape_for(sp.planned, sp.L, sp.k, sp.k, false, false);
   const double a = t.a, b = t.b, c = t.c;
   double r = 1.;
   int done = 0, x = 0;

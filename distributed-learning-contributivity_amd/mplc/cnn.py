@@ -455,6 +455,10 @@ class TrainBatch:
             # partner.model_weights of the aggregating variants: one snapshot row per (coalition, member)
             self.snap = torch.zeros((len(seq_recs) // SEQ_REC, S), **f32)
             self.snap_first_t = torch.tensor(snap_first, **i32)
+        # the server's optimizer (eng.server_optimizer): one momentum row per coalition
+        self.server_m = None
+        if getattr(eng, "server_optimizer", None) is not None:
+            self.server_m = resume["server_m"] if resume is not None else torch.zeros((C, S), **f32)
         self.resume_opt = resume["opt"] if resume is not None else None  # alloc() takes these rows over
         self.model.alloc(self)
         self.resume_opt = None
@@ -528,7 +532,7 @@ class TrainBatch:
         import torch
         eng = self.eng
         ok = (getattr(self.model, "FUSE_AVG", False) and not self.seq_mode and eng.bcast_skip and not self.record
-              and getattr(eng, "fuse_avg", True))
+              and getattr(eng, "fuse_avg", True) and getattr(eng, "server_optimizer", None) is None)
         out, first, rep_w, scale, glob_row = [], [], np.zeros(self.R), [], []
         rep = np.zeros(self.R, dtype=np.int32)
         sizes = eng.partner_sizes
@@ -588,7 +592,9 @@ class TrainBatch:
         aggregate_now = (not self.seq_mode or self.approach == "seqavg"
                          or (self.approach == "seq-with-final-agg" and epoch_end))
         for (r0, c0, nc, first, w, sc, full_bcast, fused) in self.run_args:
-            if aggregate_now:
+            if self.server_m is not None:
+                self._server_step(r0, c0, nc, first, w, sc)
+            elif aggregate_now:
                 x = self.params[r0:] if not self.seq_mode else self.snap[self.snap_row(c0):]
                 skip = None if (self.seq_mode or full_bcast or not self.eng.bcast_skip) else \
                     getattr(self.model, "BCAST_SKIP", None)
@@ -613,6 +619,20 @@ class TrainBatch:
             else:  # sequential without averaging: the coalition model as it stands
                 self._rows_copy(self.glob[c0:c0 + nc], self.params, list(range(r0, r0 + nc)))
 
+    def _server_step(self, r0, c0, nc, first, w, sc):
+        """End of a FedAvg round with a server optimizer: the average, the optimizer's step on the coalition rows, the
+        rows back to their replicas."""
+        S, NP = self.model.STRIDE, self.model.NPARAM
+        rows = self.glob[c0:c0 + nc]
+        before = rows.clone()
+        _native.check(self.lib.mplc_fedavg_aggregate(_native.ptr(self.params[r0:]), S, _native.ptr(first), _native.ptr(w),
+                                                     _native.ptr(sc), nc, NP, _native.ptr(rows), S, 0, self.stream),
+                      "mplc_fedavg_aggregate")
+        self.eng.server_optimizer.apply(rows, before, self.server_m[c0:c0 + nc], self.model.KERAS_LAYERS)
+        last = self.coal_first[c0 + nc]
+        self._rows_copy(self.params[r0:last], self.glob, [ci for ci in range(c0, c0 + nc)
+                                                          for _ in range(self.coal_first[ci], self.coal_first[ci + 1])])
+
     def snap_row(self, ci):
         return sum(len(self.coalitions[c]) for c in range(ci) if not self.coal_is_single[c])
 
@@ -630,7 +650,7 @@ class TrainBatch:
 
     def release(self):
         """Drop every device buffer of this batch (compaction: the live rows were gathered first)."""
-        self.params = self.glob = None
+        self.params = self.glob = self.server_m = None
         self.model.free(self)
         self.ws = None
         self.t = None
@@ -866,6 +886,8 @@ class CnnBatchTrainer:
                   "params": st.params.index_select(0, reps),
                   "opt": {k: v.index_select(0, reps) for k, v in st.model.opt_state(st).items()},
                   "round_len": st.round_len, "fed_steps": st.fed_steps, "total_steps": st.total_steps}
+        if st.server_m is not None:
+            resume["server_m"] = st.server_m.index_select(0, torch.tensor(live, dtype=torch.int64, device=dev))
         coalitions, epochs = [st.coalitions[ci] for ci in live], st.epochs
         st.release()
         return TrainBatch(self.eng, coalitions, epochs, self.lib, resume=resume)

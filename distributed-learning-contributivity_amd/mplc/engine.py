@@ -40,7 +40,7 @@ class CoalitionEngine:
     def __init__(self, *, x_train, y_train, x_val, y_val, x_test, y_test, partner_rows, batch_sizes,
                  epoch_count, minibatch_count, aggregation="data-volume", is_early_stopping=True, seed=0,
                  model="mnist_cnn", device=None, memory_budget_bytes=None, eval_budget_bytes=8 << 30,
-                 approach="fedavg"):
+                 approach="fedavg", server_optimizer=None):
         import torch
         if not torch.cuda.is_available():
             raise RuntimeError("MI355X (HIP) device required: the MPLC engine has no CPU fallback")
@@ -48,6 +48,13 @@ class CoalitionEngine:
         if approach not in ("fedavg", "seq-pure", "seq-with-final-agg", "seqavg"):
             raise NotImplementedError(f"multi-partner learning approach '{approach}' has no batched MI355X path")
         self.approach = approach
+        # optimizer of the server after a FedAvg round's average (mplc.muon.ServerMuon): None takes the average
+        self.server_optimizer = None
+        if server_optimizer is not None:
+            from .muon import ServerMuon
+            if approach != "fedavg":
+                raise NotImplementedError(f"a server optimizer needs the FedAvg approach, not '{approach}'")
+            self.server_optimizer = ServerMuon(server_optimizer)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.model = model
         self.seed = int(seed)
@@ -135,6 +142,11 @@ class CoalitionEngine:
                   is_early_stopping=getattr(scenario, "is_early_stopping", True),
                   seed=getattr(scenario, "engine_seed", int(os.environ.get("MPLC_ENGINE_SEED", "0"))), model=model)
         approach = getattr(getattr(scenario, "multi_partner_learning_approach", None), "engine_approach", "fedavg")
+        server = getattr(scenario, "server_optimizer", None)
+        if server is not None:
+            if target is not cls:
+                raise NotImplementedError(f"a server optimizer is not available for the {name} model")
+            kw["server_optimizer"] = server
         if target is cls:
             kw["approach"] = approach
         elif approach != "fedavg":
@@ -156,7 +168,8 @@ class CoalitionEngine:
         for i in order:
             c = coalitions[i]
             bmax = max(self.batch_sizes[p] for p in c)
-            need = len(c) * self.replica_bytes(bmax) + self.model_impl.STRIDE * 4
+            # a coalition's row; with a server optimizer also its momentum, its start of the round and the difference
+            need = len(c) * self.replica_bytes(bmax) + self.model_impl.STRIDE * (4 if self.server_optimizer is None else 16)
             if cur and (cur_bytes + need > self.memory_budget_bytes or len(cur) >= 65535):
                 batches.append(cur)
                 cur, cur_bytes = [], 0

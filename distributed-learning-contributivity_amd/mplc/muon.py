@@ -21,9 +21,8 @@ STEPS = 5
 class MuonT(ctypes.Structure):
     _fields_ = [("n_models", ctypes.c_int32), ("rows", ctypes.c_int32), ("cols", ctypes.c_int32),
                 ("dtype", ctypes.c_int32), ("steps", ctypes.c_int32), ("nesterov", ctypes.c_int32),
-                ("a", ctypes.c_float), ("b", ctypes.c_float), ("c", ctypes.c_float), ("lr", ctypes.c_float),
+                ("invariant", ctypes.c_int32), ("a", ctypes.c_float), ("b", ctypes.c_float), ("c", ctypes.c_float), ("lr", ctypes.c_float),
                 ("beta", ctypes.c_float), ("weight_decay", ctypes.c_float), ("scale", ctypes.c_float),
-                ("pad0", ctypes.c_float),
                 ("g", ctypes.c_void_p), ("g_stride", ctypes.c_int64), ("g_ld", ctypes.c_int64),
                 ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64), ("out_ld", ctypes.c_int64),
                 ("m", ctypes.c_void_p), ("m_stride", ctypes.c_int64), ("m_ld", ctypes.c_int64),
@@ -72,7 +71,7 @@ def singular_range(steps, coefficients):
     return most
 
 
-def _setup(g, name, steps, coefficients):
+def _setup(g, name, steps, coefficients, invariant):
     if not isinstance(g, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     if not g.is_cuda:
@@ -98,19 +97,20 @@ def _setup(g, name, steps, coefficients):
     t = MuonT()
     t.n_models, t.rows, t.cols, t.dtype, t.steps = G, m, n, DTYPES[str(g.dtype)], int(steps)
     t.a, t.b, t.c = coefficients
+    t.invariant = int(bool(invariant))
     _place(t, "g", g3)
     return t, g3
 
 
-def _key(kind, steps, coefficients, tensors):
+def _key(kind, steps, coefficients, invariant, tensors):
     try:
-        return (kind, steps, tuple(coefficients)) + tuple(_sig(t) for t in tensors)
+        return (kind, steps, tuple(coefficients), bool(invariant)) + tuple(_sig(t) for t in tensors)
     except (AttributeError, TypeError):  # not tensors, not numbers: the checks say so
         return None
 
 
-def _plan_orthogonalize(key, out, g, steps, coefficients):
-    t, g3 = _setup(g, "g", steps, coefficients)
+def _plan_orthogonalize(key, out, g, steps, coefficients, invariant):
+    t, g3 = _setup(g, "g", steps, coefficients, invariant)
     if out is None:
         out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
     if not isinstance(out, torch.Tensor):
@@ -124,15 +124,16 @@ def _plan_orthogonalize(key, out, g, steps, coefficients):
                                 (_three(out), g3)))
 
 
-def orthogonalize(g, steps=STEPS, coefficients=COEFFICIENTS, out=None):
+def orthogonalize(g, steps=STEPS, coefficients=COEFFICIENTS, out=None, batch_invariant=False):
     """Each matrix of g ([G, m, n] or [m, n]) divided by its Frobenius norm, then `steps` times
     X <- a X + b (X X^T) X + c (X X^T)^2 X.  A zero matrix stays zero; one with an infinity or a NaN becomes NaN.
     Sums and intermediate matrices keep fp32's accuracy whatever g's type; the result is rounded to it once.
-    out may be g itself."""
-    key = _key(2, steps, coefficients, (g, out))
+    out may be g itself.  batch_invariant: a matrix's result has the same bits whichever matrices share the call (its
+    sums are then split in one way, not in the best one for the batch)."""
+    key = _key(2, steps, coefficients, batch_invariant, (g, out))
     plan = _PLANS.get(key) if key is not None else None
     if plan is None:
-        plan = _plan_orthogonalize(key, out, g, steps, coefficients)
+        plan = _plan_orthogonalize(key, out, g, steps, coefficients, batch_invariant)
     if out is None:
         out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
     if plan.models:
@@ -145,8 +146,8 @@ def update_scale(rows, cols):
     return math.sqrt(max(1.0, cols / rows))
 
 
-def _plan_step(key, w, grad, momentum, steps, coefficients):
-    t, g3 = _setup(grad, "grad", steps, coefficients)
+def _plan_step(key, w, grad, momentum, steps, coefficients, invariant):
+    t, g3 = _setup(grad, "grad", steps, coefficients, invariant)
     for name, field, v in (("w", "w", w), ("momentum", "m", momentum)):
         if not isinstance(v, torch.Tensor):
             raise TypeError(f"{name} must be a tensor")
@@ -160,17 +161,18 @@ def _plan_step(key, w, grad, momentum, steps, coefficients):
 
 
 def muon_step(w, grad, momentum, lr, beta=0.95, nesterov=True, weight_decay=0.0, steps=STEPS,
-              coefficients=COEFFICIENTS, scale=None):
+              coefficients=COEFFICIENTS, scale=None, batch_invariant=False):
     """One Muon step on each matrix w [G, in, out] (or [in, out]), in place:
 
         momentum <- beta momentum + grad;   u = grad + beta momentum (nesterov) or momentum
         w <- (1 - lr weight_decay) w - lr scale orthogonalize(u)
 
-    w and momentum are float32, grad any supported type; scale None: update_scale(in, out).  Returns w."""
-    key = _key(3, steps, coefficients, (w, grad, momentum))
+    w and momentum are float32, grad any supported type; scale None: update_scale(in, out).  batch_invariant: as for
+    orthogonalize.  Returns w."""
+    key = _key(3, steps, coefficients, batch_invariant, (w, grad, momentum))
     plan = _PLANS.get(key) if key is not None else None
     if plan is None:
-        plan = _plan_step(key, w, grad, momentum, steps, coefficients)
+        plan = _plan_step(key, w, grad, momentum, steps, coefficients, batch_invariant)
     rows, cols = grad.shape[-2:]
     scale = update_scale(rows, cols) if scale is None else float(scale)
     lr, beta, weight_decay = float(lr), float(beta), float(weight_decay)
@@ -180,3 +182,54 @@ def muon_step(w, grad, momentum, lr, beta=0.95, nesterov=True, weight_decay=0.0,
         plan.run((w, momentum, grad), ("w", "momentum", "grad"), values=(
             ("lr", lr), ("beta", beta), ("weight_decay", weight_decay), ("scale", scale), ("nesterov", int(bool(nesterov)))))
     return w
+
+
+class ServerMuon:
+    """The server's optimizer of federated averaging: after a round's average, the matrices of a coalition's model move
+    from where they stood before the round by a Muon step along (before - average) instead of taking the average; the
+    other layers (biases) take it.  Convolution kernels [kh][kw][cin][cout] are [kh * kw * cin][cout] matrices.
+
+    spec: {"name": "muon", "lr": .., and optionally "beta", "nesterov", "weight_decay", "steps"}, or "muon" for the defaults.
+    Every coalition's result is independent of the coalitions it shares a batch with."""
+    DEFAULTS = {"lr": 0.02, "beta": 0.9, "nesterov": True, "weight_decay": 0.0, "steps": STEPS}
+    GROUP = 64  # coalitions per call: bounds the workspace
+
+    def __init__(self, spec):
+        if isinstance(spec, str):
+            spec = {"name": spec}
+        spec = dict(spec)
+        name = spec.pop("name", None)
+        if name != "muon":
+            raise ValueError(f"server optimizer '{name}' is not a valid one: 'muon'")
+        unknown = sorted(set(spec) - set(self.DEFAULTS))
+        if unknown:
+            raise ValueError(f"server optimizer 'muon' has no parameter {', '.join(unknown)}")
+        self.params = {**self.DEFAULTS, **spec}
+        p = self.params
+        numbers = [float(p[k]) for k in ("lr", "beta", "weight_decay")]
+        if not all(math.isfinite(v) for v in numbers) or not 0.0 <= numbers[1] < 1.0 or numbers[0] <= 0.0:
+            raise ValueError(f"server optimizer 'muon': lr must be positive and beta in [0, 1): {p}")
+        if not 1 <= int(p["steps"]) <= 16:
+            raise ValueError(f"server optimizer 'muon': steps must be 1 to 16, not {p['steps']}")
+
+    def describe(self):
+        """A plain value that tells runs with different settings apart (the fingerprint of persisted values)."""
+        return {"name": "muon", **self.params}
+
+    @staticmethod
+    def matrices(layers):
+        """(offset, rows, cols) of the matrices among a model row's layers (offset, shape)."""
+        return [(off, math.prod(shape[:-1]), shape[-1]) for off, shape in layers if len(shape) > 1]
+
+    def apply(self, glob, before, momentum, layers):
+        """glob, before, momentum [C, stride]: glob holds the round's averages and receives the new models; before, the
+        models at the round's start, is used up."""
+        for c in range(0, glob.shape[0], self.GROUP):
+            g, b, m = glob[c:c + self.GROUP], before[c:c + self.GROUP], momentum[c:c + self.GROUP]
+            grad = b - g
+            for off, rows, cols in self.matrices(layers):
+                w, d, mm = (t[:, off:off + rows * cols].view(t.shape[0], rows, cols) for t in (b, grad, m))
+                muon_step(w, d, mm, lr=self.params["lr"], beta=self.params["beta"], nesterov=self.params["nesterov"],
+                          weight_decay=self.params["weight_decay"], steps=int(self.params["steps"]),
+                          batch_invariant=True)
+                g[:, off:off + rows * cols].copy_(b[:, off:off + rows * cols])

@@ -27,7 +27,7 @@ logger = logging.getLogger("mplc")
 PARAMS_KNOWN = ["dataset", "dataset_name", "dataset_proportion", "methods", "multi_partner_learning_approach",
                 "aggregation", "partners_count", "amounts_per_partner", "corrupted_datasets", "samples_split_option",
                 "gradient_updates_per_pass_count", "epoch_count", "minibatch_count", "is_early_stopping",
-                "init_model_from", "is_quick_demo", "engine_seed", "coalition_values_file"]
+                "init_model_from", "is_quick_demo", "engine_seed", "coalition_values_file", "server_optimizer"]
 
 
 
@@ -51,7 +51,7 @@ class Scenario:
                  minibatch_count=constants.DEFAULT_BATCH_COUNT, epoch_count=constants.DEFAULT_EPOCH_COUNT,
                  is_early_stopping=True, methods=None, is_quick_demo=False, experiment_path=Path("./experiments"),
                  scenario_id=1, repeats_count=1, is_dry_run=True, engine_seed=0, coalition_values_file=None,
-                 **kwargs):
+                 server_optimizer=None, **kwargs):
         unknown = [k for k in kwargs if k not in PARAMS_KNOWN]
         if unknown:
             raise Exception(f"Unrecognised parameters {unknown}, check your configuration")
@@ -97,6 +97,13 @@ class Scenario:
             raise ValueError(f"aggregation approach '{aggregation_weighting}' is not a valid approach. ")
         self.aggregation_weighting = aggregation_weighting
         self.aggregation = aggregation_weighting
+        # not of the reference: the server's optimizer after a FedAvg round's average (mplc.muon.ServerMuon)
+        if server_optimizer is not None:
+            from .muon import ServerMuon
+            ServerMuon(server_optimizer)  # its checks
+            if multi_partner_learning_approach != "fedavg":
+                raise NotImplementedError("a server optimizer needs the 'fedavg' approach")
+        self.server_optimizer = server_optimizer
         self.epoch_count = epoch_count
         assert self.epoch_count > 0, "Error: in the provided config file, epoch_count should be > 0"
         self.minibatch_count = minibatch_count
@@ -232,8 +239,12 @@ class Scenario:
         content = zlib.crc32(np.ascontiguousarray(ds.y_train).tobytes())
         content = zlib.crc32(np.ascontiguousarray(np.asarray(ds.x_train)[::97]).tobytes(), content)
         content = zlib.crc32(np.ascontiguousarray(np.asarray(ds.x_test)[::97]).tobytes(), content)
+        server = {}
+        if self.server_optimizer is not None:  # only where there is one: tables saved without it stay valid
+            from .muon import ServerMuon
+            server["server_optimizer"] = ServerMuon(self.server_optimizer).describe()
         return json.dumps({
-            "content_crc32": int(content),
+            **server, "content_crc32": int(content),
             "dataset": self.dataset.name, "synthetic": bool(getattr(self.dataset, "synthetic", False)),
             "n_train": int(len(self.dataset.x_train)), "n_val": int(len(self.dataset.x_val)),
             "n_test": int(len(self.dataset.x_test)),
@@ -296,6 +307,8 @@ class Scenario:
         }
         if getattr(self.dataset, "synthetic", False):  # not a reference column: only present when true
             base["synthetic_data"] = True
+        if self.server_optimizer is not None:
+            base["server_optimizer"] = str(self.server_optimizer)
         rows = []
         if not self.contributivity_list:
             rows.append(dict(base))

@@ -94,9 +94,9 @@ int mplc_dense_backward(const mplc_dense_t* t, void* stream);
 typedef struct {
   int32_t n_models, rows, cols, dtype;
   int32_t steps, nesterov;
+  int32_t invariant;  /* != 0: a model's result does not depend on n_models (sums are split as for 16 models) */
   float a, b, c;
   float lr, beta, weight_decay, scale;
-  float pad0;
   const void* g;
   int64_t g_stride, g_ld;
   void* out; /* mplc_orthogonalize                                     */
@@ -109,7 +109,7 @@ typedef struct {
   size_t workspace_bytes;
 } mplc_muon_t;
 
-/* Bytes of workspace of either call; only sizes, dtype and steps are read. */
+/* Bytes of workspace of either call; only sizes, dtype, steps and invariant are read. */
 size_t mplc_muon_workspace_bytes(const mplc_muon_t* t);
 int mplc_orthogonalize(const mplc_muon_t* t, void* stream);
 int mplc_muon_step(const mplc_muon_t* t, void* stream);

@@ -225,3 +225,18 @@ def test_refusals():
             f()
     none = torch.empty(0, 3, 4, device="cuda")
     assert muon.orthogonalize(none).shape == (0, 3, 4)
+
+
+@pytest.mark.parametrize("size", [(128, 10), (60, 40), (1500, 100), (100, 1500), (300, 200), (200, 600)])
+def test_batch_invariant_results(size):
+    """The same bits alone, in a small and in a large batch."""
+    g = rand((40,) + size, seed=5)
+    want = muon.orthogonalize(g, batch_invariant=True)
+    for n in (1, 7):
+        assert torch.equal(muon.orthogonalize(g[:n], batch_invariant=True), want[:n])
+    close(want[3], g[3])
+    w, m = rand((40,) + size, seed=6), rand((40,) + size, seed=7)
+    w1, m1 = w[:1].clone(), m[:1].clone()
+    muon.muon_step(w, g, m, lr=0.1, batch_invariant=True)
+    muon.muon_step(w1, g[:1], m1, lr=0.1, batch_invariant=True)
+    assert torch.equal(w1, w[:1]) and torch.equal(m1, m[:1])
