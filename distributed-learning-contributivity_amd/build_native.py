@@ -25,13 +25,12 @@ ARCH = "gfx950"
 # also lets the backend fuse across statements, and which product it picks can move with unrelated code: a refactor of
 # dense1_bwd_adam_kernel flipped Adam's fusion, profiles/r06_adam_contraction.txt); `#pragma clang fp contract(off)`
 # still marks the code whose every operation rounds on its own (Adam, RMSprop, FedAvg)
+# The packed fp32 instructions (v_pk_add_f32, v_pk_mul_f32, v_pk_fma_f32), which hipcc forms by itself from scalar code,
+# are kept out of every source: some of their forms have given wrong results now and then.  The scalar instructions in
+# their place give the same bits.
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-I", INCLUDE, "-I", CSRC,
-          "-Wno-unused-result", "-munsafe-fp-atomics", "-ffp-contract=on"]
-# The packed fp32 instructions (v_pk_add_f32, v_pk_mul_f32, v_pk_fma_f32), which hipcc forms by itself from scalar
-# code, are kept out: some of their forms have given wrong results now and then.
-NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-
-
+          "-Wno-unused-result", "-munsafe-fp-atomics", "-ffp-contract=on",
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 def _deps(src):
     hdrs = glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(INCLUDE, "*.h"))
     return [src] + hdrs
@@ -50,8 +49,7 @@ def _stale(target, deps):
 # software-pipelined conv k-loops out of the MFMA gaps.  cifar_cnn.hip likewise (its Winograd loops: 10-25 % fewer
 # VALU instructions; every VALU instruction costs an f32 MFMA stream 2.5-3.5 cycles); its two head
 # kernels live in cifar_head.hip with the default flags, which keeps their expf / logf / dot-product code as it was.
-# dense.hip, muon.hip: no packed fp32 arithmetic (see NO_PACKED).
-FILE_FLAGS = {"dense.hip": NO_PACKED, "muon.hip": NO_PACKED, "mnist_cnn.hip": ["-fno-slp-vectorize"], "mnist_wgrad.hip": ["-fno-slp-vectorize"],
+FILE_FLAGS = {"mnist_cnn.hip": ["-fno-slp-vectorize"], "mnist_wgrad.hip": ["-fno-slp-vectorize"],
               "cifar_cnn.hip": ["-fno-slp-vectorize"]}
 
 
