@@ -98,14 +98,14 @@ __device__ __forceinline__ float slope(int act, float z) {
   }
 }
 
-template <Kind K> __device__ __forceinline__ f32x4 residual_at(const Epilogue& e, int g, int m, int n, int N) {
+template <Kind K, bool WIDE> __device__ __forceinline__ f32x4 residual_at(const Epilogue& e, int g, int m, int n, int N) {
   typedef typename Elem<K>::T T;
-  return e.res ? load4<K>(reinterpret_cast<const T*>(e.res) + g * e.res_stride + m * e.res_ld + n, N - n)
+  return e.res ? load4<K, WIDE>(reinterpret_cast<const T*>(e.res) + g * e.res_stride + m * e.res_ld + n, N - n)
                : f32x4{0.f, 0.f, 0.f, 0.f};
 }
-template <Kind K> __device__ __forceinline__ f32x4 bias_at(const Epilogue& e, int g, int n, int N) {
+template <Kind K, bool WIDE> __device__ __forceinline__ f32x4 bias_at(const Epilogue& e, int g, int n, int N) {
   typedef typename Elem<K>::T T;
-  return e.bias ? load4<K>(reinterpret_cast<const T*>(e.bias) + g * e.bias_stride + n, N - n) : f32x4{0.f, 0.f, 0.f, 0.f};
+  return e.bias ? load4<K, WIDE>(reinterpret_cast<const T*>(e.bias) + g * e.bias_stride + n, N - n) : f32x4{0.f, 0.f, 0.f, 0.f};
 }
 // x w of 4 columns n .. of row m of model g -> z, y
 template <Kind K>
@@ -190,14 +190,17 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
       if (m < M && n < p.n) store4<F32>(out + (int64_t)m * p.n + n, v, p.n - n);
     });
   } else {
-    const int nl = n0 + B::lane_column();
-    const f32x4 bias = nl < p.n ? bias_at<K>(e, g, nl, p.n) : f32x4{0.f, 0.f, 0.f, 0.f};
-    blk.each_row(
-        lds, m0, n0,
-        [&](int m, int n) { return m < M && n < p.n ? residual_at<K>(e, g, m, n, p.n) : f32x4{0.f, 0.f, 0.f, 0.f}; },
-        [&](int m, int n, f32x4 v, f32x4 res) {
-          if (m < M && n < p.n) finish<K>(e, g, m, n, p.n, v, bias, res);
-        });
+    by_width(p.n, [&](auto wide) {
+      constexpr bool W = decltype(wide)::value;
+      const int nl = n0 + B::lane_column();
+      const f32x4 bias = nl < p.n ? bias_at<K, W>(e, g, nl, p.n) : f32x4{0.f, 0.f, 0.f, 0.f};
+      blk.each_row(
+          lds, m0, n0,
+          [&](int m, int n) { return m < M && n < p.n ? residual_at<K, W>(e, g, m, n, p.n) : f32x4{0.f, 0.f, 0.f, 0.f}; },
+          [&](int m, int n, f32x4 v, f32x4 res) {
+            if (m < M && n < p.n) finish<K>(e, g, m, n, p.n, v, bias, res);
+          });
+    });
   }
 }
 
@@ -210,17 +213,21 @@ template <Kind K> __global__ __launch_bounds__(256) void join_kernel(const Produ
   if (!p.count_is_r && p.segments == 1 && m >= count_of(p.counts, g, p.m)) return;
   const float* src = p.partial + (int64_t)g * p.m * p.n + (int64_t)m * p.n + n;
   const int64_t step = (int64_t)p.models * p.m * p.n;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < p.splits; s0 += 8) {  // 8 loads in flight
-    f32x4 x[8];
+  by_width(p.n, [&](auto wide) {
+    constexpr bool W = decltype(wide)::value;
+    const f32x4 bias = bias_at<K, W>(e, g, n, p.n), res = residual_at<K, W>(e, g, m, n, p.n);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < p.splits; s0 += 8) {  // 8 loads in flight; behind the last split the last again, not added
+      f32x4 x[8];
 #pragma unroll
-    for (int s = 0; s < 8; ++s)
-      if (s0 + s < p.splits) x[s] = load4<F32>(src + (s0 + s) * step, p.n - n);
+      for (int s = 0; s < 8; ++s) x[s] = load4<F32, W>(src + (s0 + s < p.splits ? s0 + s : p.splits - 1) * step, p.n - n);
 #pragma unroll
-    for (int s = 0; s < 8; ++s)
-      if (s0 + s < p.splits) v += x[s];
-  }
-  finish<K>(e, g, m, n, p.n, v, bias_at<K>(e, g, n, p.n), residual_at<K>(e, g, m, n, p.n));
+      for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += s0 + s < p.splits ? x[s][i] : 0.f;
+    }
+    finish<K>(e, g, m, n, p.n, v, bias, res);
+  });
 }
 
 constexpr int DZ_ROWS = 64;  // rows summed by one workgroup
@@ -243,25 +250,28 @@ __global__ __launch_bounds__(256) void dz_kernel(const void* dy_, int64_t dy_str
   T* dz = dz_ ? reinterpret_cast<T*>(dz_) + (int64_t)g * rows * dz_ld : nullptr;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
   if (c < n)
-    for (int r = r0 + wave * (64 / LANES) + lane / LANES; r < r1; r += 4 * STEP) {
-      f32x4 d[4], zz[4];
+    by_width(n, [&](auto wide) {
+      constexpr bool W = decltype(wide)::value;
+      for (int r = r0 + wave * (64 / LANES) + lane / LANES; r < r1; r += 4 * STEP) {
+        f32x4 d[4], zz[4];
+        // rows behind the last one are the last one again, and not counted
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (r + STEP * i < r1) {
-          d[i] = load4<K>(dy + (r + STEP * i) * dy_ld + c, n - c);
-          if (act != MPLC_ACT_NONE) zz[i] = load4<F32>(z + g * z_stride + (r + STEP * i) * z_ld + c, n - c);
-        }
+        for (int i = 0; i < 4; ++i) d[i] = load4<K, W>(dy + min(r + STEP * i, r1 - 1) * dy_ld + c, n - c);
+        if (act != MPLC_ACT_NONE)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (r + STEP * i < r1) {
-          if (act != MPLC_ACT_NONE) {
+          for (int i = 0; i < 4; ++i) zz[i] = load4<F32, W>(z + g * z_stride + min(r + STEP * i, r1 - 1) * z_ld + c, n - c);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) d[i][e] *= slope(act, zz[i][e]);
-            if (dz) store4<K>(dz + (int64_t)(r + STEP * i) * dz_ld + c, d[i], n - c);
+        for (int i = 0; i < 4; ++i)
+          if (r + STEP * i < r1) {
+            if (act != MPLC_ACT_NONE) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) d[i][e] *= slope(act, zz[i][e]);
+              if (dz) store4<K>(dz + (int64_t)(r + STEP * i) * dz_ld + c, d[i], n - c);
+            }
+            sum += d[i];
           }
-          sum += d[i];
-        }
-    }
+      }
+    });
   if (sums == nullptr && db_ == nullptr) return;
 #pragma unroll
   for (int d = 32; d >= LANES; d >>= 1)
@@ -338,14 +348,14 @@ bool plan(const mplc_dense_t& t, Form form, Plan& out) {
   const Choice c = choose(f32 ? SHAPES_F32 : SHAPES_16, 5, p.models, p.m, p.n, (int64_t)p.r * p.segments, units, true);
   out.cfg = c.tile;
   // A short sum is bound by its operands' latency and its result's stores: tiles of half the length leave LDS for three
-  // workgroups per CU (45 x 9216 x 128 from 51 rows: 103 us against 142).  Operands along r would fetch half lines.
-  if (form == DW && c.tile == 0 && p.nk <= 2) out.cfg = 5;
+  // workgroups per CU (45 x 9216 x 128 from 51 rows: 103 us against 142).
+  if ((c.tile == 0 || c.tile == 3) && p.nk <= 2) out.cfg = 5;
   p.splits = c.splits;
   p.per_split = c.per_split;
-  const int64_t tiles = c.tiles_m * c.tiles_n * p.models;
+  p.tiles_m = (int)(out.cfg == 5 ? ceil_div(p.m, 128) : c.tiles_m);
+  p.tiles_n = (int)(out.cfg == 5 ? ceil_div(p.n, 128) : c.tiles_n);
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.models;
   if (tiles * c.splits > (1 << 23)) return false;
-  p.tiles_m = (int)c.tiles_m;
-  p.tiles_n = (int)c.tiles_n;
   out.blocks = tiles * p.splits;
   out.partial_bytes = p.splits > 1 ? (size_t)p.splits * p.models * p.m * p.n * sizeof(float) : 0;
   out.p = p;
@@ -366,9 +376,7 @@ template <Kind K, bool AA, bool BA> hipError_t launch(Plan& pl, const Epilogue& 
   else if (pl.cfg == 3) {
     if constexpr (K != F32) product_kernel<K, AA, BA, 2, 4, 4, 2, 128, 2><<<grid, 512, 0, s>>>(pl.p, e);
   }
-  else if (pl.cfg == 5) {
-    if constexpr (AA && BA) product_kernel<K, AA, BA, 2, 2, 2, 2, 64, 3><<<grid, 256, 0, s>>>(pl.p, e);
-  }
+  else if (pl.cfg == 5) product_kernel<K, AA, BA, 2, 2, 2, 2, 64, 3><<<grid, 256, 0, s>>>(pl.p, e);
   else product_kernel<K, AA, BA, 1, 4, 1, 1, 128, 3><<<grid, 256, 0, s>>>(pl.p, e);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || pl.p.splits == 1) return err;

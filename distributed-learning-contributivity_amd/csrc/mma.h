@@ -24,6 +24,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace mma {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -67,17 +69,13 @@ template <Kind K> __device__ __forceinline__ typename Elem<K>::T from_f32(float 
   else return f32_to_f16(v);
 }
 
-// vectors of any element alignment (gfx950 global memory takes unaligned dwordx4)
-struct __attribute__((packed, aligned(2))) U4a2 { uint32_t v[4]; };
-struct __attribute__((packed, aligned(2))) U2a2 { uint32_t v[2]; };
-struct __attribute__((packed, aligned(4))) U4a4 { uint32_t v[4]; };
+// vectors at any element's place (gfx950 global memory takes unaligned loads; as one vector type each, which the
+// compiler does not take apart)
+typedef uint32_t u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2a2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 
-__device__ __forceinline__ u32x4 load16(const void* p) {
-  const U4a2 t = *reinterpret_cast<const U4a2*>(p);
-  u32x4 r;
-  r[0] = t.v[0]; r[1] = t.v[1]; r[2] = t.v[2]; r[3] = t.v[3];
-  return r;
-}
+__device__ __forceinline__ u32x4 load16(const void* p) { return *reinterpret_cast<const u32x4a2*>(p); }
 
 // `n` valid elements from p (n <= 0: none), the rest zero
 template <Kind K> __device__ __forceinline__ u32x4 load16_edge(const typename Elem<K>::T* p, int n) {
@@ -96,38 +94,52 @@ template <Kind K> __device__ __forceinline__ u32x4 load16_edge(const typename El
   return r;
 }
 
-// 4 consecutive elements starting at p, n of them valid
-template <Kind K> __device__ __forceinline__ f32x4 load4(const typename Elem<K>::T* p, int n) {
-  f32x4 r = {0.f, 0.f, 0.f, 0.f};
-  if (n >= 4) {
+// 4 consecutive elements starting at p, n >= 1 of them valid, the others 0, without a branch: the compiler waits for what
+// each branch has loaded, one latency after the other.  WIDE: the row has 4 elements or more, and one load that ends at the
+// row's end takes a cut group; otherwise the last element is read again in the place of those that are not there.
+template <Kind K, bool WIDE> __device__ __forceinline__ f32x4 load4(const typename Elem<K>::T* p, int n) {
+  f32x4 r;
+  if constexpr (WIDE) {
+    const int d = n >= 4 ? 0 : 4 - n;
     if constexpr (K == F32) {
-      const U4a4 t = *reinterpret_cast<const U4a4*>(p);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = __uint_as_float(t.v[e]);
+      r = *reinterpret_cast<const f32x4a4*>(p - d);
     } else {
-      const U2a2 t = *reinterpret_cast<const U2a2*>(p);
+      const u32x2 t = *reinterpret_cast<const u32x2a2*>(p - d);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = to_f32<K>((uint16_t)(t.v[e >> 1] >> (16 * (e & 1))));
+      for (int e = 0; e < 4; ++e) r[e] = to_f32<K>((uint16_t)(t[e >> 1] >> (16 * (e & 1))));
     }
+    const bool two = d & 2, one = d & 1;
+    r[0] = two ? r[2] : r[0];
+    r[1] = two ? r[3] : r[1];
+    r[2] = two ? 0.f : r[2];
+    r[3] = two ? 0.f : r[3];
+    r[0] = one ? r[1] : r[0];
+    r[1] = one ? r[2] : r[1];
+    r[2] = one ? r[3] : r[2];
+    r[3] = one ? 0.f : r[3];
   } else {
 #pragma unroll
-    for (int e = 0; e < 3; ++e)
-      if (e < n) r[e] = to_f32<K>(p[e]);
+    for (int e = 0; e < 4; ++e) {
+      r[e] = to_f32<K>(p[e < n ? e : n - 1]);
+      r[e] = e < n ? r[e] : 0.f;
+    }
   }
   return r;
+}
+// f(true or false) for WIDE, chosen once
+template <typename F> __device__ __forceinline__ void by_width(int columns, F f) {
+  if (columns >= 4) f(std::true_type{});
+  else f(std::false_type{});
 }
 template <Kind K> __device__ __forceinline__ void store4(typename Elem<K>::T* p, f32x4 v, int n) {
   if (n >= 4) {
     if constexpr (K == F32) {
-      U4a4 t;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) t.v[e] = __float_as_uint(v[e]);
-      *reinterpret_cast<U4a4*>(p) = t;
+      *reinterpret_cast<f32x4a4*>(p) = v;
     } else {
-      U2a2 t;
-      t.v[0] = (uint32_t)from_f32<K>(v[0]) | ((uint32_t)from_f32<K>(v[1]) << 16);
-      t.v[1] = (uint32_t)from_f32<K>(v[2]) | ((uint32_t)from_f32<K>(v[3]) << 16);
-      *reinterpret_cast<U2a2*>(p) = t;
+      u32x2 t;
+      t[0] = (uint32_t)from_f32<K>(v[0]) | ((uint32_t)from_f32<K>(v[1]) << 16);
+      t[1] = (uint32_t)from_f32<K>(v[2]) | ((uint32_t)from_f32<K>(v[3]) << 16);
+      *reinterpret_cast<u32x2a2*>(p) = t;
     }
   } else {
 #pragma unroll
@@ -256,9 +268,7 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
 #pragma unroll
     for (int j = 0; j < PER; ++j)
 #pragma unroll
-      for (int p = 0; p < PL; ++p) {
-        *reinterpret_cast<u32x4*>(lds + p * PLANE_BYTES + (tid + j * NT) * 16) = reg.v[p][j];
-      }
+      for (int p = 0; p < PL; ++p) *reinterpret_cast<u32x4*>(lds + p * PLANE_BYTES + (tid + j * NT) * 16) = reg.v[p][j];
   }
   // the fragment of rows [i, i + 32) for k-step ks (2 chunks of r)
   __device__ __forceinline__ static u32x4 frag(const char* lds, int plane, int i, int ks, int lane) {

@@ -77,20 +77,38 @@ struct Source {
   int nesterov, rows, cols;
 };
 
-// U at (r, c .. c + 3), `valid` of them inside; FIRST: the pass that updates the momentum
-template <Kind K, bool FIRST> __device__ __forceinline__ f32x4 update4(const Source& s, int g, int64_t r, int c, int valid) {
+// U at (r, c .. c + 3), `valid` of them inside, in two steps, so that several groups' loads are on their way at a time.
+struct Raw {
+  f32x4 g, m;
+};
+// N groups at at(j, r, c, valid); the momentum's loads stand in one branch, which the compiler waits for as a whole
+template <Kind K, bool WIDE, int N, typename At> __device__ __forceinline__ void raw4(Raw (&x)[N], const Source& s, int g, At at) {
   typedef typename Elem<K>::T T;
-  f32x4 u = load4<K>(reinterpret_cast<const T*>(s.g) + g * s.g_stride + r * s.g_ld + c, valid);
-  if (s.m == nullptr) return u;
-  float* pm = s.m + g * s.m_stride + r * s.m_ld + c;
-  f32x4 m = load4<F32>(pm, valid);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    int r, c, valid;
+    at(j, r, c, valid);
+    x[j].g = load4<K, WIDE>(reinterpret_cast<const T*>(s.g) + g * s.g_stride + r * s.g_ld + c, valid);
+  }
+  if (s.m)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      int r, c, valid;
+      at(j, r, c, valid);
+      x[j].m = load4<F32, WIDE>(s.m + g * s.m_stride + r * s.m_ld + c, valid);
+    }
+}
+// FIRST: the pass that updates the momentum
+template <bool FIRST> __device__ __forceinline__ f32x4 update4(const Source& s, Raw x, int g, int64_t r, int c, int valid) {
+  if (s.m == nullptr) return x.g;
   if (FIRST) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m[i] = s.beta * m[i] + u[i];
-    store4<F32>(pm, m, valid);
+    for (int i = 0; i < 4; ++i) x.m[i] = s.beta * x.m[i] + x.g[i];
+    store4<F32>(s.m + g * s.m_stride + r * s.m_ld + c, x.m, valid);
   }
+  f32x4 u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) u[i] = s.nesterov ? s.beta * m[i] + u[i] : m[i];
+  for (int i = 0; i < 4; ++i) u[i] = s.nesterov ? s.beta * x.m[i] + x.g[i] : x.m[i];
   return u;
 }
 
@@ -133,11 +151,29 @@ template <Kind K> __global__ __launch_bounds__(256) void norm_kernel(const Sourc
   __shared__ double part[4];
   const int g = blockIdx.y;
   double sum = 0.;
-  for (Walk w(blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, (s.cols + 3) >> 2); w.r < s.rows; w.next()) {
-    const f32x4 v = update4<K, true>(s, g, w.r, w.c4 * 4, s.cols - w.c4 * 4);
+  by_width(s.cols, [&](auto wide) {
+    for (Walk w(blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, (s.cols + 3) >> 2); w.r < s.rows;) {
+      Raw x[4];
+      int r[4], c[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum += (double)v[i] * (double)v[i];
-  }
+      for (int j = 0; j < 4; ++j, w.next()) {  // behind the last row: the last one again, not used
+        r[j] = w.r;
+        c[j] = w.c4 * 4;
+      }
+      raw4<K, decltype(wide)::value>(x, s, g, [&](int j, int& row, int& col, int& valid) {
+        row = min(r[j], s.rows - 1);
+        col = c[j];
+        valid = s.cols - col;
+      });
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (r[j] < s.rows) {
+          const f32x4 v = update4<true>(s, x[j], g, r[j], c[j], s.cols - c[j]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum += (double)v[i] * (double)v[i];
+        }
+    }
+  });
   sum = block_sum(sum, part);
   if (threadIdx.x == 0) sums[(int64_t)g * gridDim.x + blockIdx.x] = sum;
 }
@@ -147,13 +183,30 @@ template <Kind K> __global__ __launch_bounds__(256) void start_kernel(const Sour
   __shared__ double part[4];
   const int g = blockIdx.y;
   const double inv = inverse_norm(block_sum(threadIdx.x < chunks ? sums[(int64_t)g * chunks + threadIdx.x] : 0., part));
-  for (Walk w(blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, x.ld >> 3); w.r < s.rows; w.next()) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (w.c4 * 4 < s.cols) v = update4<K, false>(s, g, w.r, w.c4 * 4, s.cols - w.c4 * 4);
+  by_width(s.cols, [&](auto wide) {
+    for (Walk w(blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, x.ld >> 3); w.r < s.rows;) {
+      Raw u[4];
+      int r[4], c[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (float)((double)v[i] * inv);
-    store_planes(x, g, w.r, w.c4 * 4, v);
-  }
+      for (int j = 0; j < 4; ++j, w.next()) {  // behind the last row or column: the last ones again, not used
+        r[j] = w.r;
+        c[j] = w.c4 * 4;
+      }
+      raw4<K, decltype(wide)::value>(u, s, g, [&](int j, int& row, int& col, int& valid) {
+        row = min(r[j], s.rows - 1);
+        col = c[j] < s.cols ? c[j] : (s.cols - 1) & ~3;
+        valid = s.cols - col;
+      });
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (r[j] < s.rows) {
+          f32x4 v = update4<false>(s, u[j], g, r[j], c[j], s.cols - c[j]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = c[j] < s.cols ? (float)((double)v[i] * inv) : 0.f;
+          store_planes(x, g, r[j], c[j], v);
+        }
+    }
+  });
 }
 
 // The same with L = cols: 64 x 64 tiles, transposed through LDS
@@ -164,12 +217,23 @@ template <Kind K> __global__ __launch_bounds__(256) void start_wide_kernel(const
   const double inv = inverse_norm(block_sum(threadIdx.x < chunks ? sums[(int64_t)g * chunks + threadIdx.x] : 0., part));
   const int l0 = blockIdx.x * 64, k0 = blockIdx.y * 64;
   const int q = (threadIdx.x & 15) * 4, ty = threadIdx.x >> 4;
-  for (int i = ty; i < 64; i += 16) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (k0 + i < s.rows && l0 + q < s.cols) v = update4<K, false>(s, g, k0 + i, l0 + q, s.cols - l0 - q);
+  by_width(s.cols, [&](auto wide) {
+    Raw u[4];
+    const int in = l0 + q < s.cols ? l0 + q : (s.cols - 1) & ~3;
+    raw4<K, decltype(wide)::value>(u, s, g, [&](int j, int& row, int& col, int& valid) {
+      row = min(k0 + ty + 16 * j, s.rows - 1);
+      col = in;
+      valid = s.cols - in;
+    });
 #pragma unroll
-    for (int e = 0; e < 4; ++e) tile[q + e][i] = (float)((double)v[e] * inv);
-  }
+    for (int j = 0; j < 4; ++j) {
+      const int i = ty + 16 * j;
+      const f32x4 v = update4<false>(s, u[j], g, k0 + i, l0 + q, s.cols - l0 - q);
+      const bool inside = k0 + i < s.rows && l0 + q < s.cols;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) tile[q + e][i] = inside ? (float)((double)v[e] * inv) : 0.f;
+    }
+  });
   __syncthreads();
   for (int i = ty; i < 64; i += 16)
     if (l0 + i < s.cols && k0 + q < (x.ld >> 1)) {
@@ -267,10 +331,6 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Prod p) {
     typedef typename Elem<K>::T T;
     T* dst = reinterpret_cast<T*>(p.dst) + g * p.dst_stride;
     const int rows = p.transposed ? p.n : p.m, cols = p.transposed ? p.m : p.n;
-    auto before = [&](int r, int c) {
-      if constexpr (E == STEP) return r < rows && c < cols ? load4<K>(dst + r * p.dst_ld + c, cols - c) : f32x4{0.f, 0.f, 0.f, 0.f};
-      else return 0;
-    };
     auto result = [&](int r, int c, f32x4 v, auto w) {
       if (r >= rows || c >= cols) return;
       v *= p.alpha;
@@ -279,8 +339,17 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Prod p) {
         for (int i = 0; i < 4; ++i) v[i] = p.keep * w[i] - p.step * v[i];
       store4<K>(dst + r * p.dst_ld + c, v, cols - c);
     };
-    if (p.transposed) blk.each_column(lds, m0, n0, before, result);
-    else blk.each_row(lds, m0, n0, before, result);
+    auto finish = [&](auto before) {
+      if (p.transposed) blk.each_column(lds, m0, n0, before, result);
+      else blk.each_row(lds, m0, n0, before, result);
+    };
+    if constexpr (E == STEP)
+      by_width(cols, [&](auto wide) {
+        finish([&](int r, int c) {
+          return r < rows && c < cols ? load4<K, decltype(wide)::value>(dst + r * p.dst_ld + c, cols - c) : f32x4{0.f, 0.f, 0.f, 0.f};
+        });
+      });
+    else finish([](int, int) { return 0; });
   }
 }
 
@@ -294,19 +363,21 @@ __global__ __launch_bounds__(256) void join_kernel(const Prod p) {
   const float* src = p.partial + (int64_t)g * p.m * p.n;
   const int64_t step = (int64_t)p.models * p.m * p.n;
   const int q = (threadIdx.x & 15) * 4;
-  for (int i = threadIdx.x >> 4; i < 64; i += 16) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    const int m = m0 + i, n = n0 + q;
-    if (m < p.m && n < p.n) {
-      const float* at = src + (int64_t)m * p.n + n;
-      v = load4<F32>(at, p.n - n);
-      for (int s = 1; s < p.splits; ++s) v += load4<F32>(at + s * step, p.n - n);
-      v *= p.alpha;
-    }
-    if (m < p.m && n < p.out.ld / 2) store_planes(p.out, g, m, n, v);
+  by_width(p.n, [&](auto wide) {
+    for (int i = threadIdx.x >> 4; i < 64; i += 16) {
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      const int m = m0 + i, n = n0 + q;
+      if (m < p.m && n < p.n) {
+        const float* at = src + (int64_t)m * p.n + n;
+#pragma unroll 4
+        for (int s = 0; s < p.splits; ++s) v += load4<F32, decltype(wide)::value>(at + s * step, p.n - n);
+        v *= p.alpha;
+      }
+      if (m < p.m && n < p.out.ld / 2) store_planes(p.out, g, m, n, v);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) tile[q + e][i] = v[e];
-  }
+      for (int e = 0; e < 4; ++e) tile[q + e][i] = v[e];
+    }
+  });
   if (tm == tn) return;
   __syncthreads();
   for (int i = threadIdx.x >> 4; i < 64; i += 16) {
@@ -438,16 +509,33 @@ template <Kind K, int KT, Epi E> __global__ __launch_bounds__(256) void small_ke
   for (int i = tid * 4; i < Lp * S; i += 1024) *reinterpret_cast<f32x4*>(X + i) = f32x4{0.f, 0.f, 0.f, 0.f};
   __syncthreads();
   double sum = 0.;
-  for (Walk w(tid, 256, n4); w.r < s.rows; w.next()) {
-    const int c = w.c4 * 4;
-    const f32x4 v = update4<K, true>(s, g, w.r, c, s.cols - c);
+  by_width(s.cols, [&](auto wide) {
+    for (Walk w(tid, 256, n4); w.r < s.rows;) {
+      Raw x[4];
+      int r[4], c[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (c + e < s.cols) {
-        X[p.tall ? w.r * S + c + e : (c + e) * S + w.r] = v[e];
-        sum += (double)v[e] * (double)v[e];
+      for (int j = 0; j < 4; ++j, w.next()) {  // behind the last row: the last one again, not used
+        r[j] = w.r;
+        c[j] = w.c4 * 4;
       }
-  }
+      raw4<K, decltype(wide)::value>(x, s, g, [&](int j, int& row, int& col, int& valid) {
+        row = min(r[j], s.rows - 1);
+        col = c[j];
+        valid = s.cols - col;
+      });
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (r[j] < s.rows) {
+          const f32x4 v = update4<true>(s, x[j], g, r[j], c[j], s.cols - c[j]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c[j] + e < s.cols) {
+              X[p.tall ? r[j] * S + c[j] + e : (c[j] + e) * S + r[j]] = v[e];
+              sum += (double)v[e] * (double)v[e];
+            }
+        }
+    }
+  });
   const double inv = inverse_norm(block_sum(sum, part)) * (1. / X_SCALE);
   for (int i = tid * 4; i < Lp * S; i += 1024) {
     f32x4 v = *reinterpret_cast<f32x4*>(X + i);
@@ -490,7 +578,7 @@ template <Kind K, int KT, Epi E> __global__ __launch_bounds__(256) void small_ke
     for (int e = 0; e < 4; ++e) v[e] = c + e < s.cols ? X[p.tall ? w.r * S + c + e : (c + e) * S + w.r] : 0.f;
     O* at = dst + w.r * p.dst_ld + c;
     if constexpr (E == STEP) {
-      const f32x4 old = load4<F32>(at, s.cols - c);
+      const f32x4 old = load4<F32, false>(at, s.cols - c);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = p.keep * old[e] - p.step * v[e];
       store4<F32>(at, v, s.cols - c);
@@ -578,14 +666,34 @@ template <Kind K, int KP, bool TALL, int NT> struct Piece {
     row = c / PER;
     col = (c % PER) * 4;
   }
-  template <bool FIRST> __device__ __forceinline__ void load(const Source& s, int g, int l0, int lend, int k) {
+  Raw raw[N];
+  __device__ __forceinline__ bool inside(int j, int l0, int lend, int k, int& r, int& c, int& valid) const {
+    int row, col;
+    place(j, row, col);
+    r = TALL ? l0 + row : row;
+    c = TALL ? col : l0 + col;
+    valid = (TALL ? k : lend) - c;
+    return r < (TALL ? lend : k) && valid > 0;
+  }
+  // asks for the rows, and takes what has come
+  __device__ __forceinline__ void ask(const Source& s, int g, int l0, int lend, int k) {
+    // what is not inside reads the first element's group, and is not used; a wide matrix's row goes on behind a chunk
+    raw4<K, true>(raw, s, g, [&](int j, int& r, int& c, int& valid) {
+      const bool in = inside(j, l0, lend, k, r, c, valid);
+      r = in ? r : 0;
+      valid = in ? (TALL ? valid : s.cols - c) : 4;
+      c = in ? c : 0;
+    });
+  }
+  template <bool FIRST> __device__ __forceinline__ void take(const Source& s, int g, int l0, int lend, int k) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      int row, col;
-      place(j, row, col);
-      const int r = TALL ? l0 + row : row, c = TALL ? col : l0 + col;
-      const int rend = TALL ? lend : k, cend = TALL ? k : lend;
-      u[j] = r < rend && c < cend ? update4<K, FIRST>(s, g, r, c, cend - c) : f32x4{0.f, 0.f, 0.f, 0.f};
+      int r, c, valid;
+      const bool in = inside(j, l0, lend, k, r, c, valid);
+      f32x4 v = raw[j].g;
+      if (s.m && (!FIRST || in)) v = update4<FIRST>(s, raw[j], g, r, c, valid);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[j][e] = in && e < valid ? v[e] : 0.f;
     }
   }
   // planes for a sum over l (GRAM) or over k: whichever of the stored rows' directions that is
@@ -679,8 +787,9 @@ template <Kind K, int KP, bool TALL> __global__ __launch_bounds__(GRAM_THREADS) 
   Gt gt;
   gt.init();
   int exponent = -300;  // values are below 2^(exponent + 14); nothing seen yet
-  pc.template load<true>(p.src, g, begin, end, p.k);
+  pc.ask(p.src, g, begin, end, p.k);
   for (int l0 = begin; l0 < end; l0 += Pc::TR) {
+    pc.template take<true>(p.src, g, l0, end, p.k);
     float mx = 0.f;
 #pragma unroll
     for (int j = 0; j < Pc::N; ++j)
@@ -706,7 +815,7 @@ template <Kind K, int KP, bool TALL> __global__ __launch_bounds__(GRAM_THREADS) 
     const int down = exponent > -300 ? -exponent : 0;
     pc.template store<true>(lds, [&](float v) { return ldexpf(v, down); });
     __syncthreads();
-    if (l0 + Pc::TR < end) pc.template load<true>(p.src, g, l0 + Pc::TR, end, p.k);
+    if (l0 + Pc::TR < end) pc.ask(p.src, g, l0 + Pc::TR, end, p.k);
     gt.add([&](int plane, int i, int ks) {
       if constexpr (TALL) return frag_across<Pc::RB>(lds + plane * Pc::ACROSS, i, ks, lane);
       else return frag_along<Pc::RB>(lds + plane * Pc::ALONG, i, ks, lane);
@@ -772,13 +881,14 @@ __global__ __launch_bounds__(NARROW_THREADS) void narrow_apply_kernel(const Narr
   Pc pc;
   Gt gt;
   if constexpr (GRAM) gt.init();
-  pc.template load<false>(p.src, g, begin, end, p.k);
+  pc.ask(p.src, g, begin, end, p.k);
   load_square<KP>(lds, p.q, g);
   for (int l0 = begin; l0 < end; l0 += TR) {
+    pc.template take<false>(p.src, g, l0, end, p.k);
     __syncthreads();  // the last tile is done with
     pc.template store<false>(xs, [&](float v) { return (float)((double)v * inv); });
     __syncthreads();
-    if (l0 + TR < end) pc.template load<false>(p.src, g, l0 + TR, end, p.k);
+    if (l0 + TR < end) pc.ask(p.src, g, l0 + TR, end, p.k);
     f32x16 acc[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -841,7 +951,7 @@ __global__ __launch_bounds__(NARROW_THREADS) void narrow_apply_kernel(const Narr
         if (r < rend && c < cend) {
           O* at = dst + r * p.dst_ld + c;
           if constexpr (E == STEP) {
-            const f32x4 old = load4<F32>(at, cend - c);
+            const f32x4 old = load4<F32, true>(at, cend - c);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = p.keep * old[e] - p.step * v[e];
             store4<F32>(at, v, cend - c);
@@ -1069,14 +1179,15 @@ bool space(const mplc_muon_t& t, Space& s) {
     s.phases = (t.steps + 1) / 2;
     return true;
   }
-  if (s.k <= 128 && t.steps <= 6 && t.n_models <= 65535) {  // two phases of three steps at most
+  if (s.k <= 128 && t.steps <= 6 && t.cols >= 4) {  // two phases of three steps at most; whole groups of columns
     s.narrow = s.k <= 64 ? 64 : 128;
     s.phases = (t.steps + 2) / 3;
     const int64_t tr = 16384 / s.narrow, pieces = ceil_div(s.L, tr);
     // about one workgroup per CU and round, whole pieces, at least two per workgroup where there are many
     int64_t per = ceil_div(pieces * s.planned, 512);
     if (per > pieces) per = pieces;
-    s.rows_per = (int)((per < 1 ? 1 : per) * tr);
+    per = per < 1 ? 1 : ceil_div(pieces, ceil_div(pieces, per));  // chunks of one size
+    s.rows_per = (int)(per * tr);
     s.chunks = (int)ceil_div(s.L, s.rows_per);
     const size_t G = (size_t)t.n_models, tiles = s.narrow == 128 ? 10 : 3;
     s.sums = align16(G * s.chunks * sizeof(int)) + align16(G * sizeof(double));
