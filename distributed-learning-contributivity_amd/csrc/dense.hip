@@ -204,6 +204,66 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
   }
 }
 
+// Few rows (ROWS at most): the weights stream through once and the product is a few multiply-adds per element, so there
+// is nothing for the matrix cores to share.  A wave takes 256 columns, 4 a lane, and every fourth group of 8 r; a row's
+// x[r] is one value for the whole wave, from LDS.  Each lane keeps 8 loads of w on their way.
+template <Kind K, int ROWS> __global__ __launch_bounds__(256) void rows_kernel(const Product p, const Epilogue e) {
+  typedef typename Elem<K>::T T;
+  constexpr int STEP = 512;  // r whose x is staged at a time
+  __shared__ float xs[STEP][ROWS];
+  __shared__ f32x4 part[4][ROWS][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t b = xcd_block();
+  const int tn = (int)(b % p.tiles_n), split = (int)(b / p.tiles_n % p.splits), g = (int)(b / p.tiles_n / p.splits);
+  const int M = count_of(p.counts, g, p.m);
+  if (M == 0) return;
+  const int c = (tn * 64 + lane) * 4, in = c < p.n ? c : (p.n - 1) & ~3;
+  const int first = split * p.per_split * unit_of(K), last = min(p.r, first + p.per_split * unit_of(K));
+  const T* x = reinterpret_cast<const T*>(p.a) + g * p.a_stride;
+  const T* w = reinterpret_cast<const T*>(p.b) + g * p.b_stride + in;
+  f32x4 acc[ROWS];
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  by_width(p.n, [&](auto wide) {
+    for (int r0 = first; r0 < last; r0 += STEP) {
+      const int n = min(STEP, last - r0);
+      __syncthreads();
+      for (int i = threadIdx.x; i < ROWS * STEP; i += 256) {
+        const int m = i / STEP, r = i % STEP;
+        xs[r][m] = m < M && r < n ? to_f32<K>(x[m * p.a_ld + r0 + r]) : 0.f;
+      }
+      __syncthreads();
+      for (int r = wave * 8; r < n; r += 32) {
+        f32x4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)  // behind the last r: the last one again, not added
+          v[i] = load4<K, decltype(wide)::value>(w + min(r0 + r + i, last - 1) * p.b_ld, p.n - in);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (r + i < n)
+#pragma unroll
+            for (int m = 0; m < ROWS; ++m) acc[m] += xs[r + i][m] * v[i];
+        }
+      }
+    }
+  });
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m) part[wave][m][lane] = acc[m];
+  __syncthreads();
+  by_width(p.n, [&](auto wide) {
+    constexpr bool W = decltype(wide)::value;
+    for (int m = wave; m < ROWS; m += 4)
+      if (m < M && c < p.n) {
+        f32x4 v = part[0][m][lane] + part[1][m][lane];
+        v += part[2][m][lane] + part[3][m][lane];
+        if (p.splits > 1)
+          store4<F32>(p.partial + (((int64_t)split * p.models + g) * p.m + m) * p.n + c, v, p.n - c);
+        else
+          finish<K>(e, g, m, c, p.n, v, bias_at<K, W>(e, g, c, p.n), residual_at<K, W>(e, g, m, c, p.n));
+      }
+  });
+}
+
 // adds the partial sums of one product in order and finishes it
 template <Kind K> __global__ __launch_bounds__(256) void join_kernel(const Product p, const Epilogue e) {
   const int n4 = (p.n + 3) >> 2;
@@ -315,7 +375,7 @@ __global__ __launch_bounds__(256) void db_kernel(const float* sums, int blocks, 
 enum Form { FORWARD, DX, DW };
 
 struct Plan {
-  int cfg;  // place in SHAPES_16 / SHAPES_F32
+  int cfg;  // place in SHAPES_16 / SHAPES_F32; 5: short sums; 6: few rows
   Product p;
   int64_t blocks;
   size_t partial_bytes;
@@ -352,6 +412,25 @@ bool plan(const mplc_dense_t& t, Form form, Plan& out) {
   if ((c.tile == 0 || c.tile == 3) && p.nk <= 2) out.cfg = 5;
   p.splits = c.splits;
   p.per_split = c.per_split;
+  // Few rows of weights that no 16-byte load takes whole: 81 x 2 rows, 3256 -> 653 fp16 107 us against 272 on the tiles;
+  // aligned ones stream as fast through the tiles (8 x 1 row, 4096 -> 4096 bf16: 44 against 41 us).
+  if (form == FORWARD && p.m <= 8 && p.n >= 128 && p.n % (f32 ? 4 : 8) != 0) {
+    // 256 columns a workgroup; r split until there are 4 workgroups per CU, at least 128 r each
+    out.cfg = 6;
+    p.tiles_m = 1;
+    p.tiles_n = (int)ceil_div(p.n, 256);
+    const int64_t blocks = (int64_t)p.tiles_n * p.models, least = 128 / (f32 ? unit_of(F32) : unit_of(BF16));
+    int64_t splits = ceil_div(1024, blocks > 0 ? blocks : 1);
+    if (splits > p.nk / least) splits = p.nk / least;
+    if (splits < 1) splits = 1;
+    p.per_split = (int)(p.nk > 0 ? ceil_div(p.nk, splits) : 1);
+    p.splits = (int)(p.nk > 0 ? ceil_div(p.nk, p.per_split) : 1);
+    if (blocks * p.splits > (1 << 23)) return false;
+    out.blocks = blocks * p.splits;
+    out.partial_bytes = p.splits > 1 ? (size_t)p.splits * p.models * p.m * p.n * sizeof(float) : 0;
+    out.p = p;
+    return true;
+  }
   p.tiles_m = (int)(out.cfg == 5 ? ceil_div(p.m, 128) : c.tiles_m);
   p.tiles_n = (int)(out.cfg == 5 ? ceil_div(p.n, 128) : c.tiles_n);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.models;
@@ -370,7 +449,14 @@ template <Kind K, bool AA, bool BA> hipError_t launch(Plan& pl, const Epilogue& 
   pl.p.aligned = fits(pl.p.a, pl.p.a_stride, pl.p.a_ld) && fits(pl.p.b, pl.p.b_stride, pl.p.b_ld) &&
                  (!AA || pl.p.m % ch == 0) && (!BA || pl.p.b_cols % ch == 0);
   const dim3 grid((unsigned)pl.blocks);
-  if (pl.cfg == 0) product_kernel<K, AA, BA, 2, 2, 2, 2, 128, 2><<<grid, 256, 0, s>>>(pl.p, e);
+  if (pl.cfg == 6) {
+    if constexpr (!AA && BA) {  // the forward product
+      if (pl.p.m <= 1) rows_kernel<K, 1><<<grid, 256, 0, s>>>(pl.p, e);
+      else if (pl.p.m <= 2) rows_kernel<K, 2><<<grid, 256, 0, s>>>(pl.p, e);
+      else if (pl.p.m <= 4) rows_kernel<K, 4><<<grid, 256, 0, s>>>(pl.p, e);
+      else rows_kernel<K, 8><<<grid, 256, 0, s>>>(pl.p, e);
+    }
+  } else if (pl.cfg == 0) product_kernel<K, AA, BA, 2, 2, 2, 2, 128, 2><<<grid, 256, 0, s>>>(pl.p, e);
   else if (pl.cfg == 1) product_kernel<K, AA, BA, 2, 2, 1, 1, 128, 3><<<grid, 256, 0, s>>>(pl.p, e);
   else if (pl.cfg == 4) product_kernel<K, AA, BA, 1, 4, 2, 1, 128, 2><<<grid, 256, 0, s>>>(pl.p, e);
   else if (pl.cfg == 3) {

@@ -152,6 +152,17 @@ def test_long_sums_are_split(G, B, K, N):
         check_backward(rand((G, B, N), t, 5), x, w, pre, "silu")
 
 
+@pytest.mark.parametrize("rows", [1, 2, 3, 8])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_few_rows_of_odd_weights(rows, dtype):
+    t = TYPES[dtype]
+    for K, N in ((7, 129), (1001, 333), (4100, 131)):
+        counts = torch.tensor([rows, 0, rows - 1], dtype=torch.int32, device="cuda")
+        check_forward(rand((3, rows, K), t, 1), rand((3, K, N), t, 2, K ** -0.5), rand((3, N), t, 3), rand((3, rows, N), t, 4),
+                      "gelu", counts)
+        check_forward(rand((rows, K), t, 5), rand((3, K, N), t, 2, K ** -0.5), act="none")
+
+
 def test_long_batch():
     x, w = rand((1, 3000, 40), torch.float16, 1), rand((1, 40, 24), torch.float16, 2)
     _, pre = check_forward(x, w, act="gelu")
