@@ -64,11 +64,10 @@ class _Plan:
     spans (for the overlap check, which needs the addresses)."""
 
     def __init__(self, lib, name, struct, device, fields, tensors):
-        self.lib, self.name, self.device = lib, name, device
+        self.name, self.device = name, device
         self.fn = getattr(lib, name)
         self.index = device.index
         self.fields = fields  # (struct field, position among the call's tensors, is an output)
-        self.size = ctypes.sizeof(struct)
         self.struct = type(struct)
         self.workspace = int(getattr(lib, name + "_workspace_bytes")(ctypes.byref(struct)))
         struct.workspace_bytes = self.workspace

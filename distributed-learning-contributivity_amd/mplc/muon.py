@@ -7,6 +7,7 @@ round's average (``CoalitionEngine(server_optimizer=...)``).  Work goes to torch
 """
 import ctypes
 import math
+import operator
 
 import torch
 
@@ -87,15 +88,15 @@ def _setup(g, name, steps, coefficients, invariant):
     if G > 65535:
         raise ValueError("at most 65535 models per call")
     _tensor(g3, name, g.dtype, g.device, (G, m, n))
-    if not 1 <= int(steps) <= 16:
+    if not 1 <= operator.index(steps) <= 16:
         raise ValueError(f"steps must be 1 to 16, not {steps}")
     coefficients = tuple(float(v) for v in coefficients)
     if len(coefficients) != 3 or not all(abs(v) < 1e3 for v in coefficients):
         raise ValueError(f"coefficients must be three finite numbers (a, b, c), not {coefficients}")
-    if singular_range(int(steps), coefficients) > 2.0:
+    if singular_range(operator.index(steps), coefficients) > 2.0:
         raise ValueError(f"coefficients {coefficients} let singular values grow past 2")
     t = MuonT()
-    t.n_models, t.rows, t.cols, t.dtype, t.steps = G, m, n, DTYPES[str(g.dtype)], int(steps)
+    t.n_models, t.rows, t.cols, t.dtype, t.steps = G, m, n, DTYPES[str(g.dtype)], operator.index(steps)
     t.a, t.b, t.c = coefficients
     t.invariant = int(bool(invariant))
     _place(t, "g", g3)
@@ -103,9 +104,9 @@ def _setup(g, name, steps, coefficients, invariant):
 
 
 def _key(kind, steps, coefficients, invariant, tensors):
-    try:
-        return (kind, steps, tuple(coefficients), bool(invariant)) + tuple(_sig(t) for t in tensors)
-    except (AttributeError, TypeError):  # not tensors, not numbers: the checks say so
+    try:  # numbers, not what holds them: a key is compared by value
+        return (kind, operator.index(steps), tuple(float(v) for v in coefficients), bool(invariant)) + tuple(_sig(t) for t in tensors)
+    except (AttributeError, TypeError, ValueError):  # not tensors, not numbers: the checks say so
         return None
 
 
@@ -209,7 +210,7 @@ class ServerMuon:
         numbers = [float(p[k]) for k in ("lr", "beta", "weight_decay")]
         if not all(math.isfinite(v) for v in numbers) or not 0.0 <= numbers[1] < 1.0 or numbers[0] <= 0.0:
             raise ValueError(f"server optimizer 'muon': lr must be positive and beta in [0, 1): {p}")
-        if not 1 <= int(p["steps"]) <= 16:
+        if int(p["steps"]) != p["steps"] or not 1 <= p["steps"] <= 16:
             raise ValueError(f"server optimizer 'muon': steps must be 1 to 16, not {p['steps']}")
 
     def describe(self):
