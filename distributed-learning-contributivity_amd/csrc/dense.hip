@@ -1,8 +1,7 @@
 // Dense layer batched over models (gfx950): y[g] = act(x[g] w[g] + b[g]) + r[g] and its gradients, any size, fp32 / bf16 /
 // fp16, ragged row counts, one input shared by all models.  include/mplc_hip_ops.h states the operator.
 //
-// All three products run on the tiled core of mma.h without a transposition of an operand, and without a copy but for
-// large products of 16-bit rows that no 16-byte load takes whole (pad_pays()):
+// All three products run on the tiled core of mma.h without a copy or a transposition of an operand:
 //   forward  y  [row][out] = sum over in  of x[row][in]  w[in][out]    A along r, B across r
 //   dx          [row][in]  = sum over out of dz[row][out] w[in][out]   A along r, B along r
 //   dw          [in][out]  = sum over row of x[row][in]  dz[row][out]  A across r, B across r
@@ -46,7 +45,7 @@ struct Product {
   int count_is_r;        // counts limit r (dw), not m
   int tiles_m, tiles_n, nk, splits, per_split;  // nk: units of r; per_split: units of a split
   int aligned;           // 16-byte rows: tiles go straight into LDS
-  int a_cols, b_cols;    // across r: columns of A or B that may be read (m or n, or their padding too)
+  int b_cols;            // across r: columns of B that may be read (n, or its padding too)
   float* partial;        // [split][model][m][n] where splits > 1
 };
 
@@ -182,7 +181,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
       });
     }
   } else {
-    const Operand<T> a = {pa, p.a_ld, AA ? p.a_cols : M}, o = {pb, p.b_ld, BA ? p.b_cols : p.n};
+    const Operand<T> a = {pa, p.a_ld, M}, o = {pb, p.b_ld, BA ? p.b_cols : p.n};
     blk.run(lds, a, o, m0, n0, (int)min((int64_t)R, first * unit_of(K)), (int)min((int64_t)R, last * unit_of(K)), p.aligned);
   }
   if (p.splits > 1) {
@@ -289,40 +288,6 @@ template <Kind K> __global__ __launch_bounds__(256) void join_kernel(const Produ
     }
     finish<K>(e, g, m, n, p.n, v, bias, res);
   });
-}
-
-// 16-bit rows of any length and place, copied to rows of whole 16-byte chunks, zeros behind the last column; cols >= 8.
-// Rows at or behind a model's count are left out.  A cut chunk comes from a load that ends at the row's end.
-__global__ __launch_bounds__(256) void pad_kernel(const uint16_t* src, int64_t stride, int64_t ld, int rows, int cols,
-                                                  const int32_t* counts, u32x4* dst) {
-  const int g = blockIdx.y, chunks = (cols + 7) >> 3, live = count_of(counts, g, rows);
-  const int64_t first = (int64_t)blockIdx.x * 1024 + threadIdx.x;
-  if (live == 0) return;
-  src += g * stride;
-  dst += (int64_t)g * rows * chunks;
-  u32x4 v[4];
-  int64_t row[4];
-  int col[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t i = first + 256 * j;
-    row[j] = i / chunks;
-    col[j] = (int)(i - row[j] * chunks);
-    const int64_t r = row[j] < live ? row[j] : live - 1;
-    v[j] = load16(src + r * ld + min(col[j] * 8, cols - 8));
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int drop = max(0, col[j] * 8 + 8 - cols) * 16;  // bits that belong to the chunk before
-    uint64_t lo = v[j][0] | (uint64_t)v[j][1] << 32, hi = v[j][2] | (uint64_t)v[j][3] << 32;
-    lo = drop >= 64 ? hi : lo;
-    hi = drop >= 64 ? 0 : hi;
-    const int d = drop & 63;
-    lo = d ? lo >> d | hi << (64 - d) : lo;
-    hi >>= d;
-    if (row[j] < live)
-      dst[row[j] * chunks + col[j]] = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
-  }
 }
 
 constexpr int DZ_ROWS = 64;  // rows summed by one workgroup
@@ -476,52 +441,13 @@ bool plan(const mplc_dense_t& t, Form form, Plan& out) {
   return true;
 }
 
-// One model's matrix [rows][cols] of a batch, of which `cols` columns may be read.
-struct Matrix {
-  const void* p;
-  int64_t stride, ld;
-  int rows, cols;
-};
-
-// rows that 16-byte loads take
-template <Kind K> bool fits(const Matrix& m) {
+template <Kind K, bool AA, bool BA> hipError_t launch(Plan& pl, const Epilogue& e, hipStream_t s) {
   const int ch = K == F32 ? 4 : 8;
-  return ((uintptr_t)m.p & 15) == 0 && m.stride % ch == 0 && m.ld % ch == 0;
-}
-
-// Bytes of a padded copy of `models` 16-bit matrices; 0 where their rows are whole chunks.
-size_t pad_bytes(int models, int rows, int cols) {
-  return cols % 8 ? (size_t)models * rows * ((cols + 7) & ~7) * 2 : 0;
-}
-// Whether padded copies pay: products of 16-bit rows that are not aligned run at about 400 TFLOP/s, of aligned ones at
-// 900; a copy moves its bytes twice at 3.5 TB/s and is a launch more (3 us).
-bool pad_pays(const mplc_dense_t& t, size_t bytes, int copies, int products) {
-  if (t.dtype == MPLC_DTYPE_F32 || t.in < 8 || t.out < 8 || bytes == 0 || copies * (int64_t)t.n_models > (1 << 20)) return false;
-  const double flops = 2. * t.n_models * t.rows * (double)t.in * t.out * products;
-  return flops * (1. / 400e12 - 1. / 900e12) > bytes * 2 / 3.5e12 + copies * 3e-6;
-}
-hipError_t pad(Matrix& m, int models, const int32_t* counts, char*& ws, hipStream_t s) {
-  const int chunks = (m.cols + 7) / 8;
-  const dim3 grid((unsigned)ceil_div((int64_t)m.rows * chunks, 1024), (unsigned)models);
-  pad_kernel<<<grid, 256, 0, s>>>(reinterpret_cast<const uint16_t*>(m.p), m.stride, m.ld, m.rows, m.cols, counts,
-                                  reinterpret_cast<u32x4*>(ws));
-  m = Matrix{ws, models > 1 ? (int64_t)m.rows * chunks * 8 : 0, chunks * 8, m.rows, chunks * 8};
-  ws += (size_t)models * m.rows * chunks * 16;
-  return hipGetLastError();
-}
-
-template <Kind K, bool AA, bool BA>
-hipError_t launch(Plan& pl, const Matrix& a, const Matrix& b, const Epilogue& e, hipStream_t s) {
-  const int ch = K == F32 ? 4 : 8;
-  pl.p.a = a.p;
-  pl.p.a_stride = a.stride;
-  pl.p.a_ld = a.ld;
-  pl.p.a_cols = a.cols;
-  pl.p.b = b.p;
-  pl.p.b_stride = b.stride;
-  pl.p.b_ld = b.ld;
-  pl.p.b_cols = b.cols;
-  pl.p.aligned = fits<K>(a) && fits<K>(b) && (!AA || a.cols % ch == 0) && (!BA || b.cols % ch == 0);
+  auto fits = [&](const void* base, int64_t stride, int64_t ld) {
+    return ((uintptr_t)base & 15) == 0 && stride % ch == 0 && ld % ch == 0;
+  };
+  pl.p.aligned = fits(pl.p.a, pl.p.a_stride, pl.p.a_ld) && fits(pl.p.b, pl.p.b_stride, pl.p.b_ld) &&
+                 (!AA || pl.p.m % ch == 0) && (!BA || pl.p.b_cols % ch == 0);
   const dim3 grid((unsigned)pl.blocks);
   if (pl.cfg == 6) {
     if constexpr (!AA && BA) {  // the forward product
@@ -555,25 +481,9 @@ bool sizes_ok(const mplc_dense_t& t) {
 // a tensor of [models][rows][cols]: rows may not overlap one another
 bool view_ok(const void* p, int64_t ld, int cols) { return p != nullptr && ld >= cols; }
 
-// The workspace of a forward call: partial sums, padded x, padded w.
-struct ForwardSpace {
-  Plan plan;
-  size_t partial, pad, total;  // pad: 0 where the product takes its operands as they are
-};
-
-bool forward_space(const mplc_dense_t& t, ForwardSpace& s) {
-  s = ForwardSpace{};
-  if (!plan(t, FORWARD, s.plan)) return false;
-  s.partial = align16(s.plan.partial_bytes);
-  const size_t x = pad_bytes(t.x_shared ? 1 : t.n_models, t.rows, t.in), w = pad_bytes(t.n_models, t.in, t.out);
-  if (s.plan.cfg != 6 && pad_pays(t, x + w, (x > 0) + (w > 0), 1)) s.pad = x + w;
-  s.total = s.partial + s.pad;
-  return true;
-}
-
 struct BackwardSpace {
   Plan dx, dw;
-  size_t dz, sums, partial, pad, total;
+  size_t dz, sums, partial, total;
   int dz_ld, blocks;
 };
 
@@ -595,28 +505,23 @@ bool backward_space(const mplc_dense_t& t, BackwardSpace& s) {
     partial = partial > s.dw.partial_bytes ? partial : s.dw.partial_bytes;
   }
   s.partial = align16(partial);  // dx's partial sums are joined before dw's are written: one place for both
-  const size_t w = t.dx ? pad_bytes(t.n_models, t.in, t.out) : 0, x = t.dw ? pad_bytes(t.x_shared ? 1 : t.n_models, t.rows, t.in) : 0;
-  const size_t dy = (t.dx || t.dw) && t.activation == MPLC_ACT_NONE ? pad_bytes(t.n_models, t.rows, t.out) : 0;
-  if (pad_pays(t, x + w + dy, (x > 0) + (w > 0) + (dy > 0), (t.dx != nullptr) + (t.dw != nullptr))) s.pad = x + w + dy;
-  s.total = s.dz + s.sums + s.partial + s.pad;
+  s.total = s.dz + s.sums + s.partial;
   return s.blocks <= (1 << 23) && ceil_div(t.out, 256) <= 65535;  // the grid of dz_kernel
 }
 
-template <Kind K> int forward(const mplc_dense_t& t, ForwardSpace& sp, hipStream_t s) {
-  Matrix x = {t.x, t.x_shared ? 0 : t.x_stride, t.x_ld, t.rows, t.in}, w = {t.w, t.w_stride, t.w_ld, t.in, t.out};
-  sp.plan.p.partial = reinterpret_cast<float*>(t.workspace);
-  if (sp.pad) {
-    char* ws = reinterpret_cast<char*>(t.workspace) + sp.partial;
-    const bool pad_x = x.cols % 8 && !fits<K>(x), pad_w = w.cols % 8 != 0;
-    hipError_t err;
-    if ((pad_x || fits<K>(x)) && (pad_w || fits<K>(w))) {  // both operands will be aligned
-      if (pad_x && (err = pad(x, t.x_shared ? 1 : t.n_models, t.x_shared ? nullptr : t.counts, ws, s)) != hipSuccess) return (int)err;
-      if (pad_w && (err = pad(w, t.n_models, nullptr, ws, s)) != hipSuccess) return (int)err;
-    }
-  }
+template <Kind K> int forward(const mplc_dense_t& t, const Plan& pl0, hipStream_t s) {
+  Plan pl = pl0;
+  pl.p.a = t.x;
+  pl.p.a_stride = t.x_shared ? 0 : t.x_stride;
+  pl.p.a_ld = t.x_ld;
+  pl.p.b = t.w;
+  pl.p.b_stride = t.w_stride;
+  pl.p.b_ld = t.w_ld;
+  pl.p.b_cols = pl.p.n;
+  pl.p.partial = reinterpret_cast<float*>(t.workspace);
   Epilogue e = {t.bias, t.bias_stride, t.residual, t.residual_stride, t.residual_ld, t.y, t.y_stride, t.y_ld,
                 t.z, t.z_stride, t.z_ld, t.activation};
-  return (int)launch<K, false, true>(sp.plan, x, w, e, s);
+  return (int)launch<K, false, true>(pl, e, s);
 }
 
 template <Kind K> int backward(const mplc_dense_t& t, BackwardSpace& sp, hipStream_t s) {
@@ -624,7 +529,6 @@ template <Kind K> int backward(const mplc_dense_t& t, BackwardSpace& sp, hipStre
   void* dz = sp.dz ? ws : nullptr;
   float* sums = sp.sums ? reinterpret_cast<float*>(ws + sp.dz) : nullptr;
   float* partial = reinterpret_cast<float*>(ws + sp.dz + sp.sums);
-  ws += sp.dz + sp.sums + sp.partial;
   hipError_t err;
   if (dz || t.db) {
     const int lanes = t.out > 128 ? 64 : t.out > 64 ? 32 : 16;
@@ -643,34 +547,38 @@ template <Kind K> int backward(const mplc_dense_t& t, BackwardSpace& sp, hipStre
       if ((err = hipGetLastError()) != hipSuccess) return (int)err;
     }
   }
-  Matrix d = {t.dy, t.dy_stride, t.dy_ld, t.rows, t.out}, x = {t.x, t.x_shared ? 0 : t.x_stride, t.x_ld, t.rows, t.in},
-         w = {t.w, t.w_stride, t.w_ld, t.in, t.out};
-  if (dz) d = Matrix{dz, (int64_t)t.rows * sp.dz_ld, sp.dz_ld, t.rows, sp.dz_ld};
-  if (sp.pad && t.rows > 0) {
-    // each product gets its copies where they make both operands aligned: w for dx, x for dw, dy for both
-    const bool d_fits = d.cols % 8 || fits<K>(d);
-    const bool for_dx = t.dx && d_fits && (w.cols % 8 || fits<K>(w)), for_dw = t.dw && d_fits && (x.cols % 8 || fits<K>(x));
-    if (d.cols % 8 && (for_dx || for_dw) && (err = pad(d, t.n_models, t.counts, ws, s)) != hipSuccess) return (int)err;
-    if (for_dx && w.cols % 8 && !fits<K>(w) && (err = pad(w, t.n_models, nullptr, ws, s)) != hipSuccess) return (int)err;
-    if (for_dw && x.cols % 8 &&
-        (err = pad(x, t.x_shared ? 1 : t.n_models, t.x_shared ? nullptr : t.counts, ws, s)) != hipSuccess)
-      return (int)err;
-  }
+  const void* d = dz ? dz : t.dy;
+  const int64_t d_stride = dz ? (int64_t)t.rows * sp.dz_ld : t.dy_stride, d_ld = dz ? sp.dz_ld : t.dy_ld;
   if (t.dx && t.rows > 0) {
-    sp.dx.p.partial = partial;
+    Plan& pl = sp.dx;
+    pl.p.a = d;
+    pl.p.a_stride = d_stride;
+    pl.p.a_ld = d_ld;
+    pl.p.b = t.w;
+    pl.p.b_stride = t.w_stride;
+    pl.p.b_ld = t.w_ld;
+    pl.p.partial = partial;
     Epilogue e = {};
     e.out = t.dx;
     e.out_stride = t.x_shared ? 0 : t.dx_stride;
     e.out_ld = t.dx_ld;
-    if ((err = launch<K, false, false>(sp.dx, d, w, e, s)) != hipSuccess) return (int)err;
+    if ((err = launch<K, false, false>(pl, e, s)) != hipSuccess) return (int)err;
   }
   if (t.dw) {
-    sp.dw.p.partial = partial;
+    Plan& pl = sp.dw;
+    pl.p.a = t.x;
+    pl.p.a_stride = t.x_shared ? 0 : t.x_stride;
+    pl.p.a_ld = t.x_ld;
+    pl.p.b_cols = dz ? sp.dz_ld : pl.p.n;
+    pl.p.b = d;
+    pl.p.b_stride = d_stride;
+    pl.p.b_ld = d_ld;
+    pl.p.partial = partial;
     Epilogue e = {};
     e.out = t.dw;
     e.out_stride = t.dw_stride;
     e.out_ld = t.dw_ld;
-    if ((err = launch<K, true, true>(sp.dw, x, d, e, s)) != hipSuccess) return (int)err;
+    if ((err = launch<K, true, true>(pl, e, s)) != hipSuccess) return (int)err;
   }
   return MPLC_OK;
 }
@@ -678,9 +586,9 @@ template <Kind K> int backward(const mplc_dense_t& t, BackwardSpace& sp, hipStre
 }  // namespace
 
 extern "C" size_t mplc_dense_forward_workspace_bytes(const mplc_dense_t* t) {
-  ForwardSpace s;
-  if (t == nullptr || !sizes_ok(*t) || !forward_space(*t, s)) return 0;
-  return s.total;
+  Plan pl;
+  if (t == nullptr || !sizes_ok(*t) || !plan(*t, FORWARD, pl)) return 0;
+  return pl.partial_bytes;
 }
 
 extern "C" size_t mplc_dense_backward_workspace_bytes(const mplc_dense_t* t) {
@@ -695,14 +603,14 @@ extern "C" int mplc_dense_forward(const mplc_dense_t* t, void* stream) {
   if (!view_ok(t->x, t->x_ld, t->in) || !view_ok(t->w, t->w_ld, t->out) || !view_ok(t->y, t->y_ld, t->out))
     return MPLC_E_ARG;
   if ((t->residual && t->residual_ld < t->out) || (t->z && t->z_ld < t->out)) return MPLC_E_ARG;
-  ForwardSpace sp;
-  if (!forward_space(*t, sp)) return MPLC_E_SHAPE;
-  if (sp.total && (t->workspace == nullptr || t->workspace_bytes < sp.total)) return MPLC_E_WORKSPACE;
+  Plan pl;
+  if (!plan(*t, FORWARD, pl)) return MPLC_E_SHAPE;
+  if (pl.partial_bytes && (t->workspace == nullptr || t->workspace_bytes < pl.partial_bytes)) return MPLC_E_WORKSPACE;
   if (((uintptr_t)t->workspace & 15) != 0) return MPLC_E_ARG;
   hipStream_t s = (hipStream_t)stream;
-  if (t->dtype == MPLC_DTYPE_F32) return forward<F32>(*t, sp, s);
-  if (t->dtype == MPLC_DTYPE_BF16) return forward<BF16>(*t, sp, s);
-  return forward<F16>(*t, sp, s);
+  if (t->dtype == MPLC_DTYPE_F32) return forward<F32>(*t, pl, s);
+  if (t->dtype == MPLC_DTYPE_BF16) return forward<BF16>(*t, pl, s);
+  return forward<F16>(*t, pl, s);
 }
 
 extern "C" int mplc_dense_backward(const mplc_dense_t* t, void* stream) {

@@ -11,7 +11,8 @@
 //
 // One workgroup computes a BM x BN tile over tiles of r, BKB bytes of an operand "along r" long.  Where the operands'
 // rows are 16-byte aligned their tiles go from memory into LDS directly (global_load_lds, no registers), in a ring of
-// STAGES tiles, whose loads run ahead by STAGES - 1 tiles; one barrier per tile.  Other operands, and the last tile of an r that no tile divides, go through registers.
+// STAGES tiles, whose loads run ahead by STAGES - 1 tiles; one barrier per tile.  Other operands, and the last tile of an
+// r that no tile divides, go through registers.
 //
 // LDS.  A tile is a sequence of 16-byte chunks, row by row; which chunk of a row is at which place is exchanged by row
 // (XOR), so that the rows that one pass of a read touches fall on different banks: along r, the 16 rows of a
@@ -92,6 +93,17 @@ template <Kind K> __device__ __forceinline__ u32x4 load16_edge(const typename El
       if (e < n) r[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
   }
   return r;
+}
+
+// a chunk's elements from place n on, at the front, zeros behind them
+template <typename T> __device__ __forceinline__ u32x4 drop_front(u32x4 v, int n) {
+  const int bits = n * (int)sizeof(T) * 8, d = bits & 63;
+  uint64_t lo = v[0] | (uint64_t)v[1] << 32, hi = v[2] | (uint64_t)v[3] << 32;
+  lo = bits & 64 ? hi : lo;
+  hi = bits & 64 ? 0 : hi;
+  lo = d ? lo >> d | hi << (64 - d) : lo;
+  hi >>= d;
+  return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
 }
 
 // 4 consecutive elements starting at p, n >= 1 of them valid, the others 0, without a branch: the compiler waits for what
@@ -196,7 +208,8 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
   }
 
   // Points at the tile of rows [i0, i0 + BT) and r = r0 ...  Rows behind o.rows (never stored) repeat the last one, so
-  // that only the end of r needs checks; chunks of columns across r behind o.rows read the row's first ones.
+  // that only the end of r needs checks; chunks of columns across r behind o.rows read the row's first ones, and a chunk
+  // that o.rows cuts is read from where it ends at the row's end.
   __device__ __forceinline__ void seek(const Operand<T>& o, int i0, int r0, int tid) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
@@ -206,7 +219,7 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
       if constexpr (ACROSS) {
         const int i = i0 + ch * CH;
         live[j] = o.rows - i;
-        off = (int64_t)(r0 + row) * o.ld + (live[j] > 0 ? column(i) : 0);
+        off = (int64_t)(r0 + row) * o.ld + (live[j] > 0 ? column(i) : 0) - (o.rows >= CH ? behind(j) : 0);
       } else {
         off = (int64_t)min(i0 + row, o.rows - 1) * o.ld + column(r0 + ch * CH);
       }
@@ -214,6 +227,8 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
       for (int p = 0; p < PL; ++p) ptr[p][j] = o.p + off + 32 * p;
     }
   }
+  // ACROSS: elements of the chunk that are not there
+  __device__ __forceinline__ int behind(int j) const { return live[j] > 0 && live[j] < CH ? CH - live[j] : 0; }
   __device__ __forceinline__ void advance(int64_t ld) {
 #pragma unroll
     for (int p = 0; p < PL; ++p)
@@ -232,27 +247,66 @@ template <Kind K, bool ACROSS, int BT, int BKB, int NT, int PL> struct Tile {
       for (int j = 0; j < PER; ++j)
         __builtin_amdgcn_global_load_lds((glb_u32*)ptr[p][j], (lds_u32*)(lds + p * PLANE_BYTES + (j * NT + (tid & ~63)) * 16), 16, 0, 0);
   }
-  // the tile at ptr, of which `left` r are valid (left >= BK: all); `whole`: no chunk of columns is cut (uniform); rows
-  // at or behind `rows` contribute nothing
+  // the tile at ptr, of which `left` r are valid (left >= BK: all); columns (ACROSS, uniform): WHOLE, no chunk of them is
+  // cut; CUT, one may be; FEW, there are fewer than a chunk's; rows at or behind `rows` contribute nothing
+  enum Columns { WHOLE, CUT, FEW };
+  static __device__ __forceinline__ Columns columns(int i0, int rows) {
+    return !ACROSS || i0 + BT <= rows || rows % CH == 0 ? WHOLE : rows >= CH ? CUT : FEW;
+  }
   struct Regs {
     u32x4 v[PL][PER];
   };
-  __device__ __forceinline__ void load(Regs& reg, int left, bool whole, int i0, int rows, bool drop, int tid) const {
-    if (left >= BK && (!ACROSS || whole)) {
+  // ld, rend: of the operand; where the tile is cut, every load still is one of whole chunks that ends inside the operand,
+  // without a branch (the compiler waits for what each branch has loaded, one latency after the other: forward of 24 x 128
+  // rows, 1001 -> 1027 bf16, 28 us against 55 with cut chunks loaded by elements)
+  __device__ __forceinline__ void load(Regs& reg, int left, Columns cols, int64_t ld, int rend, int i0, int rows, bool drop,
+                                       int tid) const {
+    if (left >= BK && cols != FEW) {
 #pragma unroll
       for (int p = 0; p < PL; ++p)
 #pragma unroll
         for (int j = 0; j < PER; ++j) reg.v[p][j] = load16(ptr[p][j]);
+    } else if (ACROSS ? cols != FEW : rend >= CH) {
+      // along r: a chunk that r's end cuts, or that lies behind it, is read from where it ends there; across r: rows
+      // behind the end read the last one
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        int row, ch;
+        place(j, tid, row, ch);
+        const int64_t back = ACROSS ? (row < left ? 0 : (row - left + 1) * ld) : max(0, CH - (left - ch * CH));
+#pragma unroll
+        for (int p = 0; p < PL; ++p) reg.v[p][j] = load16(ptr[p][j] - back);
+      }
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        int row, ch;
+        place(j, tid, row, ch);
+        const int n = left - ch * CH;
+        const bool there = ACROSS ? row < left : n > 0;
+#pragma unroll
+        for (int p = 0; p < PL; ++p) {
+          u32x4 v = reg.v[p][j];
+          if constexpr (!ACROSS) v = drop_front<T>(v, n > 0 && n < CH ? CH - n : 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) reg.v[p][j][e] = there ? v[e] : 0;
+        }
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         int row, ch;
         place(j, tid, row, ch);
-        const int n = ACROSS ? (row < left ? (live[j] > 0 ? live[j] : (whole ? CH : 0)) : 0) : left - ch * CH;
+        const int n = ACROSS ? (row < left ? live[j] : 0) : left - ch * CH;
 #pragma unroll
         for (int p = 0; p < PL; ++p) reg.v[p][j] = load16_edge<K>(ptr[p][j], n);
       }
     }
+    if constexpr (ACROSS)
+      if (cols == CUT)
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+#pragma unroll
+          for (int p = 0; p < PL; ++p) reg.v[p][j] = drop_front<T>(reg.v[p][j], behind(j));
     if constexpr (!ACROSS)
       if (drop)
 #pragma unroll
@@ -449,8 +503,8 @@ struct Block {
     auto load_cut = [&]() {
       ta.seek(A, m0, cut, tid);
       tb.seek(B, n0, cut, tid);
-      ta.load(ra, rend - cut, true, m0, 0, false, tid);
-      tb.load(rb, rend - cut, true, n0, 0, false, tid);
+      ta.load(ra, rend - cut, TA::WHOLE, A.ld, rend, m0, 0, false, tid);
+      tb.load(rb, rend - cut, TB::WHOLE, B.ld, rend, n0, 0, false, tid);
     };
     if (EARLY && cut < rend) load_cut();
     if (n > 0)
@@ -538,18 +592,19 @@ struct Block {
     typename TB::Regs rb;
     Operand<T> A, B;
     int r0, rend, rows, s = (int)(from / n), t = (int)(from - (int64_t)s * n);
-    bool whole_a, whole_b;
+    typename TA::Columns cols_a;
+    typename TB::Columns cols_b;
     auto seek = [&]() {
       rows = at(s, A, B, r0, rend);
       ta.seek(A, m0, r0 + t * BK, tid);
       tb.seek(B, n0, r0 + t * BK, tid);
-      whole_a = m0 + BM <= A.rows || A.rows % TA::CH == 0;
-      whole_b = n0 + BN <= B.rows || B.rows % TB::CH == 0;
+      cols_a = TA::columns(m0, A.rows);
+      cols_b = TB::columns(n0, B.rows);
     };
     auto load = [&]() {
       const int left = rend - r0 - t * BK;
-      ta.load(ra, left, whole_a, m0, rows, rows < min(A.rows, m0 + BM), tid);
-      tb.load(rb, left, whole_b, n0, 0, false, tid);
+      ta.load(ra, left, cols_a, A.ld, rend, m0, rows, rows < min(A.rows, m0 + BM), tid);
+      tb.load(rb, left, cols_b, B.ld, rend, n0, 0, false, tid);
     };
     seek();
     load();
@@ -591,8 +646,8 @@ struct Block {
   }
 
   // f(m, n, v, x): 4 consecutive columns n .. n + 3 of row m, neighbouring lanes at neighbouring columns, 32 FN of a row,
-  // through the wave's own part of LDS (which run() has left): stores cover whole lines.  pre(m, n) loads what f(m, n, v, x) adds, for all rows of a pass before
-  // any of them is stored.
+  // through the wave's own part of LDS (which run() has left): stores cover whole lines.  pre(m, n) loads what f adds, for
+  // all rows of a pass before any of them is stored.
   template <typename P, typename F> __device__ __forceinline__ void each_row(char* lds, int m0, int n0, P pre, F f) const {
     constexpr int LD = 32 * FN + 4;  // floats; the rows one pass writes fall on different banks
     constexpr int PERROW = 8 * FN, ROWS = 64 / PERROW, N = 32 / ROWS;

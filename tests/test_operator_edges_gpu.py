@@ -191,8 +191,8 @@ def padded(x):
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("K,N", [(1001, 1003), (1001, 1000), (1008, 1003)])
 def test_large_products_of_cut_rows(K, N, dtype):
-    """Large enough that operands are copied to padded rows: ragged batches with NaN behind the counts, operands shared by
-    the models or repeated for each, aligned rows with NaN behind their last column, a base that no copy makes aligned."""
+    """Large tiles at odd borders: ragged batches with NaN behind the counts, operands shared by the models or repeated for
+    each, aligned rows with NaN behind their last column, a base that is not aligned."""
     t = TYPES[dtype]
     G, B = 3, 2500
     counts = torch.tensor([2500, 0, 2311], dtype=torch.int32, device="cuda")
