@@ -784,7 +784,7 @@ template <Kind K, int KP, bool TALL> __global__ __launch_bounds__(GRAM_THREADS) 
   __shared__ __attribute__((aligned(16))) char lds[BYTES > SUM ? BYTES : SUM];
   __shared__ float most[GRAM_THREADS / 64];
   const int g = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 63;
-  const int begin = chunk * p.rows_per, end = min(p.L, begin + p.rows_per);
+  const int begin = chunk * p.rows_per, end = begin + min(p.L - begin, p.rows_per);  // no sum passes L
   Pc pc;
   Gt gt;
   gt.init();
@@ -876,7 +876,7 @@ __global__ __launch_bounds__(NARROW_THREADS) void narrow_apply_kernel(const Narr
   __shared__ __attribute__((aligned(16))) char lds[2 * QB + (REST > SUM ? REST : SUM)];
   char* const xs = lds + 2 * QB;
   const int g = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int begin = chunk * p.rows_per, end = min(p.L, begin + p.rows_per);
+  const int begin = chunk * p.rows_per, end = begin + min(p.L - begin, p.rows_per);  // no sum passes L
   const int wr = KP == 128 ? wave >> 1 : wave, wc = KP == 128 ? wave & 1 : 0;  // 32 rows l, 64 columns
   const double inv = p.inv[g] * (double)X_SCALE;
   const float back = GRAM ? 1.f / p.q_scale : 1.f / (X_SCALE * p.q_scale);

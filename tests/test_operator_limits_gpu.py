@@ -1,0 +1,39 @@
+"""GPU: the batched operators at the ends of what they accept - the longest matrices, inputs that no model reaches, the
+tails of the activations, results as the exact parts of one buffer."""
+import pytest
+import torch
+
+from mplc import muon
+
+pytestmark = pytest.mark.gpu
+
+
+def test_longest_row():
+    """A 1 x L matrix whose last chunk of columns ends less than a chunk below 2^31.  k = 1: O(u) = u / |u| times the number
+    that five steps make of 1.  A sum of squares is fp32, each partial sum at most 3 * 2^16 additions long (4194304 columns,
+    16 a matrix instruction, 4 waves, 3 instructions each): off by less than 3 * 2^16 * 2^-24 = 1.2 %.  Such errors of both
+    phases' sums change the result by at most 2 % (the recurrence with sums off by 1.2 % up or down); its rounding is 2^-9.  X = u / |u| is held
+    in two fp16 numbers at a scale of 2^14, whose last place is 2^-24: off by at most half of that, 2^-39 of |u|, which shows
+    where u itself is below 2^-24 or so of |u|; X Q1 Q2 multiplies that by less than 1."""
+    L = 2147400000
+    u = torch.empty(1, L, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    square = 0.0
+    for i in range(0, L, 1 << 28):
+        part = u[0, i:i + (1 << 28)]
+        part.copy_(torch.randn(part.numel(), device="cuda", generator=g, dtype=torch.bfloat16))
+        square += float(part.double().square_().sum())
+    out = torch.zeros_like(u)
+    assert muon.orthogonalize(u, out=out) is out
+    s = 1.0
+    a, b, c = muon.COEFFICIENTS
+    for _ in range(5):
+        s = s * (a + s * s * (b + s * s * c))
+    for i in (0, 1 << 30, 511 * 4194304 - 5, 511 * 4194304, L - (1 << 21), L - 1):
+        part = slice(i, min(L, i + (1 << 20)))
+        want = u[0, part].double() * (s / square ** 0.5)
+        assert ((out[0, part].double() - want).abs() <= (0.02 + 2.0 ** -9) * want.abs() + 2.0 ** -39).all(), i
+    # every column is written: no zero but where |u| is below 2^-39 of |U|, as above
+    for i in range(0, L, 1 << 28):
+        part = slice(i, min(L, i + (1 << 28)))
+        assert not ((out[0, part] == 0) & (u[0, part].abs() > square ** 0.5 * 2.0 ** -39)).any(), i
