@@ -40,7 +40,8 @@ struct Product {
   const void* b;
   int64_t b_stride, b_ld;
   int m, n, r;           // sizes of one model's product
-  int models, segments;  // segments > 1: one product, r runs over (model, r)
+  int models, segments;
+  int joined;            // one product, r runs over (segments, r): counts limit a segment's rows, every row is written
   const int32_t* counts;
   int count_is_r;        // counts limit r (dw), not m
   int tiles_m, tiles_n, nk, splits, per_split;  // nk: units of r; per_split: units of a split
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
   b /= tiles;
   const int split = (int)(b % p.splits), g = (int)(b / p.splits);
   const int m0 = tm * B::BM, n0 = tn * B::BN;
-  const bool seg = p.segments > 1;
+  const bool seg = p.joined;
   const int cnt = seg ? p.m : count_of(p.counts, g, p.count_is_r ? p.r : p.m);
   const int M = p.count_is_r ? p.m : cnt, R = p.count_is_r ? cnt : p.r;
   if (m0 >= M) return;
@@ -273,7 +274,7 @@ template <Kind K> __global__ __launch_bounds__(256) void join_kernel(const Produ
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (t >= (int64_t)p.m * n4) return;
   const int g = blockIdx.y, m = (int)(t / n4), n = (int)(t % n4) * 4;
-  if (!p.count_is_r && p.segments == 1 && m >= count_of(p.counts, g, p.m)) return;
+  if (!p.count_is_r && !p.joined && m >= count_of(p.counts, g, p.m)) return;
   const float* src = p.partial + (int64_t)g * p.m * p.n + (int64_t)m * p.n + n;
   const int64_t step = (int64_t)p.models * p.m * p.n;
   by_width(p.n, [&](auto wide) {
@@ -400,6 +401,7 @@ bool plan(const mplc_dense_t& t, Form form, Plan& out) {
   const bool shared_dx = form == DX && t.x_shared;
   p.models = shared_dx ? 1 : t.n_models;
   p.segments = shared_dx ? t.n_models : 1;
+  p.joined = shared_dx && (t.n_models > 1 || t.counts);  // a row behind one model's count gets 0 like any that none reaches
   p.m = form == DW ? t.in : t.rows;
   p.n = form == DX ? t.in : t.out;
   p.r = form == FORWARD ? t.in : form == DX ? t.out : t.rows;

@@ -354,4 +354,6 @@ def dense_backward(dout, x, w, preact=None, activation="none", counts=None, need
         db = torch.empty((G, w.shape[2]), dtype=w.dtype, device=w.device)
     if G and need:
         plan.run((dx, dw, db, x, w, dout, preact, counts), _BACKWARD)
+    elif dx is not None:
+        dx.zero_()  # the sum over no models
     return dx, dw, db

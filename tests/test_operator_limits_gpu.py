@@ -3,7 +3,8 @@ tails of the activations, results as the exact parts of one buffer."""
 import pytest
 import torch
 
-from mplc import muon
+from mplc import dense, muon
+from test_dense_gpu import TYPES, check_backward, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +38,25 @@ def test_longest_row():
     for i in range(0, L, 1 << 28):
         part = slice(i, min(L, i + (1 << 28)))
         assert not ((out[0, part] == 0) & (u[0, part].abs() > square ** 0.5 * 2.0 ** -39)).any(), i
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("B,K,N", [(70, 33, 45), (40, 64, 128), (5, 40, 9000), (300, 264, 520)])
+def test_shared_rows_that_no_model_reaches(B, K, N, dtype):
+    """One model behind its count, and no model at all: such rows of a given dx get 0, as with several models."""
+    t = TYPES[dtype]
+    x, w = rand((B, K), t, 1), rand((1, K, N), t, 2, 0.2)
+    for n in (B - 3, 0):
+        counts = torch.tensor([n], dtype=torch.int32, device="cuda")
+        dout = rand((1, B, N), t, 3)
+        dout[:, n:] = float("nan")
+        for act in ("none", "silu"):
+            pre = rand((1, B, N), torch.float32, 4)
+            dx = torch.full_like(x, 5.0)
+            gx, _, _ = check_backward(dout, x, w, pre, act, counts, dx=dx)
+            assert gx is dx and (dx[n:] == 0).all()
+    for shape in ((B, K), (1, B, K)):
+        dx = torch.full(shape, 5.0, dtype=t, device="cuda")
+        none = torch.empty(0, K, N, dtype=t, device="cuda")
+        gx, _, _ = dense.dense_backward(torch.empty(0, B, N, dtype=t, device="cuda"), x.view(shape), none, dx=dx)
+        assert gx is dx and (dx == 0).all()
