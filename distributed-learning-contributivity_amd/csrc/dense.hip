@@ -56,38 +56,54 @@ __device__ __forceinline__ int count_of(const int32_t* counts, int g, int most) 
   return c < 0 ? 0 : (c > most ? most : c);
 }
 
-// Standard normal: the probability of values below z and its density.  The tail below -|z| is half of
-// erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), x = |z| / sqrt 2 (Abramowitz and Stegun 7.1.26, off by at
-// most 1.5e-7): a tenth of erff's instructions, and the exponential is the density's.
-__device__ __forceinline__ float normal(float z, float& density) {
-  const float x = fabsf(z) * 0.70710678118654752f;
-  const float e = __expf(-x * x);
-  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
-  const float tail = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+// Standard normal: the probability of values below z and its density.  The tail below -|z| is exp(-z^2 / 2) t (c0 + c1 t + ..
+// + c8 t^8) with t = 1 / (1 + 0.28 |z|): the coefficients were fitted here to the least relative error over |z| <= 64
+// (9.1e-8), so that gelu keeps its digits far in the negative tail, where an error that is small beside 1 alone would be larger
+// than the result.  In fp32 the square and its product with log2(e) / 2 are carried in two parts, as their rounding would be
+// multiplied by z^2: relative error of the tail 4.2e-7, and 7.5e-6 without (enough for 16-bit results).
+template <Kind K> __device__ __forceinline__ float normal(float z, float& density) {
+  const float a = fminf(fabsf(z), 64.f), s = a * a;
+  float e;
+  if constexpr (K == F32) {
+    constexpr double L = 0.72134752044448170;
+    const float h = s * (float)L;
+    const float l = __builtin_fmaf(__builtin_fmaf(a, a, -s), (float)L, __builtin_fmaf(s, (float)(L - (float)L), __builtin_fmaf(s, (float)L, -h)));
+    e = __builtin_amdgcn_exp2f(-h);
+    e = __builtin_fmaf(e, l * -0.69314718056f, e);
+  } else {
+    e = __expf(-0.5f * s);
+  }
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.28f, a, 1.f));
+  constexpr float c[9] = {0.11170406639575958f, 0.11169082671403885f, 0.10321412980556488f, 0.08275685459375381f, 0.07594385743141174f,
+                          -0.012980633415281773f, 0.10007699579000473f, -0.09832608699798584f, 0.02592002972960472f};
+  float q = c[8];
+#pragma unroll
+  for (int i = 7; i >= 0; --i) q = __builtin_fmaf(q, t, c[i]);
+  const float tail = e * t * q;
   density = 0.39894228040143268f * e;
   return z < 0.f ? tail : 1.f - tail;
 }
 
 // far in the negative tail the result is 0, at -infinity too
-__device__ __forceinline__ float activate(int act, float z) {
+template <Kind K> __device__ __forceinline__ float activate(int act, float z) {
   switch (act) {
     case MPLC_ACT_RELU: return z < 0.f ? 0.f : z;
     case MPLC_ACT_GELU: {
       float density;
-      const float p = normal(z, density);
+      const float p = normal<K>(z, density);
       return z < -64.f ? 0.f : z * p;
     }
     case MPLC_ACT_SILU: return z < -1e4f ? 0.f : z / (1.f + __expf(-z));
     default: return z;
   }
 }
-__device__ __forceinline__ float slope(int act, float z) {
+template <Kind K> __device__ __forceinline__ float slope(int act, float z) {
   switch (act) {
     case MPLC_ACT_RELU: return z > 0.f ? 1.f : 0.f;
     case MPLC_ACT_GELU: {
       if (fabsf(z) > 64.f) return z > 0.f ? 1.f : 0.f;
       float density;
-      const float p = normal(z, density);
+      const float p = normal<K>(z, density);
       return p + z * density;
     }
     case MPLC_ACT_SILU: {
@@ -117,7 +133,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int g, int m, int n, i
   if (e.z) store4<F32>(e.z + g * e.z_stride + m * e.z_ld + n, v, valid);
   if (e.act != MPLC_ACT_NONE)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = activate(e.act, v[i]);
+    for (int i = 0; i < 4; ++i) v[i] = activate<K>(e.act, v[i]);
   if (e.res) v += res;
   store4<K>(reinterpret_cast<T*>(e.out) + g * e.out_stride + m * e.out_ld + n, v, valid);
 }
@@ -330,7 +346,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const void* dy_, int64_t dy_str
           if (r + STEP * i < r1) {
             if (act != MPLC_ACT_NONE) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) d[i][e] *= slope(act, zz[i][e]);
+              for (int e = 0; e < 4; ++e) d[i][e] *= slope<K>(act, zz[i][e]);
               if (dz) store4<K>(dz + (int64_t)(r + STEP * i) * dz_ld + c, d[i], n - c);
             }
             sum += d[i];

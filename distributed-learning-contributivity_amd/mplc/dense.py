@@ -258,7 +258,7 @@ def dense_forward(x, w, bias=None, residual=None, activation="none", counts=None
     """act(x @ w + bias) + residual for every model of the batch.
 
     x [G, B, K], or [1, B, K] / [B, K] shared by all models; w [G, K, N]; bias [G, N]; residual [G, B, N]; all of one
-    type.  activation: "none", "relu", "gelu" (exact) or "silu".  counts (int32 [G], on the device): rows of each model's
+    type.  activation: "none", "relu", "gelu" (of the error function) or "silu".  counts (int32 [G], on the device): rows of each model's
     batch (clamped to [0, B]); rows behind a model's count are not read, and those of `out` and `preact` stay as they
     are.  preact (float32 [G, B, N]): receives x @ w + bias, which dense_backward needs for an activation.
     Returns out [G, B, N] (allocated where not given; then rows behind a count are 0)."""

@@ -1,10 +1,12 @@
 """GPU: the batched operators at the ends of what they accept - the longest matrices, inputs that no model reaches, the
 tails of the activations, results as the exact parts of one buffer."""
+import math
+
 import pytest
 import torch
 
 from mplc import dense, muon
-from test_dense_gpu import TYPES, check_backward, rand
+from test_dense_gpu import TYPES, check_backward, half, rand, tiny
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +62,27 @@ def test_shared_rows_that_no_model_reaches(B, K, N, dtype):
         none = torch.empty(0, K, N, dtype=t, device="cuda")
         gx, _, _ = dense.dense_backward(torch.empty(0, B, N, dtype=t, device="cuda"), x.view(shape), none, dx=dx)
         assert gx is dx and (dx == 0).all()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("N", [20000, 20001])
+def test_gelu_keeps_its_digits_in_the_tail(N, dtype):
+    """z = 1 * w, exactly.  gelu: the documented relative error, 2^-19 in fp32 and 2^-16 for 16-bit results, and the rounding.
+    Its slope cdf + z density (db of one row, with dout = 1): for z <= -2 twice that (the two terms cancel by a factor of 1.6
+    at most), elsewhere 2^-20 as well.  Results below 2^-120 may be off by that."""
+    t = TYPES[dtype]
+    z = torch.linspace(-16.0, 8.0, N, dtype=torch.float64).to(t).cuda()
+    rel = 2.0 ** -19 if dtype == "fp32" else 2.0 ** -16
+    zd = z.double()
+    cdf = 0.5 * torch.erfc(-zd / math.sqrt(2))
+    one = torch.ones(1, 1, 1, dtype=t, device="cuda")
+    pre = torch.empty(1, 1, N, device="cuda")
+    y = dense.dense_forward(one, z.view(1, 1, N), activation="gelu", preact=pre)[0, 0]
+    assert torch.equal(pre[0, 0].double(), zd)
+    want = zd * cdf
+    err = rel * want.abs()
+    assert ((y.double() - want).abs() <= err + half(t) * (want.abs() + err) + tiny(t) + 2.0 ** -120).all()
+    _, _, db = dense.dense_backward(torch.ones(1, 1, N, dtype=t, device="cuda"), one, z.view(1, 1, N), preact=pre, activation="gelu")
+    want = cdf + zd * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi)
+    err = 2 * rel * want.abs() + torch.where(zd <= -2, 0.0, 2.0 ** -20)
+    assert ((db[0].double() - want).abs() <= err + half(t) * (want.abs() + err) + tiny(t) + 2.0 ** -120).all()
