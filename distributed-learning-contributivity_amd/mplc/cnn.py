@@ -630,8 +630,9 @@ class TrainBatch:
                       "mplc_fedavg_aggregate")
         self.eng.server_optimizer.apply(rows, before, self.server_m[c0:c0 + nc], self.model.KERAS_LAYERS)
         last = self.coal_first[c0 + nc]
-        self._rows_copy(self.params[r0:last], self.glob, [ci for ci in range(c0, c0 + nc)
-                                                          for _ in range(self.coal_first[ci], self.coal_first[ci + 1])])
+        _native.check(self.lib.mplc_cnn_copy_rows(_native.ptr(self.params[r0:last]), _native.ptr(self.glob), S,
+                                                  _native.ptr(self.src_map[r0:last]), last - r0, self.stream),
+                      "mplc_cnn_copy_rows")
 
     def snap_row(self, ci):
         return sum(len(self.coalitions[c]) for c in range(ci) if not self.coal_is_single[c])
