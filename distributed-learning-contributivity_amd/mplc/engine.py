@@ -49,7 +49,7 @@ class CoalitionEngine:
             raise NotImplementedError(f"multi-partner learning approach '{approach}' has no batched MI355X path")
         self.approach = approach
         # optimizer of the server after a FedAvg round's average (mplc.muon.ServerMuon): None takes the average
-        self.server_optimizer = None
+        self.server_optimizer = self._server_step = None
         if server_optimizer is not None:
             from .muon import ServerMuon
             if approach != "fedavg":
@@ -160,6 +160,16 @@ class CoalitionEngine:
     def replica_bytes(self, bmax):
         return self.model_impl.replica_bytes(bmax)
 
+    def server_bytes(self, coalitions):
+        """What the server optimizer adds to a lockstep batch of so many coalitions: each one's momentum and its row at the
+        round's start, and the step of one group at a time on every stream."""
+        if self.server_optimizer is None:
+            return 0
+        if self._server_step is None:
+            self._server_step = self.server_optimizer.step_bytes(self.model_impl.KERAS_LAYERS, self.model_impl.STRIDE)
+        most = self.concurrent_batches * self.server_optimizer.GROUP
+        return coalitions * 8 * self.model_impl.STRIDE + min(coalitions, most) * self._server_step
+
     def plan_batches(self, coalitions):
         """Split coalitions into lockstep batches that fit the HBM budget (cost-sorted so that a batch holds
         coalitions of similar size; every coalition's replicas stay together)."""
@@ -168,9 +178,8 @@ class CoalitionEngine:
         for i in order:
             c = coalitions[i]
             bmax = max(self.batch_sizes[p] for p in c)
-            # a coalition's row; with a server optimizer also its momentum, its start of the round and the difference
-            need = len(c) * self.replica_bytes(bmax) + self.model_impl.STRIDE * (4 if self.server_optimizer is None else 16)
-            if cur and (cur_bytes + need > self.memory_budget_bytes or len(cur) >= 65535):
+            need = len(c) * self.replica_bytes(bmax) + self.model_impl.STRIDE * 4
+            if cur and (cur_bytes + need + self.server_bytes(len(cur) + 1) > self.memory_budget_bytes or len(cur) >= 65535):
                 batches.append(cur)
                 cur, cur_bytes = [], 0
             cur.append(i)
@@ -218,7 +227,7 @@ class CoalitionEngine:
         import torch
         if self.concurrent_batches <= 1:
             return
-        need = sum(len(c) * self.replica_bytes(max(self.batch_sizes[p] for p in c)) for c in coal)
+        need = sum(len(c) * self.replica_bytes(max(self.batch_sizes[p] for p in c)) for c in coal) + self.server_bytes(len(coal))
         idle = torch.cuda.memory_reserved(self.device) - torch.cuda.memory_allocated(self.device)
         if idle > 0 and idle + need > self.memory_budget_bytes:
             self.release()

@@ -222,6 +222,16 @@ class ServerMuon:
         """(offset, rows, cols) of the matrices among a model row's layers (offset, shape)."""
         return [(off, math.prod(shape[:-1]), shape[-1]) for off, shape in layers if len(shape) > 1]
 
+    def step_bytes(self, layers, stride):
+        """Device memory that apply() takes for each of a group's models: their differences and the steps' workspaces (those of
+        different sizes side by side, as the allocator keeps a freed block for its size)."""
+        total = 4 * stride
+        for _, rows, cols in self.matrices(layers):
+            t = MuonT()
+            t.n_models, t.rows, t.cols, t.steps, t.invariant = self.GROUP, rows, cols, int(self.params["steps"]), 1
+            total += -(-_lib().mplc_muon_step_workspace_bytes(ctypes.byref(t)) // self.GROUP)
+        return total
+
     def apply(self, glob, before, momentum, layers):
         """glob, before, momentum [C, stride]: glob holds the round's averages and receives the new models; before, the
         models at the round's start, is used up."""
