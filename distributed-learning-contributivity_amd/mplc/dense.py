@@ -5,7 +5,8 @@
 for g over the models of a lockstep batch, beside the trainers' own dense layers (which are fixed to their two models):
 kernels are [in][out] as Keras keeps them and may be views into the models' parameter rows, e.g.
 ``params[:, off:off + k * n].view(G, k, n)``.  Types: float32, bfloat16, float16; sums are fp32.  Rows may have any
-stride; the elements of a row are contiguous.  Work goes to torch's current stream of the tensors' device.
+stride; the elements of a row are contiguous.  Work goes to torch's current stream of the tensors' device.  No autograd graph
+is recorded: in grad mode, tensors that require grad are refused.
 """
 import ctypes
 
@@ -80,6 +81,11 @@ class _Plan:
     def run(self, tensors, names, same=(), values=()):
         """Launch on torch's current stream.  same: pairs of positions that may be one and the same tensor; values:
         further fields of the struct."""
+        if torch.is_grad_enabled():
+            for t, name in zip(tensors, names):
+                if t is not None and t.requires_grad:
+                    raise ValueError(f"{name} requires grad, and the batched operators record no graph for it: call them under "
+                                     "torch.no_grad() or with detached tensors")
         p = [0 if t is None else t.data_ptr() for t in tensors]
         _no_overlap(tensors, names, p, self.spans, self.outs, self.ins, same)
         st = self.struct.from_buffer_copy(self.bytes)
@@ -98,6 +104,7 @@ class _Plan:
                 status = self.fn(ctypes.byref(st), _raw_stream(self.index))
         if status:
             _native.check(status, self.name)
+        torch.autograd.graph.increment_version([tensors[i] for i in self.outs])  # written behind torch's back
 
 
 def _raw_stream(index):

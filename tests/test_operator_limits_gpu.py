@@ -86,3 +86,37 @@ def test_gelu_keeps_its_digits_in_the_tail(N, dtype):
     want = cdf + zd * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi)
     err = 2 * rel * want.abs() + torch.where(zd <= -2, 0.0, 2.0 ** -20)
     assert ((db[0].double() - want).abs() <= err + half(t) * (want.abs() + err) + tiny(t) + 2.0 ** -120).all()
+
+
+def test_tensors_that_require_grad():
+    """No result without its graph: refused in grad mode, computed under no_grad; what a call overwrites is seen by a graph
+    that has saved it."""
+    x, w, d, pre = rand((2, 6, 8), torch.float32, 1), rand((2, 8, 10), torch.float32, 2), rand((2, 6, 10), torch.float32, 3), torch.empty(2, 6, 10, device="cuda")
+    want = dense.dense_forward(x, w, preact=pre)
+    m = torch.zeros_like(w)
+    calls = [lambda t: dense.dense_forward(t(x), w), lambda t: dense.dense_forward(x, t(w)), lambda t: dense.dense_forward(x, w, residual=t(d)),
+             lambda t: dense.dense_forward(x, w, out=t(d)), lambda t: dense.dense_backward(d, x, t(w)),
+             lambda t: dense.dense_backward(t(d), x, w), lambda t: dense.dense_backward(d, x, w, preact=t(pre), activation="silu"),
+             lambda t: muon.orthogonalize(t(w)), lambda t: muon.orthogonalize(t(w[0])), lambda t: muon.muon_step(t(w), w.clone(), m, lr=0.1),
+             lambda t: muon.muon_step(w.clone(), t(w), m, lr=0.1)]
+
+    def leaf(t):
+        return t.detach().clone().requires_grad_()
+    for f in calls:
+        with pytest.raises(ValueError, match="requires grad"):
+            f(leaf)
+        with torch.no_grad():
+            f(leaf)
+    with torch.no_grad():
+        assert torch.equal(dense.dense_forward(leaf(x), leaf(w)), want)
+    a = torch.ones(2, 8, 10, device="cuda", requires_grad=True)
+    for write in (lambda v: dense.dense_backward(d, x, w, need=("dw",), dw=v), lambda v: muon.muon_step(v, w.clone(), m, lr=0.1),
+                  lambda v: muon.muon_step(w.clone(), w.clone(), v, lr=0.1), lambda v: muon.orthogonalize(v, out=v),
+                  lambda v: muon.orthogonalize(w[0], out=v[0])):
+        v = w.clone()
+        loss = (a * v).sum()
+        write(v)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        assert torch.equal(dense.dense_forward(x, w, out=torch.empty(2, 6, 10, device="cuda")), want)
