@@ -165,23 +165,28 @@ def _no_overlap(tensors, names, ptrs, spans, outs, ins, same=()):
 
 
 def _interleaved(t, u):
-    """Views of the same parameter rows at different places of a row: the spans cross, the elements do not."""
-    if t.dim() < 2 or u.dim() < 2 or t.element_size() != u.element_size():
-        return False
-    s = t.stride(0)
-    if s <= 0 or s != u.stride(0) or t.shape[0] < 2 or u.shape[0] < 2:
+    """Views whose spans cross but whose elements do not: of the same parameter rows at different places of a row, or of the
+    same matrix rows at different columns."""
+    if t.element_size() != u.element_size():
         return False
     size = t.element_size()
     base = min(t.data_ptr(), u.data_ptr())
-    places = []
-    for v in (t, u):
-        if (v.data_ptr() - base) % size:
-            return False
-        start = (v.data_ptr() - base) // size % s
-        n = 1 + sum((d - 1) * k for d, k in zip(v.shape[1:], v.stride()[1:]))
-        places.append((start, start + n))
-    (a, b), (c, d) = places
-    return b <= s and d <= s and (b <= c or d <= a)
+    if (t.data_ptr() - base) % size or (u.data_ptr() - base) % size:
+        return False
+    steps = [[(d, s) for d, s in zip(v.shape, v.stride()) if d > 1] for v in (t, u)]
+    for period in {s for dims in steps for _, s in dims if s > 1}:
+        # both lie in the same places of every `period` elements
+        places = []
+        for v, dims in zip((t, u), steps):
+            if any(s >= period and s % period for _, s in dims):
+                break
+            start = (v.data_ptr() - base) // size % period
+            places.append((start, start + 1 + sum((d - 1) * s for d, s in dims if s < period)))
+        else:
+            (a, b), (c, d) = places
+            if b <= period and d <= period and (b <= c or d <= a):
+                return True
+    return False
 
 
 def _ld(t):

@@ -120,3 +120,20 @@ def test_tensors_that_require_grad():
             loss.backward()
     with torch.inference_mode():
         assert torch.equal(dense.dense_forward(x, w, out=torch.empty(2, 6, 10, device="cuda")), want)
+
+
+@pytest.mark.parametrize("G", [1, 2])
+def test_results_into_columns_of_one_buffer(G):
+    """Two layers' results side by side, the second's input and residual in the same rows."""
+    x, w, v = rand((G, 9, 20), torch.float32, 1), rand((G, 20, 12), torch.float32, 2), rand((G, 12, 12), torch.float32, 3)
+    buf = torch.full((G, 9, 40), 3.0, device="cuda")
+    a, b, r = buf[:, :, :12], buf[:, :, 12:24], buf[:, :, 25:37]
+    want = dense.dense_forward(x, w)
+    want2 = dense.dense_forward(want, v, residual=r.clone(), activation="silu")
+    dense.dense_forward(x, w, out=a)
+    dense.dense_forward(a, v, residual=r, activation="silu", out=b)
+    assert torch.equal(a, want) and torch.equal(b, want2) and (buf[:, :, 24:] == 3).all()
+    g = rand((G, 8, 30), torch.float32, 4)
+    o = muon.orthogonalize(g[:, :, :14].contiguous())
+    muon.orthogonalize(g[:, :, :14], out=g[:, :, 14:28])
+    assert torch.equal(g[:, :, 14:28], o)
