@@ -23,3 +23,73 @@ def test_a_round_does_not_wait_for_the_device():
     for ci, rows in ((0, (0, 1)), (2, (3, 4, 5))):
         for r in rows:
             assert torch.equal(st.params[r], st.glob[ci])
+
+
+def test_rounds_are_the_recurrence_through_stops_and_compaction():
+    """Four rounds of hand-filled replicas against m = beta m + (before - average), u = difference + beta m, w = (1 - lr wd)
+    before - lr scale O(u) in 64 bits, each round from the device's own models; the middle coalition stops after the second,
+    which splits the runs; a batch compacted there continues with the same bits.  Tolerances: of w as for one round (2^-9 of
+    the step in the Frobenius norm and fp32's rounding of the weights); of m two roundings of its terms a round."""
+    import numpy as np
+    import torch
+    from mplc import cnn, muon
+    from mplc.fedavg import aggregation_weights
+    from test_server_muon import exact
+    lr, beta, wd = 0.05, 0.8, 0.1
+    eng = engine(server_optimizer={"name": "muon", "lr": lr, "beta": beta, "weight_decay": wd})
+    coals = [(0, 1), (2,), (1, 2, 3), (0, 3), (0, 2)]
+    whole, small = (eng.trainer.prepare(coals, 1) for _ in range(2))
+    live = list(range(len(coals)))
+    place = {ci: ci for ci in live}  # coalition -> its row in `small`
+    mats = muon.ServerMuon.matrices(cnn.KERAS_LAYERS)
+    mom = {ci: [np.zeros((r, c)) for _, r, c in mats] for ci in live}
+    size = {ci: [np.zeros((r, c)) for _, r, c in mats] for ci in live}
+
+    def fill(st, ci, row, n):
+        """The round's partner models: the coalition's model and a change that only the round, the coalition and the member set."""
+        for k in range(st.coal_first[row + 1] - st.coal_first[row]):
+            gen = torch.Generator().manual_seed(1000 * n + 10 * ci + k)
+            st.params[st.coal_first[row] + k] = st.glob[row] + 0.01 * torch.randn(cnn.STRIDE, generator=gen).cuda()
+
+    for n in range(4):
+        if n == 2:  # coalition 2 stops: (0, 1) before it, (0, 3) and (0, 2) behind it
+            for st in (whole, small):
+                st.stop([2])
+            live = [ci for ci in live if ci != 2]
+            stood = whole.glob[2].clone(), whole.server_m[2].clone()
+            small = eng.trainer._compact(small, live)
+            place = {ci: i for i, ci in enumerate(live)}
+        before = whole.glob.clone()
+        for ci in live:
+            fill(whole, ci, ci, n)
+            fill(small, ci, place[ci], n)
+        for st in (whole, small):
+            st.aggregate()
+        for ci in live:
+            if len(coals[ci]) == 1:
+                continue
+            for t in ("glob", "server_m"):
+                assert torch.equal(getattr(whole, t)[ci], getattr(small, t)[place[ci]]), (n, ci, t)
+            rows = whole.params[whole.coal_first[ci]:whole.coal_first[ci + 1]]
+            assert all(torch.equal(r, whole.glob[ci]) for r in rows)
+            w, scale = aggregation_weights([eng.partner_sizes[p] for p in coals[ci]], eng.aggregation)
+            members = []
+            for k in range(len(coals[ci])):
+                gen = torch.Generator().manual_seed(1000 * n + 10 * ci + k)
+                members.append((before[ci] + 0.01 * torch.randn(cnn.STRIDE, generator=gen).cuda()).cpu().numpy())
+            avg = (sum(m.astype(np.float64) * v for m, v in zip(members, w)) / scale).astype(np.float32)
+            b, got, m_got = (t[ci].cpu().numpy() for t in (before, whole.glob, whole.server_m))
+            for off, shape in cnn.KERAS_LAYERS:
+                if len(shape) == 1:
+                    assert np.array_equal(got[off:off + shape[0]], avg[off:off + shape[0]])
+            for i, (off, r, c) in enumerate(mats):
+                b64, a64, g64, m64 = (v[off:off + r * c].reshape(r, c).astype(np.float64) for v in (b, avg, got, m_got))
+                d = (b64 - a64).astype(np.float32).astype(np.float64)
+                mom[ci][i] = beta * mom[ci][i] + d
+                size[ci][i] = beta * size[ci][i] + np.abs(d)
+                assert (np.abs(m64 - mom[ci][i]) <= (n + 1) * 2.0 ** -22 * size[ci][i] + 2.0 ** -30).all(), (n, ci, i)
+                step = lr * muon.update_scale(r, c) * exact(d + beta * mom[ci][i])
+                want = (1 - lr * wd) * b64 - step
+                err = np.linalg.norm(g64 - want)
+                assert err <= 2.0 ** -9 * np.linalg.norm(step) + 2.0 ** -22 * np.linalg.norm(want), (n, ci, i, err)
+    assert torch.equal(whole.glob[2], stood[0]) and torch.equal(whole.server_m[2], stood[1])
