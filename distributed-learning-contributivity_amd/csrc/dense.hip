@@ -223,12 +223,13 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
   }
 }
 
-// Bound by the weights' stream: 81 x 2 rows, 3256 -> 653 fp16, 344 MB in 107 us, 3.2 TB/s from unaligned rows.
-// Few rows (ROWS at most): the weights stream through once and the product is a few multiply-adds per element, so there
-// is nothing for the matrix cores to share.  A wave takes 256 columns, 4 a lane, and every fourth group of 8 r; a row's
-// x[r] is one value for the whole wave, from LDS.  Each lane keeps 8 loads of w on their way.
-template <Kind K, int ROWS> __global__ __launch_bounds__(256) void rows_kernel(const Product p, const Epilogue e) {
-  typedef typename Elem<K>::T T;
+// Bound by the weights' stream: 8 x 1 row, 4096 -> 4097, 538 MB in 108 us, 5.0 TB/s from unaligned rows.
+// Few rows (ROWS at most) of large fp32 weights that no 16-byte load takes whole: the weights stream through once and the
+// product is a few multiply-adds per element, so there is nothing for the matrix cores to share.  A wave takes 256 columns, 4
+// a lane, and every fourth group of 8 r; a row's x[r] is one value for the whole wave, from LDS.  Each lane keeps 8 loads of w
+// on their way.
+template <int ROWS> __global__ __launch_bounds__(256) void rows_kernel(const Product p, const Epilogue e) {
+  constexpr Kind K = F32;
   constexpr int STEP = 512;  // r whose x is staged at a time
   __shared__ float xs[STEP][ROWS];
   __shared__ f32x4 part[4][ROWS][64];
@@ -239,8 +240,8 @@ template <Kind K, int ROWS> __global__ __launch_bounds__(256) void rows_kernel(c
   if (M == 0) return;
   const int c = (tn * 64 + lane) * 4, in = c < p.n ? c : (p.n - 1) & ~3;
   const int first = split * p.per_split * unit_of(K), last = min(p.r, first + p.per_split * unit_of(K));
-  const T* x = reinterpret_cast<const T*>(p.a) + g * p.a_stride;
-  const T* w = reinterpret_cast<const T*>(p.b) + g * p.b_stride + in;
+  const float* x = reinterpret_cast<const float*>(p.a) + g * p.a_stride;
+  const float* w = reinterpret_cast<const float*>(p.b) + g * p.b_stride + in;
   f32x4 acc[ROWS];
 #pragma unroll
   for (int m = 0; m < ROWS; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -250,7 +251,7 @@ template <Kind K, int ROWS> __global__ __launch_bounds__(256) void rows_kernel(c
       __syncthreads();
       for (int i = threadIdx.x; i < ROWS * STEP; i += 256) {
         const int m = i / STEP, r = i % STEP;
-        xs[r][m] = m < M && r < n ? to_f32<K>(x[m * p.a_ld + r0 + r]) : 0.f;
+        xs[r][m] = m < M && r < n ? x[m * p.a_ld + r0 + r] : 0.f;
       }
       __syncthreads();
       for (int r = wave * 8; r < n; r += 32) {
@@ -434,14 +435,17 @@ bool plan(const mplc_dense_t& t, Form form, Plan& out) {
   if ((c.tile == 0 || c.tile == 3) && p.nk <= 2) out.cfg = 5;
   p.splits = c.splits;
   p.per_split = c.per_split;
-  // Few rows of weights that no 16-byte load takes whole: 81 x 2 rows, 3256 -> 653 fp16 107 us against 272 on the tiles;
-  // aligned ones stream as fast through the tiles (8 x 1 row, 4096 -> 4096 bf16: 44 against 41 us).
-  if (form == FORWARD && p.m <= 8 && p.n >= 128 && p.n % (f32 ? 4 : 8) != 0) {
+  // Few rows of large fp32 weights whose rows are no whole 16 bytes.  8 x 1 row, 4096 -> 4097: 108 us against 147 on the tiles, 64
+  // x 2, 2304 -> 513: 39 against 68; 8 rows: 10 to 20 % faster.  Below 4 M weights the tiles' shorter start counts (1 x 1, 2304
+  // -> 513: 8.4 against 9.5 us).  16-bit weights stream faster through the tiles, cut rows too (81 x 2, 3256 -> 653 fp16: 77
+  // against 87 us, with 8 rows 77 against 137), and so do whole rows (8 x 1, 4096 -> 4096 fp32: 94 against 98).  Decided by
+  // sizes alone, as the workspace is: where `out` is whole 16 bytes but the base or ld is not, the tiles take them.
+  if (form == FORWARD && f32 && p.m <= 8 && p.n >= 128 && p.n % 4 != 0 && (int64_t)p.models * p.r * p.n >= 1 << 22) {
     // 256 columns a workgroup; r split until there are 4 workgroups per CU, at least 128 r each
     out.cfg = 6;
     p.tiles_m = 1;
     p.tiles_n = (int)ceil_div(p.n, 256);
-    const int64_t blocks = (int64_t)p.tiles_n * p.models, least = 128 / (f32 ? unit_of(F32) : unit_of(BF16));
+    const int64_t blocks = (int64_t)p.tiles_n * p.models, least = 128 / unit_of(F32);
     int64_t splits = ceil_div(1024, blocks > 0 ? blocks : 1);
     if (splits > p.nk / least) splits = p.nk / least;
     if (splits < 1) splits = 1;
@@ -472,11 +476,11 @@ template <Kind K, bool AA, bool BA> hipError_t launch(Plan& pl, const Epilogue& 
                  (!AA || pl.p.m % ch == 0) && (!BA || pl.p.b_cols % ch == 0);
   const dim3 grid((unsigned)pl.blocks);
   if (pl.cfg == 6) {
-    if constexpr (!AA && BA) {  // the forward product
-      if (pl.p.m <= 1) rows_kernel<K, 1><<<grid, 256, 0, s>>>(pl.p, e);
-      else if (pl.p.m <= 2) rows_kernel<K, 2><<<grid, 256, 0, s>>>(pl.p, e);
-      else if (pl.p.m <= 4) rows_kernel<K, 4><<<grid, 256, 0, s>>>(pl.p, e);
-      else rows_kernel<K, 8><<<grid, 256, 0, s>>>(pl.p, e);
+    if constexpr (!AA && BA && K == F32) {  // the forward product
+      if (pl.p.m <= 1) rows_kernel<1><<<grid, 256, 0, s>>>(pl.p, e);
+      else if (pl.p.m <= 2) rows_kernel<2><<<grid, 256, 0, s>>>(pl.p, e);
+      else if (pl.p.m <= 4) rows_kernel<4><<<grid, 256, 0, s>>>(pl.p, e);
+      else rows_kernel<8><<<grid, 256, 0, s>>>(pl.p, e);
     }
   } else if (pl.cfg == 0) product_kernel<K, AA, BA, 2, 2, 2, 2, 128, 2><<<grid, 256, 0, s>>>(pl.p, e);
   else if (pl.cfg == 1) product_kernel<K, AA, BA, 2, 2, 1, 1, 128, 3><<<grid, 256, 0, s>>>(pl.p, e);

@@ -55,3 +55,20 @@ def test_parts_of_the_same_rows_are_disjoint(G):
     assert not refused(top, bottom) and refused(top, both[:, 2:])
     half = torch.zeros(G, 6, 20, dtype=torch.bfloat16)
     assert not refused(half[:, :, :10], half[:, :, 10:])
+
+
+def test_few_rows_of_16_bit_weights_take_the_tiles_whether_cut_or_not():
+    """The split of a sum is the tiles' one, which does not know where rows end; fp32's large cut weights have one of their own."""
+    import ctypes
+    lib = dense._lib()
+
+    def split(dtype, G, B, K, N):
+        t = dense.DenseT()
+        t.n_models, t.rows, t.in_, t.out, t.dtype = G, B, K, N, dtype
+        return lib.mplc_dense_forward_workspace_bytes(ctypes.byref(t)) // (4 * G * B * N)
+    for B in (1, 2, 8):
+        for G, K, N in ((3, 9216, 397), (81, 3256, 653), (1, 4096, 1021)):
+            for dtype in (1, 2):
+                assert split(dtype, G, B, K, N) == split(dtype, G, B, K, N + 3), (dtype, G, B, K, N)
+        assert split(0, 3, B, 9216, 397) != split(0, 3, B, 9216, 400)
+        assert split(0, 1, B, 300, 129) == split(0, 1, B, 300, 132)

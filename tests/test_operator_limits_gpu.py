@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from mplc import dense, muon
-from test_dense_gpu import TYPES, check_backward, half, rand, tiny
+from test_dense_gpu import TYPES, check_backward, check_forward, half, live_rows, rand, tiny
 
 pytestmark = pytest.mark.gpu
 
@@ -137,3 +137,16 @@ def test_results_into_columns_of_one_buffer(G):
     o = muon.orthogonalize(g[:, :, :14].contiguous())
     muon.orthogonalize(g[:, :, :14], out=g[:, :, 14:28])
     assert torch.equal(g[:, :, 14:28], o)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 8])
+@pytest.mark.parametrize("G,K,N", [(3, 4100, 401), (1, 32771, 131), (200, 171, 130), (9, 4099, 129)])
+def test_few_rows_of_large_fp32_weights(G, K, N, rows):
+    """Weights of 4 M elements and more in cut rows: sums split and whole, one to many models, idle ones, rows behind the
+    counts that hold NaN, and an input shared by all."""
+    t = torch.float32
+    counts = torch.tensor([rows, 0, rows - 1, 99, -3][:G] + [rows] * max(0, G - 5), dtype=torch.int32, device="cuda")
+    x, w = rand((G, rows, K), t, 1), rand((G, K, N), t, 2, K ** -0.5)
+    x = torch.where(live_rows(G, rows, counts), x, float("nan"))
+    check_forward(x, w, rand((G, N), t, 3), rand((G, rows, N), t, 4), "gelu", counts)
+    check_forward(rand((rows, K), t, 5), w, act="none")
