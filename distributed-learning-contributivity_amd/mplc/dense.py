@@ -82,9 +82,9 @@ class _Plan:
         """Launch on torch's current stream.  same: pairs of positions that may be one and the same tensor; values:
         further fields of the struct."""
         if torch.is_grad_enabled():
-            for t, name in zip(tensors, names):
+            for t in tensors:
                 if t is not None and t.requires_grad:
-                    raise ValueError(f"{name} requires grad, and the batched operators record no graph for it: call them under "
+                    raise ValueError(f"{names[[u is t for u in tensors].index(True)]} requires grad, and the batched operators record no graph for it: call them under "
                                      "torch.no_grad() or with detached tensors")
         p = [0 if t is None else t.data_ptr() for t in tensors]
         _no_overlap(tensors, names, p, self.spans, self.outs, self.ins, same)
@@ -104,7 +104,8 @@ class _Plan:
                 status = self.fn(ctypes.byref(st), _raw_stream(self.index))
         if status:
             _native.check(status, self.name)
-        torch.autograd.graph.increment_version([tensors[i] for i in self.outs])  # written behind torch's back
+        for i in self.outs:  # written behind torch's back
+            torch._C._increment_version((tensors[i],))
 
 
 def _raw_stream(index):
