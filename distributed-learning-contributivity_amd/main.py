@@ -65,8 +65,7 @@ def main(argv=None):
             df["random_state"] = i
             df["scenario_id"] = scenario_id
             if _rank() == 0:
-                with open(experiment_path / "results.csv", "a") as f:
-                    df.to_csv(f, header=f.tell() == 0, index=False)
+                utils.append_results(experiment_path / "results.csv", df)
                 utils.logger.info(f"Results saved to {os.path.relpath(experiment_path)}/results.csv")
     return 0
 

@@ -7,8 +7,10 @@ YAML(typ='safe'); same result on these plain documents), logging goes through th
 there is no TensorFlow GPU setup (init_gpu_config reports the HIP device instead).
 """
 import argparse
+import csv
 import datetime
 import logging
+import os
 import sys
 from itertools import product
 from pathlib import Path
@@ -86,6 +88,25 @@ def init_result_folder(yaml_filepath, cfg, root=None):
 
 def get_config_from_file(config_filepath, root=None):
     return init_result_folder(config_filepath, load_cfg(config_filepath), root)
+
+
+def append_results(path, df):
+    """df's rows at the end of the results CSV, in the order of its header (written by the first rows).  Scenarios of one
+    experiment may differ in their columns (server_optimizer, synthetic_data, the contributivity methods'): what a row does
+    not have stays empty, and columns that the file lacks are added to it."""
+    path = Path(path)
+    header, old = [], []
+    if path.exists() and path.stat().st_size:
+        with open(path, newline="") as f:
+            header, *old = csv.reader(f)
+    new = [c for c in df.columns if c not in header]
+    if header and new:
+        part = path.with_name(path.name + ".part")
+        with open(part, "w", newline="") as f:
+            csv.writer(f, lineterminator="\n").writerows([header + new] + [r + [""] * len(new) for r in old])
+        os.replace(part, path)
+    with open(path, "a", newline="") as f:
+        df.reindex(columns=header + new).to_csv(f, header=not header, index=False)
 
 
 def parse_command_line_arguments(argv=None):
