@@ -31,6 +31,8 @@ ARCH = "gfx950"
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-I", INCLUDE, "-I", CSRC,
           "-Wno-unused-result", "-munsafe-fp-atomics", "-ffp-contract=on",
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
 def _deps(src):
     hdrs = glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(INCLUDE, "*.h"))
     return [src] + hdrs

@@ -11,7 +11,10 @@
 // sums go through the workspace and a second kernel adds them in order and applies the epilogue.
 //
 // act'(z) needs dz as an operand of two products: one pass computes it, rounds it to the operands' type and sums its
-// columns (db) on the way, in fp32, per 64 rows, the blocks of rows added in order.
+// columns (db) on the way, in fp32, per 64 rows, the blocks of rows added in order.  The rounding is a choice: a 16-bit matrix
+// instruction takes 16-bit operands, and a second plane for the rest of dz would double both products (8192 x 4096 x 4096 bf16:
+// 520 us more beside 990).  It raises the error of 16-bit dx and dw from that of their own rounding alone, 1.7e-3 in bf16 and
+// 2.1e-4 in fp16, to 2.3e-3 and 2.9e-4 (Frobenius norm); z stays fp32, as its rounding would enter dz through act' as well.
 #include <math.h>
 
 #include "mma.h"
@@ -150,8 +153,10 @@ __device__ __forceinline__ void tile_of(int idx, int tm, int tn, int& m, int& n)
 
 constexpr int unit_of(Kind k) { return k == F32 ? 32 : 64; }  // what a split takes whole numbers of
 
-// One tile of a product, or of a split of its sum.  Bound by the matrix cores where there are tiles for all CUs: 8192 x
-// 4096 x 4096 bf16 on 256 x 256 tiles 1037 / 1112 / 1118 TFLOP/s (forward / dx / dw), fp32 on 128 x 128 about 134.
+// One tile of a product, or of a split of its sum.  Bound by the matrix cores where there are tiles for all CUs.  8192 x 4096 x
+// 4096 bf16 on 256 x 256 tiles, products alone: 285 / 260 / 263 us (forward / dx / dw), 960 to 1060 TFLOP/s.  In a training
+// step with gelu, residual and z: 371 / 266 / 283 us, 740 / 1035 / 970 TFLOP/s - with one workgroup per CU nothing hides the
+// forward's epilogue.  fp32 on 128 x 128: 130 TFLOP/s.
 template <Kind K, bool AA, bool BA, int WM, int WN, int FM, int FN, int BKB, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, const Epilogue e) {
   typedef typename Elem<K>::T T;
@@ -314,8 +319,8 @@ template <Kind K> __global__ __launch_bounds__(256) void join_kernel(const Produ
 constexpr int DZ_ROWS = 64;  // rows summed by one workgroup
 
 // dz = dy act'(z) and the sums of its columns over DZ_ROWS rows.  A wave takes LANES groups of 4 columns of 64 / LANES
-// rows at a time (a narrow matrix would leave lanes idle), 4 such passes in flight.  Bound by HBM: 24 x 1023 x 1027 fp16,
-// gelu, 201 MB in 52 us, 3.9 TB/s.
+// rows at a time (a narrow matrix would leave lanes idle), 4 such passes in flight.  Bound by HBM: 8192 x 4096 bf16,
+// gelu, 268 MB in 61 us, 4.4 TB/s.
 template <Kind K, int LANES>
 __global__ __launch_bounds__(256) void dz_kernel(const void* dy_, int64_t dy_stride, int64_t dy_ld, const float* z,
                                                  int64_t z_stride, int64_t z_ld, int act, int rows, int n,
@@ -431,7 +436,7 @@ bool plan(const mplc_dense_t& t, Form form, Plan& out) {
   const Choice c = choose(f32 ? SHAPES_F32 : SHAPES_16, 5, p.models, p.m, p.n, (int64_t)p.r * p.segments, units, true);
   out.cfg = c.tile;
   // A short sum is bound by its operands' latency and its result's stores: tiles of half the length leave LDS for three
-  // workgroups per CU (45 x 9216 x 128 from 51 rows: 103 us against 142).
+  // workgroups per CU (45 x 9216 x 128 from 51 rows: fp32 106 us against 118, fp16 47 against 92).
   if ((c.tile == 0 || c.tile == 3) && p.nk <= 2) out.cfg = 5;
   p.splits = c.splits;
   p.per_split = c.per_split;

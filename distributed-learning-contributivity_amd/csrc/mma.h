@@ -430,8 +430,7 @@ struct Block {
   }
   // One tile's products.  The fragments of step ks + 1 are on their way while the matrix cores work on step ks, across
   // the tile's end too: turn() - called once every read of this tile has arrived - makes the next tile's LDS ready and
-  // returns it (nullptr: no more), so neither its barrier nor its first reads leave the matrix cores idle.  (Reads at
-  // the start of each tile, after the barrier: 40 % of the cycles busy at 256 x 256.)
+  // returns it (nullptr: no more), so neither its barrier nor its first reads leave the matrix cores idle.
   static constexpr int KS = BKB / 32;
   static constexpr bool PIPE = PL * (FM + FN) <= 8;  // registers for two sets of fragments
   static_assert(KS % 2 == 0, "the sets alternate");

@@ -270,8 +270,10 @@ __device__ __forceinline__ void lower_tile(int i, int& tm, int& tn) {
   tn = i - tm * (tm + 1) / 2;
 }
 
-// GRAM: both operands are X and the sum runs over its rows.  Bound by the latency of a tile's step where the k x k products
-// give a CU one workgroup (2 x 2048 x 2048, five steps: 1.47 ms, 234 TFLOP/s of 341), by fp16's rate / 3 where there are more.
+// GRAM: both operands are X and the sum runs over its rows.  Bound by the latency of a tile's step and the two epilogues of a
+// mirrored tile where the k x k products give a CU one workgroup: 16 x 512^3 takes 22 to 29 us, 3 x 777^3 16 to 18, the matrix cores
+// busy 17 to 27 % of the CUs' cycles.  2 x 2048 x 2048, five steps: 1.46 ms, 236 TFLOP/s of the 341 that split fp16 allows,
+// busy 34 to 57 %.
 template <Kind K, bool GRAM, Epi E, int WM, int WN, int FM, int FN, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Prod p) {
   typedef Block<F16, GRAM, GRAM, WM, WN, FM, FN, 64, 2, STAGES> B;
@@ -593,8 +595,9 @@ template <Kind K, int KT, Epi E> __global__ __launch_bounds__(256) void small_ke
 // ------------------------------------------------------------------------------------------ narrow matrices: k <= 128
 // U is read three times and nothing of its size but the result is written: the Gram matrix of U itself (whose trace is
 // |U|^2: no pass for the norm), the Gram matrix of U Q1 formed on the way, and the result U (Q1 Q2).  What is between runs
-// on one workgroup per model with all k x k matrices in LDS.  Bound by HBM: 128 KB of matrix per workgroup need 1.2 to
-// 2.3 thousand cycles of matrix instructions and 7.7 thousand of HBM.
+// on one workgroup per model with all k x k matrices in LDS.  45 x 9216 x 128 fp32: 68, 127 and 103 us, where their bytes at a
+// copy's rate or their products need 44, 60 and 89.  A workgroup alone on its CU passes three or four barriers per piece
+// of rows with nothing to fill them, and the second pass spends 47 % of its LDS cycles in bank conflicts (Y, read across).
 // KP: k padded to 64 or 128; a workgroup of 8 waves takes TR = 16384 / KP rows l of X at a time, the next ones on their
 // way in registers.  TALL: L = rows.  Before |U| is known, a workgroup scales by a power of two that it raises (with what
 // it has summed) when a larger value comes: split fp16 holds any range.
@@ -967,7 +970,7 @@ __global__ __launch_bounds__(NARROW_THREADS) void narrow_apply_kernel(const Narr
   if constexpr (GRAM) gt.finish(xs, p.partial + ((int64_t)g * p.chunks + chunk) * (Gt::TILES * 1024));
 }
 
-// The steps of a phase on one workgroup: 8 or 5 products that wait for one another, 29 us for k = 128 whatever the batch
+// The steps of a phase on one workgroup: 8 or 5 products that wait for one another, 24 to 33 us for k = 128 whatever the batch
 // up to 256 models.  Matrices live in registers (as the matrix instruction leaves them) and, as
 // planes, in the two places of LDS when they are operands.
 struct Chain {
