@@ -169,7 +169,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
   b /= tiles;
   const int split = (int)(b % p.splits), g = (int)(b / p.splits);
   const int m0 = tm * B::BM, n0 = tn * B::BN;
-  const bool seg = p.joined;
+  const bool seg = !AA && !BA && p.joined;  // dx
   const int cnt = seg ? p.m : count_of(p.counts, g, p.count_is_r ? p.r : p.m);
   const int M = p.count_is_r ? p.m : cnt, R = p.count_is_r ? cnt : p.r;
   if (m0 >= M) return;
@@ -198,11 +198,19 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const Product p, 
     if (p.aligned && p.counts == nullptr && R % B::BK == 0) {
       if (from < to) blk.ring(lds, m0, n0, nk, from, to, at);
     } else {
-      blk.through_registers(lds, m0, n0, nk, from, to, [&](int s, Operand<T>& a, Operand<T>& o, int& r0, int& rend) {
+      auto piece = [&](int s, Operand<T>& a, Operand<T>& o, int& r0, int& rend) {
         at(s, a, o, r0);
         rend = R;
         return count_of(p.counts, s, p.m);
-      });
+      };
+      blk.through_registers(lds, m0, n0, nk, from, to, piece);
+      // A zero in the place of a row behind a count, times an infinite or NaN weight, is NaN: once more, row by row.  (The
+      // tiles of short sums would lose a workgroup per CU to its registers; with counts they are not taken.)
+      if constexpr (BKB != 64)
+        if (p.counts != nullptr && blk.not_finite(lds)) {
+          blk.clear();
+          blk.masked(lds, m0, n0, nk, from, to, piece);
+        }
     }
   } else {
     const Operand<T> a = {pa, p.a_ld, M}, o = {pb, p.b_ld, BA ? p.b_cols : p.n};
@@ -437,7 +445,7 @@ bool plan(const mplc_dense_t& t, Form form, Plan& out) {
   out.cfg = c.tile;
   // A short sum is bound by its operands' latency and its result's stores: tiles of half the length leave LDS for three
   // workgroups per CU (45 x 9216 x 128 from 51 rows: fp32 106 us against 118, fp16 47 against 92).
-  if ((c.tile == 0 || c.tile == 3) && p.nk <= 2) out.cfg = 5;
+  if ((c.tile == 0 || c.tile == 3) && p.nk <= 2 && !(p.joined && p.counts)) out.cfg = 5;
   p.splits = c.splits;
   p.per_split = c.per_split;
   // Few rows of large fp32 weights whose rows are no whole 16 bytes.  8 x 1 row, 4096 -> 4097: 108 us against 147 on the tiles, 64

@@ -578,7 +578,7 @@ struct Block {
   }
 
   // The same through registers, pieces of n tiles of which the last may be cut: at(s, A, B, r0, rend) returns how many
-  // rows of A take part in piece s (the others contribute nothing).
+  // rows of A take part in piece s (the others are zeros, and contribute nothing where B is finite).
   template <typename At>
   __device__ __forceinline__ void through_registers(char* lds, int m0, int n0, int n, int64_t from, int64_t to, At at) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -636,6 +636,68 @@ struct Block {
       });
     }
     __syncthreads();
+  }
+
+  // whether any of the workgroup's sums is not finite
+  __device__ __forceinline__ bool not_finite(char* lds) const {
+    bool bad = false;
+    each_pair([&](int i, int j) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) bad |= !(fabsf(acc[i][j][e]) < INFINITY);
+    });
+    int* any = reinterpret_cast<int*>(lds);
+    if (threadIdx.x == 0) *any = 0;
+    __syncthreads();
+    if (bad) *any = 1;
+    __syncthreads();
+    const bool result = *any != 0;
+    __syncthreads();
+    return result;
+  }
+
+  // The sum of through_registers() in the same order, rows that take no part in a piece left as they are whatever B holds:
+  // nothing is read ahead, and each matrix instruction's result is taken row by row.
+  template <typename At>
+  __device__ __forceinline__ void masked(char* lds, int m0, int n0, int n, int64_t from, int64_t to, At at) {
+    static_assert(PL == 1, "one plane");
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave / WN, wn = wave % WN;
+    if (n <= 0) return;
+    for (int64_t pos = from; pos < to; ++pos) {
+      Operand<T> A, B;
+      int r0, rend;
+      const int s = (int)(pos / n), t = (int)(pos - (int64_t)s * n);
+      const int rows = at(s, A, B, r0, rend), left = rend - r0 - t * BK;
+      if (rows <= m0) continue;
+      {
+        TA ta;
+        typename TA::Regs ra;
+        ta.seek(A, m0, r0 + t * BK, tid);
+        ta.load(ra, left, TA::columns(m0, A.rows), A.ld, rend, m0, rows, rows < min(A.rows, m0 + BM), tid);
+        ta.store(ra, lds, tid);
+      }
+      {
+        TB tb;
+        typename TB::Regs rb;
+        tb.seek(B, n0, r0 + t * BK, tid);
+        tb.load(rb, left, TB::columns(n0, B.rows), B.ld, rend, n0, 0, false, tid);
+        tb.store(rb, lds + TA::BYTES, tid);
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int ks = 0; ks < KS; ++ks)
+        each_pair([&](int i, int j) {
+          const u32x4 a = TA::frag(lds, 0, (wm * FM + i) * 32, ks, lane);
+          const u32x4 b = TB::frag(lds + TA::BYTES, 0, (wn * FN + j) * 32, ks, lane);
+          f32x16 d = acc[i][j];
+#pragma unroll
+          for (int e = 0; e < (K == F32 ? 4 : 1); ++e) mfma<K>(d, b, a, e);
+          const bool part = m0 + (wm * FM + i) * 32 + (lane & 31) < rows;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] = part ? d[e] : acc[i][j][e];
+        });
+      __syncthreads();
+    }
   }
 
   // the first of the columns, from n0, that each_row() gives this lane

@@ -150,3 +150,29 @@ def test_few_rows_of_large_fp32_weights(G, K, N, rows):
     x = torch.where(live_rows(G, rows, counts), x, float("nan"))
     check_forward(x, w, rand((G, N), t, 3), rand((G, rows, N), t, 4), "gelu", counts)
     check_forward(rand((rows, K), t, 5), w, act="none")
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("B,K,N,pad", [(40, 33, 45, 0), (130, 64, 128, 0), (130, 60, 128, 4), (5, 40, 9000, 0), (300, 520, 264, 0),
+                                       (700, 1030, 96, 0), (2048, 2304, 512, 0)])
+def test_shared_gradient_beside_models_that_are_not_finite(B, K, N, pad, dtype):
+    """A shared input's dx sums each row over the models that have it: a model that has no row there, idle or behind its
+    count, adds nothing, be its weights infinite or NaN.  Rows that such a model has are not finite."""
+    t = TYPES[dtype]
+    counts = torch.tensor([B - 2, 0, B, 1, -3, B // 2, 2 * B], dtype=torch.int32, device="cuda")
+    G = len(counts)
+    live = live_rows(G, B, counts)
+    x = rand((B, K + pad), t, 1)[:, :K]
+    w = rand((G, K, N + pad), t, 2, 0.2)[:, :, :N]
+    dout, pre = rand((G, B, N), t, 3), rand((G, B, N), torch.float32, 4)
+    dout, pre = torch.where(live, dout, float("nan")), torch.where(live, pre, float("inf"))
+    for act in ("none", "gelu"):
+        want, _, _ = check_backward(dout, x, w, pre, act, counts)
+        bad = w.clone()
+        bad[1], bad[4] = float("nan"), float("inf")
+        dx = torch.full((B, K), 5.0, dtype=t, device="cuda")
+        got, _, _ = dense.dense_backward(dout, x, bad, preact=pre, activation=act, counts=counts, need=("dx",), dx=dx)
+        assert got is dx and torch.equal(got, want)
+        bad[3], bad[5, :, 0] = float("inf"), float("nan")
+        got, _, _ = dense.dense_backward(dout, x, bad, preact=pre, activation=act, counts=counts, need=("dx",))
+        assert torch.equal(got[B // 2:], want[B // 2:]) and got[:B // 2].isnan().all()
