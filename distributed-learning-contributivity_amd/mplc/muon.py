@@ -3,7 +3,8 @@
 ``orthogonalize`` brings the singular values of every matrix of a batch near one by Newton-Schulz products;
 ``muon_step`` is the Muon update of weights kept as [in][out] matrices, for instance views into the models' parameter rows
 (``glob[:, off:off + k * n].view(C, k, n)``).  Beside mplc.fedavg: the engine uses it as the server's optimizer after a
-round's average (``CoalitionEngine(server_optimizer=...)``).  Work goes to torch's current stream of the device.
+round's average (``CoalitionEngine(server_optimizer=...)``).  Work goes to torch's current stream of the device.  No autograd
+graph is recorded: in grad mode, tensors that require grad are refused.
 """
 import ctypes
 import math

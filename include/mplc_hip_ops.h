@@ -42,7 +42,8 @@ extern "C" {
  * model's count are neither read nor written.
  * Backward, from dy and z (z is read only for an activation):
  *   dz = dy act'(z),  dx = dz w^T (x_shared: summed over the models),  dw = x^T dz,  db = sum over the rows of dz
- * A row of a shared x's dx that no model reaches gets 0.  act'(0) = 0 for relu.  The gradient of the residual is dy.  Each of dx, dw, db may be NULL (not wanted).  A model
+ * A model adds nothing to the rows of a shared x's dx behind its count, whatever its weights hold; a row that no model
+ * reaches gets 0.  act'(0) = 0 for relu.  The gradient of the residual is dy.  Each of dx, dw, db may be NULL (not wanted).  A model
  * whose count is 0 gets dw = db = 0.  Where an activation is differentiated, dz enters the two products rounded to
  * dtype; db is summed before that rounding.
  * ---------------------------------------------------------------------------------------------- */
