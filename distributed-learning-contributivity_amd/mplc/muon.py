@@ -18,6 +18,7 @@ from .dense import _PLANS, DTYPES, _Plan, _ld, _place, _remember, _sig, _tensor,
 # a s + b s^3 + c s^5 per step: takes singular values of 0.01 .. 1 to about 0.7 .. 1.2 in five steps
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 STEPS = 5
+MAX_FLOAT = 3.4e38
 
 
 class MuonT(ctypes.Structure):
@@ -178,7 +179,7 @@ def muon_step(w, grad, momentum, lr, beta=0.95, nesterov=True, weight_decay=0.0,
     rows, cols = grad.shape[-2:]
     scale = update_scale(rows, cols) if scale is None else float(scale)
     lr, beta, weight_decay = float(lr), float(beta), float(weight_decay)
-    if not math.isfinite(lr * scale) or not math.isfinite(beta) or not math.isfinite(lr * weight_decay):
+    if not all(abs(v) < MAX_FLOAT for v in (lr, lr * scale, beta, weight_decay, lr * weight_decay, scale)):  # as fp32, and not NaN
         raise ValueError(f"lr, beta, weight_decay and scale must be finite: {lr}, {beta}, {weight_decay}, {scale}")
     if plan.models:
         plan.run((w, momentum, grad), ("w", "momentum", "grad"), values=(

@@ -176,3 +176,16 @@ def test_shared_gradient_beside_models_that_are_not_finite(B, K, N, pad, dtype):
         bad[3], bad[5, :, 0] = float("inf"), float("nan")
         got, _, _ = dense.dense_backward(dout, x, bad, preact=pre, activation=act, counts=counts, need=("dx",))
         assert torch.equal(got[B // 2:], want[B // 2:]) and got[:B // 2].isnan().all()
+
+
+def test_step_sizes_that_are_not_finite_in_fp32():
+    """Refused before anything is written."""
+    w, g, m = rand((2, 6, 8), torch.float32, 1), rand((2, 6, 8), torch.float32, 2), rand((2, 6, 8), torch.float32, 3)
+    keep = w.clone(), m.clone()
+    nan, big = float("nan"), 1e39
+    for kw in (dict(lr=big), dict(lr=nan), dict(lr=-big), dict(lr=0.0, scale=big), dict(lr=1e30, scale=1e30), dict(lr=0.1, beta=big),
+               dict(lr=0.1, beta=nan), dict(lr=0.1, weight_decay=big), dict(lr=0.0, weight_decay=float("inf")),
+               dict(lr=1e30, weight_decay=1e30)):
+        with pytest.raises(ValueError, match="finite"):
+            muon.muon_step(w, g, m, **kw)
+    assert torch.equal(w, keep[0]) and torch.equal(m, keep[1])
