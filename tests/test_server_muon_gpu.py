@@ -93,3 +93,46 @@ def test_rounds_are_the_recurrence_through_stops_and_compaction():
                 err = np.linalg.norm(g64 - want)
                 assert err <= 2.0 ** -9 * np.linalg.norm(step) + 2.0 ** -22 * np.linalg.norm(want), (n, ci, i, err)
     assert torch.equal(whole.glob[2], stood[0]) and torch.equal(whole.server_m[2], stood[1])
+
+
+def test_two_streams_give_the_values_of_one():
+    """CIFAR10's default of two lockstep batches at once: momenta, workspaces and averages of one do not meet the other's."""
+    import itertools
+    import numpy as np
+    from mplc.dataset import Cifar10
+    from mplc.engine import CoalitionEngine
+    from mplc.scenario import Scenario
+    ds = Cifar10(synthetic=True, n_train=3000, n_test=500, signal=0.3)
+    sc = Scenario(6, [0.1, 0.15, 0.15, 0.2, 0.2, 0.2], dataset=ds, epoch_count=1, minibatch_count=3, is_early_stopping=False,
+                  server_optimizer="muon").provision()
+    eng = CoalitionEngine.for_scenario(sc)
+    coals = [c for k in range(1, 7) for c in itertools.combinations(range(6), k)][:40]
+    eng.concurrent_batches = 1
+    one = eng.evaluate(coals)
+    eng.concurrent_batches = 2
+    assert eng._concurrent_ok(coals, eng.epoch_count, eng.is_early_stopping, None, False)
+    assert np.array_equal(one, eng.evaluate(coals))
+    assert len(np.unique(one)) > 5
+
+
+def test_early_stopping_with_and_without_compaction():
+    """Coalitions that stop at different epochs: the same values, epochs and traces whether the batch is kept whole or
+    compacted whenever a replica is idle."""
+    from itertools import combinations
+    import numpy as np
+    from mplc.dataset import ArrayDataset, digits_as_mnist
+    from mplc.engine import CoalitionEngine
+    from mplc.scenario import Scenario
+    from test_compaction_gpu import _both, _check
+    x, y = digits_as_mnist()
+    y = np.argmax(np.array(y), 1)
+    rng = np.random.default_rng(0)
+    flip = rng.random(1500) < 0.6
+    y[np.arange(1500)[flip]] = rng.integers(0, 10, size=int(flip.sum()))
+    ds = ArrayDataset(x[:1500], y[:1500], x[1500:], y[1500:])
+    sc = Scenario(4, [0.1, 0.2, 0.3, 0.4], dataset=ds, minibatch_count=2, gradient_updates_per_pass_count=16,
+                  epoch_count=24, is_early_stopping=True, server_optimizer={"name": "muon", "lr": 0.01}).provision()
+    eng = CoalitionEngine.for_scenario(sc, memory_budget_bytes=8 << 30, eval_budget_bytes=1 << 30)
+    out = _both(eng, [c for r in range(1, 5) for c in combinations(range(4), r)])
+    print(out[0.0][0]["epochs_done"], out[1.0][1])
+    _check(out)
